@@ -372,6 +372,73 @@ int zrnn_beam_decode_batch_sharded(zrnn_model* m, zrnn_comm* c, const int* src_i
                                    int longest_sent, int* out_ids, int* out_len, float* out_score);
 int zrnn_model_destroy(zrnn_model* m);
 
+/* ------------------------------------------------------------------------------------------
+ * Operators of a decoding step, for a host program that drives the layer objects itself (no counterparts in the reference, whose
+ * decoder runs them inside its drivers or on the host).  Their vectors may be 32-bit or 16-bit floats (zrnn_elem); sums,
+ * softmax statistics and activations are computed in 32 bits, results rounded once to the element type.  All calls are
+ * asynchronous on `stream` (of the current device), allocate nothing, keep nothing between calls and may be captured into a
+ * graph; scratch memory is the caller's `d_workspace`, of the size that the *_workspace call names for the same arguments:
+ * calls that can overlap on the GPU (other streams, other graphs) need workspaces of their own.
+ * ---------------------------------------------------------------------------------------- */
+typedef enum { ZRNN_ELEM_F32 = 0, ZRNN_ELEM_BF16 = 1, ZRNN_ELEM_F16 = 2 } zrnn_elem;
+
+/* Source memory in 4 bits.  The states that attention reads (one vector of `heads` x d elements per slot and source column; heads = 1,
+ * d = H for this library's models) in groups of 32 elements of a head (the last group of a head is filled with zeros):
+ *   s = fp16(min(a * (1/7), 9352)), a the largest magnitude of the group;  q = x / s rounded to the nearest integer, ties to
+ *   even, within -7 .. 7;  the element's value is then q * s rounded to fp16.
+ * d_codes [B][S_cap][heads][groups * 16] bytes: q + 8 in 4 bits, the even element of a pair in the low ones; d_scales
+ * [B][S_cap][heads][groups] fp16; groups = ceil(d / 32).  4.5 bits per element.  A group of zeros has s = 0; one that holds an
+ * infinity or a NaN has s = NaN, and a column that attends to it gets NaN; magnitudes beyond 65472 saturate.
+ * zrnn_memory4_sizes gives the bytes of d_codes (16-byte aligned) and the number of scales. */
+int zrnn_memory4_sizes(int B, int S_cap, int heads, int d, size_t* code_bytes, size_t* n_scales);
+/* Writes slots slot0 .. slot0 + S - 1 of every column from d_x (element i of column b in slot s at s * ld_slot + b * ld_col + i);
+ * other slots stay as they are, so a memory can be filled slot by slot. */
+int zrnn_memory4_pack(int elem, const void* d_x, long long ld_slot, long long ld_col, int S, int B, int heads, int d, int slot0,
+                      int S_cap, void* d_codes, void* d_scales, void* stream);
+/* Reads slots back: d_out [B][S][heads][d], the values rounded to the element type. */
+int zrnn_memory4_unpack(int elem, const void* d_codes, const void* d_scales, int B, int S_cap, int heads, int d, int slot0, int S,
+                        void* d_out, void* stream);
+/* Global dot attention over the memory: target column c (at d_q + c * ld_q, heads x d elements) of B * cols_per_sentence
+ * belongs to source column c / cols_per_sentence, and per head
+ *   out = sum_s softmax_s(scale * q . v_s) v_s   over the slots offset <= s < offset + len of that source column
+ * (slots outside the memory do not count; d_offset NULL: 0).  Whatever other slots hold is not looked at.  A column without
+ * slots, or with d_mask01[c] == 0 (NULL: all 1), gets zeros.  d <= 1024.  d_out must not overlap d_q. */
+int zrnn_memory4_attend_workspace(int B, int cols_per_sentence, int S_cap, int heads, int d, size_t* bytes);
+int zrnn_memory4_attend(int elem, const void* d_codes, const void* d_scales, int B, int S_cap, int heads, int d, const int* d_len,
+                        const int* d_offset, const void* d_q, long long ld_q, int cols_per_sentence, const int* d_mask01, float scale,
+                        void* d_out, long long ld_out, void* d_workspace, size_t workspace_bytes, void* stream);
+
+/* Y = act(W X + b) + R for n_cols columns: X (K x n_cols), Y and R (n_rows x n_cols) column-major as all activations; the K
+ * weights of an output are contiguous and those of the next ldw further (W^T column-major).  d_bias (n_rows, fp32) and
+ * d_residual may be NULL; d_residual may be d_Y itself (with ldr == ldy).  ZRNN_ELEM_F32 is accurate to fp32 (3xTF32 or FMA),
+ * the 16-bit types multiply their operands as they are.  gelu is x/2 (1 + erf(x / sqrt 2)), silu x / (1 + exp -x). */
+typedef enum {
+  ZRNN_ACT_NONE = 0, ZRNN_ACT_TANH = 1, ZRNN_ACT_SIGMOID = 2, ZRNN_ACT_RELU = 3, ZRNN_ACT_GELU = 4, ZRNN_ACT_SILU = 5
+} zrnn_activation;
+int zrnn_linear_workspace(int elem, int n_rows, int n_cols, int K, const void* d_W, long long ldw, const void* d_X, long long ldx,
+                          size_t* bytes);
+int zrnn_linear(int elem, int act, int n_rows, int n_cols, int K, const void* d_W, long long ldw, const void* d_X, long long ldx,
+                const float* d_bias, const void* d_residual, long long ldr, void* d_Y, long long ldy, void* d_workspace,
+                size_t workspace_bytes, void* stream);
+
+/* The k best continuations of every sentence.  Row r = sentence * beam + j of d_logp (V values, ld apart) belongs to
+ * hypothesis j of the sentence; the candidate (j, v) is worth d_scores[r] + (d_logp[r][v] - d_lse[r]), each operation rounded
+ * to fp32 (d_lse NULL: log-probabilities).  A hypothesis with d_done[r] != 0 (NULL: none) has one candidate, (j, eos), worth
+ * d_scores[r].  A NaN or -inf is no candidate.  Outputs [n_sent][k], best first, equal ones by j and then v: value, word v, and
+ * parent = r as zrnn_beam_reorder takes it; where a sentence has fewer than k candidates: -inf, -1, -1.  k <= 64. */
+int zrnn_beam_select_workspace(int elem, int n_sent, int beam, int V, int k, size_t* bytes);
+int zrnn_beam_select(int elem, const void* d_logp, long long ld, const float* d_lse, const float* d_scores, const int* d_done,
+                     int n_sent, int beam, int V, int k, int eos, float* d_score_out, int* d_word_out, int* d_parent_out,
+                     void* d_workspace, size_t workspace_bytes, void* stream);
+/* Column c of every array becomes its column d_parent[c] (swap_states_decoding, src/Input_To_Hidden_Layer.hpp:1231-1260): array i has
+ * n_src_cols dense columns of bytes_per_col[i] bytes at d_src[i], and n_cols at d_dst[i]; d_parent[c] < 0 makes zeros.  An array
+ * whose destination is its source is reordered in place: its columns move within groups of `group` (<= 64) consecutive ones,
+ * for which a call with any such array sets n_cols == n_src_cols, a multiple of group.  A parent that is no source column
+ * (or, in place, not of the group) gives zeros (in place: leaves the column as it was), and the next synchronising call
+ * reports it.  At most 40 arrays; other overlaps are refused. */
+int zrnn_beam_reorder(int n_arrays, const void* const* d_src, void* const* d_dst, const size_t* bytes_per_col, const int* d_parent,
+                      int n_cols, int n_src_cols, int group, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

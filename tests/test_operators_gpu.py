@@ -1,0 +1,579 @@
+"""The operators of a decoding step against plain 64-bit implementations (tests/operators_ref.py).
+
+Tolerances.  eps = 2^-24 is half a step of 32 bits, h the output type's.  A sum of n products in 32 bits strays from the exact sum by
+about sqrt(n) eps times the sum of the products' magnitudes where the roundings are to nearest; a tensor core cuts its sums off
+instead, so n / 16 additions (of 16 products) may add up to n / 16 * 2 eps.  The tests allow (8 + sqrt(n) + n / 16) 2 eps.
+Attention: a score that is off by t changes a weight by a factor 1 + t, so the output by at most 2 t max|v|; the weights' sum and the
+weighted sum add as much as a sum of S products; with 16-bit operands the weights are rounded to half precision (2^-11).
+Whole numbers, codes and scales are equal.
+"""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from tests import operators_ref as ref
+
+pytestmark = pytest.mark.gpu
+EPS = 2.0 ** -24
+
+
+@pytest.fixture(scope="module")
+def api():
+    from zoph_rnn_b200 import api as a
+    return a
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def randn(g, *shape, dtype="f32"):
+    return torch.randn(shape, generator=g, device="cuda").to(ref.TYPES[dtype])
+
+
+def f64(t):
+    return t.detach().double().cpu().numpy()
+
+
+def sum_tol(n):
+    return (8 + n ** 0.5 + n / 16) * 2 * EPS
+
+
+# ------------------------------------------------------------------ memory4: pack, unpack
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("S, B, heads, d", [(1, 1, 1, 1), (1, 3, 1, 31), (5, 2, 1, 32), (7, 3, 1, 33), (3, 5, 4, 20), (50, 4, 1, 1000), (9, 2, 16, 64), (2, 3, 2, 251), (4, 1, 1, 2048)])
+def test_pack_and_unpack(api, dtype, S, B, heads, d):
+    g = gen(S + 7 * d)
+    x = randn(g, S, B, heads * d, dtype=dtype)
+    x[0, 0, : d // 2] *= 1e-3
+    m = api.memory4(B, S, d, heads=heads).pack(x)
+    codes, scales = ref.pack(f64(x), heads, d)
+    np.testing.assert_array_equal(m.scales.cpu().numpy().view(np.uint16), scales.view(np.uint16))
+    np.testing.assert_array_equal(m.codes.cpu().numpy(), codes)
+    for t in ("f32", "bf16", "f16"):
+        want = torch.from_numpy(ref.unpack(codes, scales, d)).to(ref.TYPES[t])
+        assert torch.equal(m.unpack(ref.TYPES[t]).cpu(), want)
+
+
+def test_codes_next_to_the_middle_between_two(api):
+    """Quotients that 32 bits round onto k + 1/2 from either side, and exact ties."""
+    s = np.float16(0.0123)
+    rows = []
+    for k in range(-7, 7):
+        mid = (k + 0.5) * float(s)  # exact in 32 bits
+        f = np.float32(mid)
+        rows += [f, np.nextafter(f, np.float32(-9)), np.nextafter(f, np.float32(9))]
+    x = np.zeros((1, len(rows), 32), np.float32)
+    x[0, :, 0] = rows
+    x[0, :, 1] = np.float32(7 * float(s))  # the group's largest: its scale is s
+    m = api.memory4(len(rows), 1, 32).pack(torch.from_numpy(x).cuda())
+    codes, scales = ref.pack(x.astype(np.float64), 1, 32)
+    assert (scales == s).all()
+    np.testing.assert_array_equal(m.codes.cpu().numpy(), codes)
+
+
+def test_pack_of_numbers_at_the_ends_of_the_range(api):
+    x = torch.zeros(1, 10, 64, device="cuda")
+    x[0, 0, :32] = 1e-9          # below half precision: zeros
+    x[0, 1, :32] = 3e-7          # a scale of a few steps
+    x[0, 2, :3] = torch.tensor([1e-7, -4e-7, 2e-7])
+    x[0, 3, 5] = 65504.0
+    x[0, 4, 5] = -3.0e38         # saturates
+    x[0, 5, 40] = float("inf")   # the second group only
+    x[0, 6, 3] = float("nan")
+    x[0, 7, :] = -0.0
+    x[0, 8, 0], x[0, 8, 1] = 1.0, 1e-40
+    m = api.memory4(10, 1, 64).pack(x)
+    codes, scales = ref.pack(f64(x), 1, 64)
+    np.testing.assert_array_equal(m.scales.cpu().numpy().view(np.uint16), scales.view(np.uint16))
+    np.testing.assert_array_equal(m.codes.cpu().numpy(), codes)
+    v = m.unpack().cpu().reshape(10, 64)
+    # (7 * 9352 = 65464, and half precision has steps of 32 there: 65472)
+    assert v[4, 5] == -65472 and v[5, :32].eq(0).all() and v[5, 32:].isnan().all() and v[6, :32].isnan().all() and v[9].eq(0).all()
+
+
+def test_pack_slot_by_slot_leaves_the_others(api):
+    g = gen(3)
+    x = randn(g, 6, 3, 100)
+    whole = api.memory4(3, 6, 100).pack(x)
+    m = api.memory4(3, 9, 100)
+    m.codes.fill_(77)
+    m.scales.fill_(5.0)
+    for s in (4, 0, 5, 1, 3, 2):
+        m.pack(x[s:s + 1], slot0=s + 2)
+    assert torch.equal(m.codes[:, 2:8], whole.codes) and torch.equal(m.scales[:, 2:8], whole.scales)
+    assert m.codes[:, :2].eq(77).all() and m.codes[:, 8:].eq(77).all() and m.scales[:, 8:].eq(5).all()
+    assert torch.equal(m.unpack(slot0=3, S=2), whole.unpack()[:, 1:3])
+    assert m.unpack(slot0=3, S=0).numel() == 0
+    wide = torch.randn(6, 3, 128, device="cuda")  # columns and slots further apart than they are long
+    wide[..., 9:109] = x
+    assert torch.equal(api.memory4(3, 6, 100).pack(wide[..., 9:109]).codes, whole.codes)
+    by_col = x.permute(1, 0, 2).contiguous().permute(1, 0, 2)
+    assert torch.equal(api.memory4(3, 6, 100).pack(by_col).codes, whole.codes)
+
+
+# ------------------------------------------------------------------ memory4: attend
+def attend_case(api, dtype, B, cols, S, heads, d, lens, offsets, scale=None, seed=0, mask=None, qmul=1.0):
+    g = gen(seed)
+    hs = torch.tanh(0.5 * torch.randn(S, B, heads * d, generator=g, device="cuda"))
+    q = (qmul * torch.tanh(torch.randn(B * cols, heads * d, generator=g, device="cuda"))).to(ref.TYPES[dtype])
+    m = api.memory4(B, S, d, heads=heads).pack(hs)
+    scale = (1.0 if heads == 1 else d ** -0.5) if scale is None else scale
+    ln, of = torch.tensor(lens, dtype=torch.int32, device="cuda"), torch.tensor(offsets, dtype=torch.int32, device="cuda")
+    mk = None if mask is None else torch.tensor(mask, dtype=torch.int32, device="cuda")
+    out = m.attend(q, ln, of, scale=scale, mask01=mk)
+    v = ref.unpack(m.codes.cpu().numpy(), m.scales.cpu().numpy(), d)
+    check_attend(out, v, f64(q), lens, offsets, scale, dtype, mask)
+    return m, q, ln, of, scale, out
+
+
+def check_attend(out, v, q, lens, offsets, scale, dtype, mask=None):
+    want, mag = ref.attend(v, q, lens, offsets, scale, mask)
+    B, S, heads, d = v.shape
+    vmax = np.nanmax(np.abs(v))
+    n = max([1] + [min(o + l, S) - max(o, 0) for o, l in zip(offsets, lens)])
+    tol = vmax * (2 * sum_tol(d) * mag + 4 * sum_tol(n) + (0.0 if dtype == "f32" else 2 * 2.0 ** -11))[..., None] + ref.HALF_STEP[dtype] * np.abs(want)
+    tol = np.where(mag[..., None] == 0, ref.HALF_STEP[dtype] * np.abs(want), tol)  # (columns without slots: zeros)
+    err = np.abs(f64(out).reshape(want.shape) - want)
+    assert np.isfinite(err).all() and (err <= tol).all(), (err.max(), (err / np.maximum(tol, 1e-300)).max())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("B, cols, S, heads, d", [
+    (1, 1, 1, 1, 1), (1, 12, 23, 1, 1000), (3, 5, 33, 1, 100), (2, 12, 64, 1, 512), (4, 1, 31, 1, 320), (2, 17, 65, 1, 1024), (2, 33, 40, 1, 96), (3, 2, 100, 8, 64),
+    (2, 4, 129, 4, 33), (1, 3, 700, 2, 128), (1, 16, 3000, 1, 200), (2, 3, 257, 16, 20), (1, 40, 50, 3, 251), (5, 8, 90, 1, 129), (2, 1, 4500, 1, 640)])
+def test_attend(api, dtype, B, cols, S, heads, d):
+    lens = [max(1, S - 3 * b) for b in range(B)]
+    attend_case(api, dtype, B, cols, S, heads, d, lens, [S - n for n in lens], seed=d + S)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("heads, d", [(1, 1000), (4, 64)])
+def test_attend_lengths_and_masks(api, dtype, heads, d):
+    """Empty sentences, one slot, windows at either end and in the middle of a tile, windows that stick out, masked columns."""
+    S, B, cols = 150, 10, 3
+    lens = [0, 1, 150, 1, 32, 33, 31, 400, 20, -5]
+    offs = [0, 149, 0, 0, 32, 31, 100, -7, 145, 10]
+    mask = [1] * (B * cols)
+    mask[7] = mask[8] = mask[20] = 0
+    *_, out = attend_case(api, dtype, B, cols, S, heads, d, lens, offs, mask=mask)
+    out = out.view(B, cols, -1)
+    assert out[0].eq(0).all() and out[9].eq(0).all() and out.view(B * cols, -1)[[7, 8, 20]].eq(0).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("heads, d, S", [(1, 500, 90), (8, 64, 300)])
+def test_what_lies_outside_the_window_is_not_looked_at(api, dtype, heads, d, S):
+    B, cols = 3, 4
+    lens, offs = [S - 40, 7, 33], [13, S - 7, 40]
+    m, q, ln, of, scale, out = attend_case(api, dtype, B, cols, S, heads, d, lens, offs)
+    for b in range(B):
+        for at in (slice(0, offs[b]), slice(offs[b] + lens[b], S)):
+            m.codes[b, at] = 255
+            m.scales[b, at] = float("nan")
+    assert torch.equal(m.attend(q, ln, of, scale=scale), out)
+    # a NaN inside reaches the columns of its sentence and no other
+    m.scales[1, offs[1] + 2, 0, 0] = float("nan")
+    bad = m.attend(q, ln, of, scale=scale).view(B, cols, heads, d)
+    assert bad[1, :, 0].isnan().all() and torch.equal(bad[[0, 2]], out.view(B, cols, heads, d)[[0, 2]])
+    assert torch.equal(bad[1, :, 1:], out.view(B, cols, heads, d)[1, :, 1:])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_attend_with_large_and_small_queries(api, dtype):
+    """Scores in the thousands (one slot takes all the weight), scores of nothing (equal weights), zero queries."""
+    for mul in (30.0, 1e-6, 0.0) + (() if dtype == "f16" else (1e-30, 1e5)):
+        attend_case(api, dtype, 2, 12, 77, 1, 256, [77, 50], [0, 5], seed=5, qmul=mul)
+    attend_case(api, dtype, 2, 5, 600, 4, 64, [600, 1], [0, 599], seed=5, qmul=20.0, scale=-0.7)
+
+
+def test_attend_on_strided_queries_and_outputs(api):
+    g = gen(11)
+    B, cols, S, d = 3, 4, 45, 100
+    hs = torch.tanh(torch.randn(S, B, d, generator=g, device="cuda"))
+    m = api.memory4(B, S, d).pack(hs)
+    lens = torch.tensor([45, 20, 3], dtype=torch.int32, device="cuda")
+    for t in ref.TYPES.values():
+        wide = torch.randn(B * cols, d + 7, generator=g, device="cuda").to(t)
+        q = wide[:, 3:3 + d]
+        out = torch.full((B * cols, d + 5), 9.0, dtype=t, device="cuda")
+        m.attend(q, lens, out=out[:, 2:2 + d])
+        assert torch.equal(out[:, 2:2 + d], m.attend(q.contiguous(), lens)) and out[:, :2].eq(9).all() and out[:, 2 + d:].eq(9).all()
+
+
+def test_attend_repeats_itself(api):
+    """Equal inputs give equal bits, whatever ran before; and a sentence's result does not depend on the others."""
+    m, q, ln, of, scale, out = attend_case(api, "f32", 4, 12, 2000, 1, 300, [2000, 1500, 1, 700], [0, 500, 3, 0])
+    torch.randn(1 << 24, device="cuda")
+    assert torch.equal(m.attend(q, ln, of, scale=scale), out)
+
+
+def test_attend_at_the_far_end_of_a_long_memory(api):
+    """More than 2^32 bytes of codes: offsets of 64 bits."""
+    S, d = (1 << 23) + 1000, 1024
+    if torch.cuda.mem_get_info()[0] < 8 << 30:
+        pytest.skip("needs 8 GB")
+    m = api.memory4(1, S, d)
+    g = gen(2)
+    hs = torch.tanh(torch.randn(45, 1, d, generator=g, device="cuda"))
+    q = torch.tanh(torch.randn(5, d, generator=g, device="cuda"))
+    m.pack(hs, slot0=S - 45)
+    n, o = torch.tensor([45], dtype=torch.int32, device="cuda"), torch.tensor([S - 45], dtype=torch.int32, device="cuda")
+    small = api.memory4(1, 45, d).pack(hs)
+    assert torch.equal(m.unpack(slot0=S - 45, S=45), small.unpack())
+    check_attend(m.attend(q, n, o), f64(small.unpack()), f64(q), [45], [0], 1.0, "f32")
+
+
+# ------------------------------------------------------------------ linear
+def linear_case(api, dtype, n, K, N, act="none", bias=True, residual=False, pad=(0, 0, 0, 0), seed=0, inplace=False, xmul=1.0):
+    """pad: how much further apart than they are long the rows of W, X, R and Y are."""
+    g = gen(seed)
+    W = randn(g, n, K + pad[0], dtype=dtype)[:, :K]
+    W.mul_(K ** -0.5)
+    X = (xmul * randn(g, N, K + pad[1])).to(ref.TYPES[dtype])[:, :K]
+    b = 0.5 * randn(g, n) if bias else None
+    Y = torch.full((N, n + pad[3]), 7.0, dtype=ref.TYPES[dtype], device="cuda")
+    R = randn(g, N, n + pad[2], dtype=dtype)[:, :n] if residual else None
+    if inplace:
+        Y[:, :n] = R
+        want_R, R = R, Y[:, :n]
+    else:
+        want_R = R
+    z = X.double() @ W.double().t()
+    if bias:
+        z = z + b.double()
+    want = ref.act(z, act)
+    if residual:
+        want = want + want_R.double()
+    out = api.linear(W, X, bias=b, act=act, residual=R, out=Y[:, :n])
+    mag = X.double().abs() @ W.double().abs().t() + (b.double().abs() if bias else 0)
+    # the activations' slopes are at most 1.13; they are evaluated to within a few roundings of 32 bits
+    tol = 1.13 * sum_tol(K) * mag + 16 * EPS * (1 + want.abs()) + ref.HALF_STEP[dtype] * (want.abs() + 1e-7)
+    err = (out.double() - want).abs()
+    assert bool((err <= tol).all()), (float(err.max()), float((err / tol).max()))
+    assert Y[:, n:].eq(7).all()
+    return W, X, b, out
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("n, K, N", [
+    (1, 1, 1), (3, 5, 2), (64, 64, 1), (1000, 2000, 12), (1000, 2000, 5), (129, 257, 16), (200, 1000, 17), (500, 96, 33), (256, 512, 64), (300, 40, 65), (1000, 1000, 100),
+    (1000, 2000, 768), (333, 777, 200), (777, 1024, 129), (2048, 320, 300), (130, 4096, 257), (37, 1173, 1), (4100, 64, 513), (515, 8, 1000), (8, 515, 1000)])
+def test_linear(api, dtype, n, K, N):
+    linear_case(api, dtype, n, K, N, seed=n + K)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("act", ["none", "tanh", "sigmoid", "relu", "gelu", "silu"])
+@pytest.mark.parametrize("n, K, N", [(200, 96, 7), (260, 160, 300)])
+def test_linear_epilogues(api, dtype, act, n, K, N):
+    linear_case(api, dtype, n, K, N, act, bias=False, seed=1)
+    linear_case(api, dtype, n, K, N, act, residual=True, seed=2, xmul=4.0)
+    linear_case(api, dtype, n, K, N, act, residual=True, inplace=True, seed=3)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("pad", [(8, 0, 0, 0), (0, 8, 24, 8), (3, 0, 0, 0), (0, 1, 0, 0), (5, 3, 1, 7), (4, 4, 4, 4)])
+@pytest.mark.parametrize("n, K, N", [(136, 200, 9), (264, 136, 301), (141, 205, 40)])
+def test_linear_strides(api, dtype, pad, n, K, N):
+    linear_case(api, dtype, n, K, N, "tanh", residual=True, pad=pad, seed=4)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_linear_on_operands_that_start_anywhere(api, dtype):
+    g = gen(8)
+    t = ref.TYPES[dtype]
+    for n, K, N in ((130, 96, 6), (270, 128, 200)):
+        for off in (1, 2, 4, 8):
+            Wb, Xb = randn(g, n * K + 16, dtype=dtype), randn(g, N * K + 16, dtype=dtype)
+            W, X = Wb[off:off + n * K].view(n, K), Xb[16 - off:16 - off + N * K].view(N, K)
+            out = torch.empty(N * n + 16, dtype=t, device="cuda")[off:off + N * n].view(N, n)
+            api.linear(W, X, out=out)
+            want, mag = X.double() @ W.double().t(), X.double().abs() @ W.double().abs().t()
+            assert bool(((out.double() - want).abs() <= sum_tol(K) * mag + ref.HALF_STEP[dtype] * want.abs()).all())
+
+
+def test_linear_in_32_bits_of_wide_ranges(api):
+    """fp32 operands over the whole range of magnitudes that 3xTF32 must carry: nothing is rounded to half precision on the way."""
+    g = gen(9)
+    for n, K, N in ((100, 300, 5), (300, 300, 200)):
+        W = randn(g, n, K) * torch.exp2(torch.randint(-60, 60, (n, 1), generator=g, device="cuda").float())
+        X = randn(g, N, K) * torch.exp2(torch.randint(-40, 60, (N, 1), generator=g, device="cuda").float())
+        out = api.linear(W, X).double()
+        want, mag = X.double() @ W.double().t(), X.double().abs() @ W.double().abs().t()
+        assert bool(((out - want).abs() <= sum_tol(K) * mag).all())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("N", [6, 200])
+def test_linear_numbers_that_are_not_finite(api, dtype, N):
+    """An infinity or a NaN in a column of X reaches that column alone, one in a row of W that output alone."""
+    g = gen(10)
+    n, K = 200, 130
+    W, X = randn(g, n, K, dtype=dtype), randn(g, N, K, dtype=dtype)
+    clean = api.linear(W, X, act="tanh")
+    X2, W2 = X.clone(), W.clone()
+    X2[3, 129] = float("nan")
+    X2[4, 0] = float("inf")
+    W2[150, 7] = float("nan")
+    got = api.linear(W2, X2, act="tanh")
+    assert got[3].isnan().all() and got[:, 150].isnan().all()
+    keep_c = [c for c in range(N) if c not in (3, 4)]
+    keep_n = [i for i in range(n) if i != 150]
+    assert torch.equal(got[keep_c][:, keep_n], clean[keep_c][:, keep_n])
+    # (3xTF32 splits an infinity into inf + NaN: the column is not finite, as inf * x is not)
+    assert bool((got[4, keep_n].isnan() | (got[4, keep_n].abs() == 1)).all())
+
+
+def test_linear_output_beyond_2_to_the_32(api):
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("needs 24 GB")
+    n, N, K = 70000, 66000, 8
+    g = gen(12)
+    W, X = randn(g, n, K, dtype="bf16"), randn(g, N, K, dtype="bf16")
+    out = api.linear(W, X)
+    at = torch.tensor([0, 1, 31000, 61356, 61357, 65535, 65999], device="cuda")
+    want = X[at].double() @ W.double().t()
+    mag = X[at].double().abs() @ W.double().abs().t()
+    assert bool(((out[at].double() - want).abs() <= sum_tol(K) * mag + ref.HALF_STEP["bf16"] * want.abs()).all())
+
+
+# ------------------------------------------------------------------ selection
+def select_case(api, z, scores, beam, k, lse=None, done=None, eos=1):
+    got = api.beam_select(z, scores, beam, k, lse=lse, done=done, eos=eos)
+    c = lambda t: None if t is None else t.cpu().numpy()  # noqa: E731
+    want = ref.select(z.float().cpu().numpy(), c(scores), beam, k, c(lse), c(done), eos)
+    for a, b, name in zip(got, want, ("values", "words", "parents")):
+        np.testing.assert_array_equal(a.cpu().numpy(), b, err_msg=name)
+    return got
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("n, beam, V, k", [
+    (1, 1, 1, 1), (1, 1, 7, 7), (2, 3, 5, 15), (1, 12, 40000, 12), (5, 12, 5003, 12), (3, 5, 129, 64), (7, 2, 1000, 4), (40, 8, 3001, 8), (2, 32, 20001, 64), (1, 1, 200000, 33),
+    (300, 4, 777, 5), (2, 64, 33, 64), (1, 7, 100003, 50)])
+def test_beam_select(api, dtype, n, beam, V, k):
+    g = gen(n + V)
+    z = 2 * randn(g, n * beam, V, dtype=dtype)
+    scores = -20 + 3 * randn(g, n * beam)
+    lse = torch.logsumexp(z.float(), 1)
+    select_case(api, z, scores, beam, k, lse=lse)
+    select_case(api, z, scores, beam, k)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n, beam, V", [(3, 12, 2001), (2, 5, 30000), (1, 12, 120000)])
+def test_beam_select_finished_and_dead_hypotheses(api, dtype, n, beam, V):
+    g = gen(V)
+    z = 2 * randn(g, n * beam, V, dtype=dtype)
+    scores = -20 + 3 * randn(g, n * beam)
+    done = (torch.rand(n * beam, generator=g, device="cuda") < 0.4).int()
+    scores[2] = float("-inf")
+    scores[beam - 1] = float("nan")
+    z[1, 5] = float("nan")
+    z[1, 9:40] = float("-inf")
+    lse = torch.logsumexp(torch.nan_to_num(z.float(), nan=0.0), 1)
+    for eos in (1, 0, V - 1):
+        select_case(api, z, scores, beam, beam, lse=lse, done=done, eos=eos)
+    # every hypothesis finished: as many candidates as hypotheses, the rest of the output is empty
+    k = min(64, beam + 3)
+    scores = -20 + 3 * randn(g, n * beam)
+    val, word, parent = select_case(api, z, scores, beam, k, done=torch.ones_like(done), eos=2)
+    assert word[:, :beam].eq(2).all() and word[:, beam:].eq(-1).all() and parent[:, beam:].eq(-1).all() and val[:, beam:].eq(float("-inf")).all()
+    # no hypothesis alive
+    val, word, parent = select_case(api, z, torch.full_like(scores, float("-inf")), beam, 4)
+    assert word.eq(-1).all() and parent.eq(-1).all()
+    done[:] = torch.arange(n * beam, device="cuda") % 3
+    val, word, parent = select_case(api, torch.full_like(z, float("-inf")), scores, beam, 8, done=done)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("V", [50, 5000, 70001])
+def test_beam_select_ties_go_to_the_lowest_candidate(api, dtype, V):
+    """All candidates equal; a few values only; +0 and -0; +inf."""
+    n, beam, k = 2, 6, 20
+    z = torch.zeros(n * beam, V, dtype=ref.TYPES[dtype], device="cuda")
+    s = torch.zeros(n * beam, device="cuda")
+    _, word, parent = select_case(api, z, s, beam, k)
+    assert word[0].tolist() == list(range(k)) and parent[1].tolist() == [beam] * k
+    g = gen(4)
+    z = torch.randint(-2, 2, (n * beam, V), generator=g, device="cuda").to(ref.TYPES[dtype])
+    z = torch.where(z == 1, -0.0, z.float()).to(ref.TYPES[dtype])
+    select_case(api, z, s, beam, 64)
+    select_case(api, z, -s, beam, 64)
+    z[3, V // 2] = z[1, V - 1] = float("inf")
+    select_case(api, z, s, beam, k)
+    up = torch.arange(V, device="cuda").float().repeat(n * beam, 1).to(ref.TYPES[dtype])  # every new value is better than all before
+    select_case(api, up, s, beam, 64)
+    select_case(api, -up, s, beam, 64)
+
+
+def test_beam_select_on_rows_that_start_anywhere(api):
+    g = gen(6)
+    for dtype in ref.TYPES:
+        for V, ld in ((1001, 1003), (999, 1000), (4097, 4097), (64, 65)):
+            buf = randn(g, 3 * 4 * ld + 8, dtype=dtype)
+            for off in (0, 1, 3):
+                z = buf[off:off + 12 * ld].view(12, ld)[:, :V]
+                select_case(api, z, randn(g, 12), 4, 6)
+
+
+# ------------------------------------------------------------------ reorder
+@pytest.mark.parametrize("n_src, n, dtype, widths", [
+    (12, 12, torch.float32, (1000, 1000, 64)), (24, 60, torch.bfloat16, (333,)), (7, 5, torch.uint8, (1, 3, 17)), (768, 768, torch.float32, (1000,) * 5), (4, 1, torch.float16, (6, 2)),
+    (1, 9, torch.float32, (130,))])
+def test_beam_reorder(api, n_src, n, dtype, widths):
+    g = gen(n)
+    xs = [(100 * torch.randn(n_src, w, generator=g, device="cuda")).to(dtype) for w in widths]
+    p = torch.randint(-1, n_src, (n,), generator=g, device="cuda", dtype=torch.int32)
+    out = api.beam_reorder(xs, p)
+    for x, o in zip(xs, out):
+        want = torch.where((p >= 0)[:, None], x[p.clamp(min=0).long()], torch.zeros((), dtype=dtype, device="cuda"))
+        assert torch.equal(o, want)
+
+
+@pytest.mark.parametrize("beam", [1, 2, 5, 12, 16, 33, 64])
+def test_beam_reorder_in_place(api, beam):
+    g = gen(beam)
+    n = 6 * beam
+    xs = [torch.randn(n, w, generator=g, device="cuda") for w in (1000, 3, 40)] + [torch.randn(n, 33, generator=g, device="cuda").half()]
+    p = torch.randint(0, beam, (6, beam), generator=g, device="cuda", dtype=torch.int32) + torch.arange(6, device="cuda", dtype=torch.int32)[:, None] * beam
+    p.view(-1)[n // 2] = -1
+    want = [torch.where((p.view(-1) >= 0)[:, None], x[p.view(-1).clamp(min=0).long()], 0.0) for x in xs]
+    other = torch.empty_like(xs[1])
+    got = api.beam_reorder(xs + [xs[1].clone()], p, out=xs + [other], group=beam)  # the last one out of place
+    for a, b in zip(got, want + [want[1]]):
+        assert torch.equal(a, b)
+
+
+def test_beam_reorder_reports_a_parent_that_is_no_column(api):
+    assert api.lib().zrnn_tc_error() == 0
+    x = torch.randn(6, 100, device="cuda")
+    keep = x.clone()
+    p = torch.tensor([0, 6, 2, 2**31 - 1, -7, 1], dtype=torch.int32, device="cuda")
+    out, = api.beam_reorder([x], p)
+    torch.cuda.synchronize()
+    assert api.lib().zrnn_tc_error() == 101
+    assert out[[1, 3, 4]].eq(0).all() and torch.equal(out[[0, 2, 5]], x[[0, 2, 1]])
+    api.beam_reorder([x], torch.tensor([1, 0, 3, 2, 3, 4], dtype=torch.int32, device="cuda"), out=[x], group=3)
+    torch.cuda.synchronize()
+    assert api.lib().zrnn_tc_error() == 101  # columns 2 and 4 asked for the other group
+    assert torch.equal(x, keep[[1, 0, 2, 3, 3, 4]])
+
+
+# ------------------------------------------------------------------ together
+class Step:
+    """A decoder's step made of the operators: attention over the packed source, the combiner, the vocabulary's logits, selection, reorder."""
+
+    def __init__(self, api, n=3, beam=4, H=96, V=501, S=37, dtype="f32"):
+        g = gen(21)
+        t = ref.TYPES[dtype]
+        self.api, self.n, self.beam, self.H, self.V, self.dtype = api, n, beam, H, V, dtype
+        self.hs = torch.tanh(torch.randn(S, n, H, generator=g, device="cuda")).to(t)
+        self.lens = torch.tensor([S, 9, 1][:n], dtype=torch.int32, device="cuda")
+        self.offs = S - self.lens
+        self.Wc = (torch.randn(H, 2 * H, generator=g, device="cuda") * 0.2).to(t)
+        self.bc = torch.randn(H, generator=g, device="cuda") * 0.1
+        self.D = torch.randn(V, H, generator=g, device="cuda").to(t)
+        self.bd = torch.randn(V, generator=g, device="cuda") * 0.1
+        self.h = torch.tanh(torch.randn(n * beam, H, generator=g, device="cuda")).to(t)
+        self.scores = torch.randn(n * beam, generator=g, device="cuda") - 3
+
+    def run(self, mem):
+        a = self.api
+        ctx = mem.attend(self.h, self.lens, self.offs)
+        ht = a.linear(self.Wc, torch.cat([ctx, self.h], 1), bias=self.bc, act="tanh", residual=self.h)
+        z = a.linear(self.D, ht, bias=self.bd)
+        lse = torch.logsumexp(z.float(), 1)
+        val, word, parent = a.beam_select(z, self.scores, self.beam, self.beam, lse=lse)
+        new, = a.beam_reorder([ht], parent)
+        return ctx, ht, z, lse, val, word, parent, new
+
+    def check(self, mem, got):
+        ctx, ht, z, lse, val, word, parent, new = got
+        v = ref.unpack(mem.codes.cpu().numpy(), mem.scales.cpu().numpy(), self.H)
+        check_attend(ctx, v, f64(self.h), self.lens.tolist(), self.offs.tolist(), 1.0, self.dtype)
+        X = torch.cat([ctx, self.h], 1).double()
+        want = torch.tanh(X @ self.Wc.double().t() + self.bc.double()) + self.h.double()
+        tol = sum_tol(2 * self.H) * (X.abs() @ self.Wc.double().abs().t() + 1) + (16 * EPS + ref.HALF_STEP[self.dtype]) * (1 + want.abs())
+        assert bool(((ht.double() - want).abs() <= tol).all())
+        want = ht.double() @ self.D.double().t() + self.bd.double()
+        tol = sum_tol(self.H) * (ht.double().abs() @ self.D.double().abs().t() + 1) + (16 * EPS + ref.HALF_STEP[self.dtype]) * (1 + want.abs())
+        assert bool(((z.double() - want).abs() <= tol).all())
+        w = ref.select(z.float().cpu().numpy(), self.scores.cpu().numpy(), self.beam, self.beam, lse.cpu().numpy())
+        for a, b in zip((val, word, parent), w):
+            np.testing.assert_array_equal(a.cpu().numpy(), b)
+        assert torch.equal(new, ht[parent.view(-1).long()])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_a_step_of_all_operators(api, dtype):
+    s = Step(api, dtype=dtype)
+    mem = api.memory4(3, 37, 96).pack(s.hs)
+    s.check(mem, s.run(mem))
+
+
+def test_a_captured_step_gives_what_the_calls_give(api):
+    """Capture, replay on changed inputs, two graphs replayed on two streams at once."""
+    steps = [Step(api), Step(api, n=2, beam=12, H=320, V=3000)]
+    mems = [api.memory4(s.n, 37, s.H).pack(s.hs) for s in steps]
+    graphs, outs = [], []
+    for s, m in zip(steps, mems):
+        st = torch.cuda.Stream()
+        st.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(st):
+            s.run(m)
+        torch.cuda.current_stream().wait_stream(st)
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            outs.append(s.run(m))
+        graphs.append(gr)
+    for round_ in range(3):
+        for s in steps:
+            s.h.copy_(torch.tanh(torch.randn(s.h.shape, generator=gen(50 + round_), device="cuda")))
+        torch.cuda.synchronize()
+        streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+        for _ in range(5):
+            for gr, st in zip(graphs, streams):
+                with torch.cuda.stream(st):
+                    gr.replay()
+        torch.cuda.synchronize()
+        for s, m, o in zip(steps, mems, outs):
+            s.check(m, o)
+            for a, b in zip(o, s.run(m)):
+                assert torch.equal(a, b)
+
+
+def test_calls_on_two_streams_at_once(api):
+    """Each call's scratch memory is its own."""
+    m, q, ln, of, scale, out = attend_case(api, "f32", 2, 12, 5000, 1, 256, [5000, 4000], [0, 1000])
+    g = gen(31)
+    z, sc = 2 * randn(g, 24, 60000), randn(g, 24)
+    W, X = randn(g, 700, 333), randn(g, 300, 333)
+    base = [out, *api.beam_select(z, sc, 12, 12), api.linear(W, X)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    got = []
+    for _ in range(6):
+        for st in streams:
+            with torch.cuda.stream(st):
+                got.append([m.attend(q, ln, of, scale=scale), *api.beam_select(z, sc, 12, 12), api.linear(W, X)])
+    torch.cuda.synchronize()
+    for r in got:
+        for a, b in zip(r, base):
+            assert torch.equal(a, b)
+
+
+def test_the_calls_allocate_nothing(api):
+    """Through the C ABI, with the caller's workspaces."""
+    s = Step(api)
+    mem = api.memory4(3, 37, 96).pack(s.hs)
+    s.run(mem)
+    torch.cuda.synchronize()
+    before = torch.cuda.mem_get_info()[0]
+    for _ in range(10):
+        s.run(mem)
+    torch.cuda.synchronize()
+    assert torch.cuda.mem_get_info()[0] >= before

@@ -12,10 +12,12 @@ LIB_PATH = os.path.join(_HERE, "libzrnn.so")
 c_int_p = ctypes.POINTER(ctypes.c_int)
 c_float_p = ctypes.POINTER(ctypes.c_float)
 c_void_p = ctypes.c_void_p
+c_size_p = ctypes.POINTER(ctypes.c_size_t)
 
 OK, E_ARG, E_CUDA, E_NCCL, E_TIMEOUT, E_IO, E_STATE = range(7)
 F32, BF16, TF32, F32_SIMT, F32_3XTF32, F32_F16X2 = 0, 1, 2, 3, 4, 5
 ATT_NONE, ATT_LOCAL_P, ATT_GLOBAL_DOT = 0, 1, 2
+ELEM_F32, ELEM_BF16, ELEM_F16 = 0, 1, 2
 
 
 class ModelConfig(ctypes.Structure):
@@ -148,6 +150,21 @@ SIGNATURES = {
                                                       ctypes.c_int, ctypes.c_float, ctypes.c_float, ctypes.c_float,
                                                       ctypes.c_int, c_void_p, c_void_p, c_void_p]),
     "zrnn_model_destroy": (ctypes.c_int, [c_void_p]),
+    "zrnn_memory4_sizes": (ctypes.c_int, [ctypes.c_int] * 4 + [c_size_p, c_size_p]),
+    "zrnn_memory4_pack": (ctypes.c_int, [ctypes.c_int, c_void_p, ctypes.c_longlong, ctypes.c_longlong] + [ctypes.c_int] * 6 + [c_void_p] * 3),
+    "zrnn_memory4_unpack": (ctypes.c_int, [ctypes.c_int, c_void_p, c_void_p] + [ctypes.c_int] * 6 + [c_void_p, c_void_p]),
+    "zrnn_memory4_attend_workspace": (ctypes.c_int, [ctypes.c_int] * 5 + [c_size_p]),
+    "zrnn_memory4_attend": (ctypes.c_int, [ctypes.c_int, c_void_p, c_void_p] + [ctypes.c_int] * 4 +
+                            [c_void_p, c_void_p, c_void_p, ctypes.c_longlong, ctypes.c_int, c_void_p, ctypes.c_float, c_void_p,
+                             ctypes.c_longlong, c_void_p, ctypes.c_size_t, c_void_p]),
+    "zrnn_linear_workspace": (ctypes.c_int, [ctypes.c_int] * 4 + [c_void_p, ctypes.c_longlong, c_void_p, ctypes.c_longlong, c_size_p]),
+    "zrnn_linear": (ctypes.c_int, [ctypes.c_int] * 5 + [c_void_p, ctypes.c_longlong, c_void_p, ctypes.c_longlong, c_void_p, c_void_p,
+                                                        ctypes.c_longlong, c_void_p, ctypes.c_longlong, c_void_p, ctypes.c_size_t, c_void_p]),
+    "zrnn_beam_select_workspace": (ctypes.c_int, [ctypes.c_int] * 5 + [c_size_p]),
+    "zrnn_beam_select": (ctypes.c_int, [ctypes.c_int, c_void_p, ctypes.c_longlong, c_void_p, c_void_p, c_void_p] + [ctypes.c_int] * 5 +
+                         [c_void_p, c_void_p, c_void_p, c_void_p, ctypes.c_size_t, c_void_p]),
+    "zrnn_beam_reorder": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(c_void_p), ctypes.POINTER(c_void_p), c_size_p, c_void_p] +
+                          [ctypes.c_int] * 3 + [c_void_p]),
 }
 
 _LIB = None

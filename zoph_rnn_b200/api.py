@@ -515,6 +515,184 @@ def decode_ensemble(models, sources_per_model, beam=12, k_best=1, min_ratio=0.5,
     return ids, ln, sc
 
 
+# ---- operators of a decoding step (their vectors may be float32, bfloat16 or float16 tensors)
+_ELEM = {torch.float32: _lib.ELEM_F32, torch.bfloat16: _lib.ELEM_BF16, torch.float16: _lib.ELEM_F16}
+ACTIVATIONS = ("none", "tanh", "sigmoid", "relu", "gelu", "silu")
+
+
+def _elem(t, what):
+    if t.dtype not in _ELEM:
+        raise ValueError(f"{what}: float32, bfloat16 or float16 tensors, not {t.dtype}")
+    return _ELEM[t.dtype]
+
+
+def _here(what, *tensors):
+    """The library works on the current device: tensors that lie elsewhere are refused."""
+    dev = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and (not t.is_cuda or t.device.index != dev):
+            raise ValueError(f"{what}: a tensor lies on {t.device}, the current device is cuda:{dev}")
+
+
+def _rows(t, what, width=None):
+    """(columns, leading dimension) of a [columns, width] tensor whose rows are contiguous."""
+    if t.dim() != 2 or (t.size(1) > 1 and t.stride(1) != 1) or (width is not None and t.size(1) != width):
+        raise ValueError(f"{what}: expected [columns, {'n' if width is None else width}] with contiguous rows, got "
+                         f"{tuple(t.shape)} with strides {t.stride()}")
+    return t.size(0), (max(t.stride(0), t.size(1)) if t.size(0) <= 1 else t.stride(0))
+
+
+def _dense(t, what, dtype, shape):
+    if t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+        raise ValueError(f"{what}: expected a contiguous {dtype} tensor of shape {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+    return t
+
+
+def _scratch(nbytes, device):
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+class memory4:
+    """The states that attention reads, held in 4 bits (zrnn_memory4_* in include/zrnn.h): B source columns of S_max slots with
+    `heads` vectors of d elements each (heads = 1, d = H for this library's models).  codes [B, S_max, heads, groups * 16] uint8 and
+    scales [B, S_max, heads, groups] float16 may be given; otherwise they are made, uninitialised."""
+
+    def __init__(self, B, S_max, d, heads=1, codes=None, scales=None):
+        nc, ns = ctypes.c_size_t(), ctypes.c_size_t()
+        check(lib().zrnn_memory4_sizes(B, S_max, heads, d, ctypes.byref(nc), ctypes.byref(ns)))
+        self.B, self.S_max, self.heads, self.d = B, S_max, heads, d
+        g = -(-d // 32)
+        if codes is None:
+            codes = torch.empty(B, S_max, heads, g * 16, dtype=torch.uint8, device="cuda")
+        if scales is None:
+            scales = torch.empty(B, S_max, heads, g, dtype=torch.float16, device="cuda")
+        self.codes = _dense(codes, "memory4: codes", torch.uint8, (B, S_max, heads, g * 16))
+        self.scales = _dense(scales, "memory4: scales", torch.float16, (B, S_max, heads, g))
+        _here("memory4", self.codes, self.scales)
+
+    def pack(self, hs, slot0=0):
+        """hs [S, B, heads * d] (any strides but the last): slots slot0 .. slot0 + S - 1 of every column."""
+        e = _elem(hs, "memory4.pack")
+        _here("memory4.pack", hs, self.codes)
+        if hs.dim() != 3 or hs.size(1) != self.B or hs.size(2) != self.heads * self.d or (hs.size(2) > 1 and hs.stride(2) != 1):
+            raise ValueError(f"memory4.pack: expected [S, {self.B}, {self.heads * self.d}] with contiguous vectors, got {tuple(hs.shape)}")
+        check(lib().zrnn_memory4_pack(e, _ptr(hs), hs.stride(0), hs.stride(1), hs.size(0), self.B, self.heads, self.d, slot0, self.S_max,
+                                      _ptr(self.codes), _ptr(self.scales), _stream()))
+        return self
+
+    def unpack(self, dtype=torch.float32, slot0=0, S=None):
+        """[B, S, heads, d]: the numbers that the codes stand for."""
+        S = self.S_max - slot0 if S is None else S
+        out = torch.empty(self.B, max(S, 0), self.heads, self.d, dtype=dtype, device=self.codes.device)
+        e = _elem(out, "memory4.unpack")
+        _here("memory4.unpack", self.codes)
+        check(lib().zrnn_memory4_unpack(e, _ptr(self.codes), _ptr(self.scales), self.B, self.S_max, self.heads, self.d, slot0, S, _ptr(out),
+                                        _stream()))
+        return out
+
+    def attend(self, q, lens, offsets=None, scale=1.0, mask01=None, out=None):
+        """Softmax attention of the columns of q [B * cols, heads * d] over the slots offset <= s < offset + len of their source
+        columns (lens, offsets: int32 [B]); returns [B * cols, heads * d] in q's type."""
+        e = _elem(q, "memory4.attend")
+        N, ldq = _rows(q, "memory4.attend", self.heads * self.d)
+        if N == 0 or N % self.B:
+            raise ValueError(f"memory4.attend: {N} columns for {self.B} source columns")
+        if out is None:
+            out = torch.empty(N, self.heads * self.d, dtype=q.dtype, device=q.device)
+        if out.dtype != q.dtype or out.size(0) != N:
+            raise ValueError("memory4.attend: out does not match q")
+        ldo = _rows(out, "memory4.attend: out", self.heads * self.d)[1]
+        _dense(lens, "memory4.attend: lens", torch.int32, (self.B,))
+        if offsets is not None:
+            _dense(offsets, "memory4.attend: offsets", torch.int32, (self.B,))
+        if mask01 is not None:
+            _dense(mask01, "memory4.attend: mask01", torch.int32, (N,))
+        _here("memory4.attend", q, out, lens, offsets, mask01, self.codes)
+        L, n = lib(), ctypes.c_size_t()
+        check(L.zrnn_memory4_attend_workspace(self.B, N // self.B, self.S_max, self.heads, self.d, ctypes.byref(n)))
+        work = _scratch(n.value, q.device)
+        check(L.zrnn_memory4_attend(e, _ptr(self.codes), _ptr(self.scales), self.B, self.S_max, self.heads, self.d, _ptr(lens), _ptr(offsets),
+                                    _ptr(q), ldq, N // self.B, _ptr(mask01), scale, _ptr(out), ldo, _ptr(work), n.value, _stream()))
+        return out
+
+
+def linear(W, X, bias=None, act="none", residual=None, out=None):
+    """act(X W^T + bias) + residual for the columns X [N, K] and the weights W [n, K] of each output (zrnn_linear); bias float32 [n];
+    residual and out [N, n] in X's type, and may be the same tensor."""
+    e = _elem(X, "linear")
+    n, ldw = _rows(W, "linear: W")
+    N, ldx = _rows(X, "linear: X", W.size(1))
+    if W.dtype != X.dtype:
+        raise ValueError("linear: W and X differ in type")
+    if act not in ACTIVATIONS:
+        raise ValueError(f"linear: act is one of {ACTIVATIONS}")
+    if out is None:
+        out = torch.empty(N, n, dtype=X.dtype, device=X.device)
+    ldr = 0
+    for t, name in ((out, "out"), (residual, "residual")):
+        if t is not None and (t.dtype != X.dtype or t.size(0) != N):
+            raise ValueError(f"linear: {name} does not match X")
+    ldy = _rows(out, "linear: out", n)[1]
+    if residual is not None:
+        ldr = _rows(residual, "linear: residual", n)[1]
+    if bias is not None:
+        _dense(bias, "linear: bias", torch.float32, (n,))
+    _here("linear", W, X, bias, residual, out)
+    L, nb = lib(), ctypes.c_size_t()
+    check(L.zrnn_linear_workspace(e, n, N, W.size(1), _ptr(W), ldw, _ptr(X), ldx, ctypes.byref(nb)))
+    work = _scratch(nb.value, X.device)
+    check(L.zrnn_linear(e, ACTIVATIONS.index(act), n, N, W.size(1), _ptr(W), ldw, _ptr(X), ldx, _ptr(bias), _ptr(residual), ldr, _ptr(out), ldy,
+                        _ptr(work), nb.value, _stream()))
+    return out
+
+
+def beam_select(logp, scores, beam, k, lse=None, done=None, eos=1):
+    """The k best continuations of every sentence (zrnn_beam_select): logp [n_sent * beam, V] log-probabilities, or logits with their
+    normalisers lse; scores and lse float32, done int32 [n_sent * beam].  Returns (scores, words, parents), each [n_sent, k]; parents
+    are rows of logp, as beam_reorder takes them."""
+    e = _elem(logp, "beam_select")
+    rows, ld = _rows(logp, "beam_select: logp")
+    if beam < 1 or rows % beam:
+        raise ValueError(f"beam_select: {rows} rows are no sentences of {beam} hypotheses")
+    n = rows // beam
+    for t, name, dt in ((scores, "scores", torch.float32), (lse, "lse", torch.float32), (done, "done", torch.int32)):
+        if t is not None and (t.dtype != dt or t.numel() != rows or not t.is_contiguous()):
+            raise ValueError(f"beam_select: {name} must be a contiguous {dt} tensor of {rows} elements")
+    _here("beam_select", logp, scores, lse, done)
+    val = torch.empty(n, k, dtype=torch.float32, device=logp.device)
+    words = torch.empty(n, k, dtype=torch.int32, device=logp.device)
+    parents = torch.empty(n, k, dtype=torch.int32, device=logp.device)
+    L, nb = lib(), ctypes.c_size_t()
+    check(L.zrnn_beam_select_workspace(e, n, beam, logp.size(1), k, ctypes.byref(nb)))
+    work = _scratch(nb.value, logp.device)
+    check(L.zrnn_beam_select(e, _ptr(logp), ld, _ptr(lse), _ptr(scores), _ptr(done), n, beam, logp.size(1), k, eos, _ptr(val), _ptr(words),
+                             _ptr(parents), _ptr(work), nb.value, _stream()))
+    return val, words, parents
+
+
+def beam_reorder(states, parents, out=None, group=1):
+    """Column c of every tensor of `states` ([columns, ...], contiguous) becomes its column parents[c] (zrnn_beam_reorder).  out: a list
+    of tensors to write; an entry may be the state itself (columns then move within groups of `group`).  Returns the list."""
+    states = list(states)
+    n = parents.numel()
+    if parents.dtype != torch.int32 or not parents.is_contiguous():
+        raise ValueError("beam_reorder: parents must be a contiguous int32 tensor")
+    out = [torch.empty((n,) + tuple(s.shape[1:]), dtype=s.dtype, device=s.device) for s in states] if out is None else list(out)
+    if len(out) != len(states):
+        raise ValueError("beam_reorder: as many outputs as states")
+    m = len(states)
+    if m == 0:
+        return out
+    n_src = states[0].size(0)
+    src, dst, size = (ctypes.c_void_p * m)(), (ctypes.c_void_p * m)(), (ctypes.c_size_t * m)()
+    for i, (s, o) in enumerate(zip(states, out)):
+        if not s.is_contiguous() or not o.is_contiguous() or s.dtype != o.dtype or s.size(0) != n_src or o.size(0) != n or s.shape[1:] != o.shape[1:]:
+            raise ValueError("beam_reorder: states and outputs are contiguous [columns, ...] tensors of the same type and width")
+        src[i], dst[i], size[i] = s.data_ptr(), o.data_ptr(), (o.numel() // n if n else 0) * o.element_size()
+    _here("beam_reorder", parents, *states, *out)
+    check(lib().zrnn_beam_reorder(m, src, dst, size, _ptr(parents), n, n_src, group, _stream()))
+    return out
+
 def read_model_file_header(path):
     """(header ints [9], how many the file carried, source vocabulary lines, target vocabulary lines) of a
     model.nn, parsed on the host (src/add_model_info.h:7-9)."""

@@ -19,6 +19,7 @@
 #include "../../include/zrnn_debug.h"
 #include "kernels.cuh"
 #include "model_file.hpp"
+#include "operators.cuh"
 #include "skinny_gemm.cuh"
 #include "tc_chain.cuh"
 #include "tc_vocab.cuh"
@@ -910,6 +911,8 @@ int device_error_status(const char* what) {
   if (code == 0) return ZRNN_OK;
   if (code == zrnn::kErrBadTokenId)
     return fail(ZRNN_E_ARG, std::string(what) + ": a token id on the device is outside the vocabulary (column 0 was read instead)");
+  if (code == zrnn::kErrBadParent)
+    return fail(ZRNN_E_ARG, std::string(what) + ": an earlier beam_reorder had a parent outside the columns it may move");
   return fail(ZRNN_E_TIMEOUT, std::string(what) + ": a bounded device wait gave up (role " + std::to_string(code) + ")");
 }
 }  // namespace
@@ -3037,6 +3040,224 @@ int zrnn_gemm(int mode, int n_rows, int m_cols, int K, const float* d_W, int ldw
   ZR_CUDA(e2);
   const int code = zrnn_tc_error();
   if (code != 0) return fail(ZRNN_E_TIMEOUT, "gemm: a bounded device wait gave up (role " + std::to_string(code) + ")");
+  return ZRNN_OK;
+}
+
+}  // extern "C"
+
+// ------------------------------------------------------------------------------------------
+// Operators of a decoding step for host programs: source memory in 4 bits, product with epilogue, selection and reorder
+// ------------------------------------------------------------------------------------------
+namespace {
+// a range of device memory that a call reads or writes
+struct Span {
+  uintptr_t lo, hi;
+  Span(const void* p, long long elems, int eb) : lo((uintptr_t)p), hi((uintptr_t)p + (uintptr_t)(elems * eb)) {}
+  bool meets(const Span& o) const { return lo < o.hi && o.lo < hi; }
+};
+// elements from the first one of a strided matrix to its last
+long long extent(long long cols, long long ld, long long width) { return cols > 0 ? (cols - 1) * ld + width : 0; }
+bool elem_aligned(const void* p, int elem) { return ((uintptr_t)p & (zrnn::elem_bytes(elem) - 1)) == 0; }
+
+int mem4_check(const char* what, int elem, int B, int S_cap, int heads, int d) {
+  ZR_CHECK(elem >= ZRNN_ELEM_F32 && elem <= ZRNN_ELEM_F16, std::string(what) + ": unknown element type");
+  ZR_CHECK(B >= 1 && S_cap >= 1 && heads >= 1 && d >= 1, std::string(what) + ": sizes must be positive");
+  ZR_CHECK(heads <= 65535 && (long long)heads * zrnn::mem4_groups(d) <= (1 << 20), std::string(what) + ": heads * d is too large");
+  ZR_CHECK((long long)B * S_cap <= (1ll << 40) / ((long long)heads * zrnn::mem4_groups(d)), std::string(what) + ": the memory is too large");
+  return ZRNN_OK;
+}
+}  // namespace
+
+extern "C" {
+
+int zrnn_memory4_sizes(int B, int S_cap, int heads, int d, size_t* code_bytes, size_t* n_scales) {
+  ZR_CHECK(code_bytes && n_scales, "memory4_sizes: null argument");
+  ZR_TRY(mem4_check("memory4_sizes", ZRNN_ELEM_F32, B, S_cap, heads, d));
+  *n_scales = (size_t)B * S_cap * heads * zrnn::mem4_groups(d);
+  *code_bytes = *n_scales * (zrnn::kMem4Group / 2);
+  return ZRNN_OK;
+}
+int zrnn_memory4_pack(int elem, const void* d_x, long long ld_slot, long long ld_col, int S, int B, int heads, int d, int slot0, int S_cap,
+                      void* d_codes, void* d_scales, void* stream) {
+  ZR_TRY(mem4_check("memory4_pack", elem, B, S_cap, heads, d));
+  ZR_CHECK(S >= 0 && slot0 >= 0 && slot0 <= S_cap - S, "memory4_pack: the slots lie outside the memory");
+  if (S == 0) return ZRNN_OK;
+  ZR_CHECK(d_x && d_codes && d_scales, "memory4_pack: null pointer");
+  ZR_CHECK(ld_slot >= 0 && ld_col >= 0, "memory4_pack: negative stride");
+  ZR_CHECK(elem_aligned(d_x, elem) && ((uintptr_t)d_codes & 15) == 0 && ((uintptr_t)d_scales & 1) == 0,
+           "memory4_pack: misaligned pointer (codes: 16 bytes)");
+  ZR_TRY(check_device());
+  zrnn::Mem4Pack a{d_x, ld_slot, ld_col, S, B, heads, d, slot0, S_cap, (uint8_t*)d_codes, (__half*)d_scales};
+  ZR_CUDA(zrnn::launch_mem4_pack(a, elem, (cudaStream_t)stream));
+  return ZRNN_OK;
+}
+int zrnn_memory4_unpack(int elem, const void* d_codes, const void* d_scales, int B, int S_cap, int heads, int d, int slot0, int S, void* d_out,
+                        void* stream) {
+  ZR_TRY(mem4_check("memory4_unpack", elem, B, S_cap, heads, d));
+  ZR_CHECK(S >= 0 && slot0 >= 0 && slot0 <= S_cap - S, "memory4_unpack: the slots lie outside the memory");
+  if (S == 0) return ZRNN_OK;
+  ZR_CHECK(d_out && d_codes && d_scales, "memory4_unpack: null pointer");
+  ZR_CHECK(elem_aligned(d_out, elem) && ((uintptr_t)d_codes & 15) == 0 && ((uintptr_t)d_scales & 1) == 0,
+           "memory4_unpack: misaligned pointer (codes: 16 bytes)");
+  ZR_TRY(check_device());
+  zrnn::Mem4Unpack a{(const uint8_t*)d_codes, (const __half*)d_scales, B, S_cap, heads, d, slot0, S, d_out};
+  ZR_CUDA(zrnn::launch_mem4_unpack(a, elem, (cudaStream_t)stream));
+  return ZRNN_OK;
+}
+int zrnn_memory4_attend_workspace(int B, int cols_per_sentence, int S_cap, int heads, int d, size_t* bytes) {
+  ZR_CHECK(bytes, "memory4_attend_workspace: null argument");
+  ZR_TRY(mem4_check("memory4_attend_workspace", ZRNN_ELEM_F32, B, S_cap, heads, d));
+  ZR_CHECK(cols_per_sentence >= 1, "memory4_attend_workspace: cols_per_sentence must be positive");
+  ZR_CHECK(d <= zrnn::kMem4MaxHead, "memory4_attend_workspace: a head of more than 1024 elements");
+  *bytes = zrnn::mem4_attend_work(B, cols_per_sentence, S_cap, heads, d) * sizeof(float);
+  return ZRNN_OK;
+}
+int zrnn_memory4_attend(int elem, const void* d_codes, const void* d_scales, int B, int S_cap, int heads, int d, const int* d_len,
+                        const int* d_offset, const void* d_q, long long ld_q, int cols_per_sentence, const int* d_mask01, float scale, void* d_out,
+                        long long ld_out, void* d_workspace, size_t workspace_bytes, void* stream) {
+  ZR_TRY(mem4_check("memory4_attend", elem, B, S_cap, heads, d));
+  ZR_CHECK(d <= zrnn::kMem4MaxHead, "memory4_attend: a head of more than 1024 elements");
+  ZR_CHECK(cols_per_sentence >= 1 && (long long)B * cols_per_sentence <= 0x7fffffff, "memory4_attend: bad number of columns");
+  ZR_CHECK(d_codes && d_scales && d_len && d_q && d_out, "memory4_attend: null pointer");
+  const long long width = (long long)heads * d, N = (long long)B * cols_per_sentence;
+  ZR_CHECK(ld_q >= width && ld_out >= width, "memory4_attend: leading dimension too small");
+  ZR_CHECK(elem_aligned(d_q, elem) && elem_aligned(d_out, elem) && ((uintptr_t)d_codes & 15) == 0 && ((uintptr_t)d_scales & 1) == 0,
+           "memory4_attend: misaligned pointer (codes: 16 bytes)");
+  const int eb = zrnn::elem_bytes(elem);
+  ZR_CHECK(!Span(d_q, extent(N, ld_q, width), eb).meets(Span(d_out, extent(N, ld_out, width), eb)), "memory4_attend: the output overlaps the queries");
+  const size_t need = zrnn::mem4_attend_work(B, cols_per_sentence, S_cap, heads, d) * sizeof(float);
+  ZR_CHECK(need == 0 || (d_workspace && workspace_bytes >= need && ((uintptr_t)d_workspace & 15) == 0),
+           "memory4_attend: the workspace must hold " + std::to_string(need) + " bytes (16-byte aligned)");
+  ZR_TRY(check_device());
+  zrnn::Mem4Attend a{(const uint8_t*)d_codes, (const __half*)d_scales, B, S_cap, heads, d, d_len, d_offset, d_q, ld_q, cols_per_sentence,
+                     d_mask01, scale, d_out, ld_out, (float*)d_workspace};
+  KScope ks(KC_ATT, (cudaStream_t)stream);
+  ZR_CUDA(zrnn::launch_mem4_attend(a, elem, (cudaStream_t)stream));
+  return ZRNN_OK;
+}
+
+static int linear_args(const char* what, int elem, int act, int n_rows, int n_cols, int K, const void* d_W, long long ldw, const void* d_X,
+                       long long ldx) {
+  ZR_CHECK(elem >= ZRNN_ELEM_F32 && elem <= ZRNN_ELEM_F16, std::string(what) + ": unknown element type");
+  ZR_CHECK(act >= ZRNN_ACT_NONE && act <= ZRNN_ACT_SILU, std::string(what) + ": unknown activation");
+  ZR_CHECK(n_rows >= 1 && n_cols >= 0 && K >= 1, std::string(what) + ": sizes must be positive");
+  ZR_CHECK(n_rows <= (1 << 24) && n_cols <= (1 << 24) && K <= (1 << 24), std::string(what) + ": a size of more than 2^24");
+  ZR_CHECK(ldw >= K && ldx >= K && ldw <= (1ll << 30) && ldx <= (1ll << 30), std::string(what) + ": bad leading dimension");
+  ZR_CHECK(elem_aligned(d_W, elem) && elem_aligned(d_X, elem), std::string(what) + ": misaligned pointer");
+  return ZRNN_OK;
+}
+int zrnn_linear_workspace(int elem, int n_rows, int n_cols, int K, const void* d_W, long long ldw, const void* d_X, long long ldx, size_t* bytes) {
+  ZR_CHECK(bytes, "linear_workspace: null argument");
+  ZR_TRY(linear_args("linear_workspace", elem, 0, n_rows, n_cols, K, d_W, ldw, d_X, ldx));
+  zrnn::LinearArgs a;
+  std::memset(&a, 0, sizeof(a));
+  a.n = n_rows; a.N = n_cols; a.K = K; a.W = d_W; a.X = d_X; a.ldw = ldw; a.ldx = ldx;
+  *bytes = n_cols ? zrnn::linear_work(a, elem) : 0;
+  return ZRNN_OK;
+}
+int zrnn_linear(int elem, int act, int n_rows, int n_cols, int K, const void* d_W, long long ldw, const void* d_X, long long ldx, const float* d_bias,
+                const void* d_residual, long long ldr, void* d_Y, long long ldy, void* d_workspace, size_t workspace_bytes, void* stream) {
+  ZR_TRY(linear_args("linear", elem, act, n_rows, n_cols, K, d_W, ldw, d_X, ldx));
+  if (n_cols == 0) return ZRNN_OK;
+  ZR_CHECK(d_W && d_X && d_Y, "linear: null pointer");
+  ZR_CHECK(ldy >= n_rows && ldy <= (1ll << 30) && (!d_residual || (ldr >= n_rows && ldr <= (1ll << 30))), "linear: bad leading dimension");
+  ZR_CHECK(elem_aligned(d_Y, elem) && elem_aligned(d_residual, elem) && ((uintptr_t)d_bias & 3) == 0, "linear: misaligned pointer");
+  const int eb = zrnn::elem_bytes(elem);
+  const Span y(d_Y, extent(n_cols, ldy, n_rows), eb);
+  ZR_CHECK(!y.meets(Span(d_W, extent(n_rows, ldw, K), eb)) && !y.meets(Span(d_X, extent(n_cols, ldx, K), eb)) &&
+               !(d_bias && y.meets(Span(d_bias, n_rows, 4))),
+           "linear: the output overlaps an input");
+  ZR_CHECK(!d_residual || (d_residual == d_Y && ldr == ldy) || !y.meets(Span(d_residual, extent(n_cols, ldr, n_rows), eb)),
+           "linear: the output overlaps the residual without being it");
+  zrnn::LinearArgs a;
+  std::memset(&a, 0, sizeof(a));
+  a.n = n_rows; a.N = n_cols; a.K = K; a.W = d_W; a.X = d_X; a.ldw = ldw; a.ldx = ldx;
+  a.bias = d_bias; a.R = d_residual; a.ldr = ldr; a.Y = d_Y; a.ldy = ldy; a.act = act;
+  const size_t need = zrnn::linear_work(a, elem);
+  ZR_CHECK(need == 0 || (d_workspace && workspace_bytes >= need && ((uintptr_t)d_workspace & 255) == 0),
+           "linear: the workspace must hold " + std::to_string(need) + " bytes (256-byte aligned)");
+  ZR_TRY(check_device());
+  a.work = d_workspace;
+  a.err = tc_error_word();
+  ZR_CUDA(zrnn::launch_linear(a, elem, (cudaStream_t)stream));
+  return ZRNN_OK;
+}
+
+static int select_args(const char* what, int elem, int n_sent, int beam, int V, int k) {
+  ZR_CHECK(elem >= ZRNN_ELEM_F32 && elem <= ZRNN_ELEM_F16, std::string(what) + ": unknown element type");
+  ZR_CHECK(n_sent >= 0 && beam >= 1 && V >= 1, std::string(what) + ": sizes must be positive");
+  ZR_CHECK((long long)beam * V <= 0x7fffffff && (long long)n_sent * beam <= 0x7fffffff, std::string(what) + ": too many candidates");
+  ZR_CHECK(k >= 1 && k <= zrnn::kSelectMax && k <= (long long)beam * V, std::string(what) + ": k must be in [1,64] and at most beam * V");
+  return ZRNN_OK;
+}
+int zrnn_beam_select_workspace(int elem, int n_sent, int beam, int V, int k, size_t* bytes) {
+  ZR_CHECK(bytes, "beam_select_workspace: null argument");
+  ZR_TRY(select_args("beam_select_workspace", elem, n_sent, beam, V, k));
+  *bytes = n_sent ? zrnn::beam_select_work(elem, n_sent, beam, V, k) : 0;
+  return ZRNN_OK;
+}
+int zrnn_beam_select(int elem, const void* d_logp, long long ld, const float* d_lse, const float* d_scores, const int* d_done, int n_sent, int beam,
+                     int V, int k, int eos, float* d_score_out, int* d_word_out, int* d_parent_out, void* d_workspace, size_t workspace_bytes,
+                     void* stream) {
+  ZR_TRY(select_args("beam_select", elem, n_sent, beam, V, k));
+  if (n_sent == 0) return ZRNN_OK;
+  ZR_CHECK(d_logp && d_scores && d_score_out && d_word_out && d_parent_out, "beam_select: null pointer");
+  ZR_CHECK(ld >= V, "beam_select: leading dimension too small");
+  ZR_CHECK(!d_done || (eos >= 0 && eos < V), "beam_select: finished hypotheses need an <EOF> word inside the vocabulary");
+  ZR_CHECK(elem_aligned(d_logp, elem), "beam_select: misaligned pointer");
+  const long long rows = (long long)n_sent * beam, outs = (long long)n_sent * k;
+  const Span outputs[3] = {Span(d_score_out, outs, 4), Span(d_word_out, outs, 4), Span(d_parent_out, outs, 4)};
+  for (int i = 0; i < 3; ++i)
+    ZR_CHECK(!outputs[i].meets(Span(d_logp, extent(rows, ld, V), zrnn::elem_bytes(elem))) && !outputs[i].meets(Span(d_scores, rows, 4)) &&
+                 !(d_lse && outputs[i].meets(Span(d_lse, rows, 4))) && !(d_done && outputs[i].meets(Span(d_done, rows, 4))) &&
+                 !outputs[i].meets(outputs[(i + 1) % 3]),
+             "beam_select: an output overlaps an input or another output");
+  const size_t need = zrnn::beam_select_work(elem, n_sent, beam, V, k);
+  ZR_CHECK(need == 0 || (d_workspace && workspace_bytes >= need && ((uintptr_t)d_workspace & 15) == 0),
+           "beam_select: the workspace must hold " + std::to_string(need) + " bytes (16-byte aligned)");
+  ZR_TRY(check_device());
+  zrnn::BeamSelect a{d_logp, ld, d_lse, d_scores, d_done, n_sent, beam, V, k, eos, d_score_out, d_word_out, d_parent_out,
+                     (unsigned long long*)d_workspace};
+  KScope ks(KC_BEAM, (cudaStream_t)stream);
+  ZR_CUDA(zrnn::launch_beam_select(a, elem, (cudaStream_t)stream));
+  return ZRNN_OK;
+}
+int zrnn_beam_reorder(int n_arrays, const void* const* d_src, void* const* d_dst, const size_t* bytes_per_col, const int* d_parent, int n_cols,
+                      int n_src_cols, int group, void* stream) {
+  ZR_CHECK(n_arrays >= 0 && n_arrays <= zrnn::BeamReorder::MAX_ARRAYS, "beam_reorder: at most 40 arrays");
+  ZR_CHECK(n_cols >= 0 && n_src_cols >= 0, "beam_reorder: negative number of columns");
+  if (n_arrays == 0 || n_cols == 0) return ZRNN_OK;
+  ZR_CHECK(d_src && d_dst && bytes_per_col && d_parent, "beam_reorder: null pointer");
+  zrnn::BeamReorder a;
+  std::memset(&a, 0, sizeof(a));
+  a.n_arrays = n_arrays; a.parent = d_parent; a.n_cols = n_cols; a.n_src_cols = n_src_cols; a.group = 1;
+  bool in_place = false;
+  const Span map(d_parent, n_cols, 4);
+  for (int i = 0; i < n_arrays; ++i) {
+    ZR_CHECK(d_src[i] && d_dst[i], "beam_reorder: null pointer");
+    ZR_CHECK(bytes_per_col[i] <= (1ull << 36), "beam_reorder: a column of more than 2^36 bytes");
+    a.src[i] = (const char*)d_src[i]; a.dst[i] = (char*)d_dst[i]; a.bytes[i] = (long long)bytes_per_col[i];
+    in_place = in_place || d_src[i] == d_dst[i];
+  }
+  for (int i = 0; i < n_arrays; ++i) {
+    const Span to(a.dst[i], (long long)n_cols * a.bytes[i], 1);
+    ZR_CHECK(!to.meets(map), "beam_reorder: an array overlaps the parents");
+    for (int j = 0; j < n_arrays; ++j) {
+      ZR_CHECK((i == j && a.src[i] == a.dst[i]) || !to.meets(Span(a.src[j], (long long)n_src_cols * a.bytes[j], 1)),
+               "beam_reorder: arrays overlap (in place an array is its own destination)");
+      ZR_CHECK(i == j || !to.meets(Span(a.dst[j], (long long)n_cols * a.bytes[j], 1)), "beam_reorder: destinations overlap");
+    }
+  }
+  if (in_place) {
+    ZR_CHECK(n_cols == n_src_cols, "beam_reorder: in place there are as many columns after as before");
+    ZR_CHECK(group >= 1 && group <= zrnn::kReorderGroup && n_cols % group == 0,
+             "beam_reorder: in place the columns move within groups of 1 to 64 that divide them");
+    a.group = group;
+  }
+  ZR_TRY(check_device());
+  a.err = tc_error_word();
+  KScope ks(KC_REORDER, (cudaStream_t)stream);
+  ZR_CUDA(zrnn::launch_beam_reorder(a, (cudaStream_t)stream));
   return ZRNN_OK;
 }
 
