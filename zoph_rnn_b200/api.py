@@ -6,6 +6,7 @@ calls into the reference.  PyTorch is used only to own device memory and streams
 arithmetic happens inside libzrnn.so.
 """
 import ctypes
+import functools
 
 import numpy as np
 import torch
@@ -527,29 +528,45 @@ def _elem(t, what):
 
 
 def _here(what, *tensors):
-    """The library works on the current device: tensors that lie elsewhere are refused."""
-    dev = torch.cuda.current_device()
+    """The library works on the current device: tensors that lie elsewhere are refused.  Returns its current stream."""
+    dev = torch._C._cuda_getDevice()
     for t in tensors:
-        if t is not None and (not t.is_cuda or t.device.index != dev):
+        if t is not None and t.get_device() != dev:
             raise ValueError(f"{what}: a tensor lies on {t.device}, the current device is cuda:{dev}")
+    return torch._C._cuda_getCurrentRawStream(dev)
 
 
 def _rows(t, what, width=None):
     """(columns, leading dimension) of a [columns, width] tensor whose rows are contiguous."""
-    if t.dim() != 2 or (t.size(1) > 1 and t.stride(1) != 1) or (width is not None and t.size(1) != width):
-        raise ValueError(f"{what}: expected [columns, {'n' if width is None else width}] with contiguous rows, got "
-                         f"{tuple(t.shape)} with strides {t.stride()}")
-    return t.size(0), (max(t.stride(0), t.size(1)) if t.size(0) <= 1 else t.stride(0))
+    if t.dim() == 2:
+        n, w = t.shape
+        ld, one = t.stride()
+        if (w == width or width is None) and (one == 1 or w <= 1):
+            return n, (ld if n > 1 and ld > 0 else w)
+    raise ValueError(f"{what}: expected [columns, {'n' if width is None else width}] with contiguous rows, got {tuple(t.shape)} with "
+                     f"strides {t.stride()}")
 
 
 def _dense(t, what, dtype, shape):
-    if t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+    if t.dtype != dtype or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{what}: expected a contiguous {dtype} tensor of shape {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
     return t
 
 
+@functools.lru_cache(maxsize=4096)
+def _work_bytes(fn, device, *args):
+    """What the *_workspace call `fn` of include/zrnn.h answers for these arguments."""
+    n = ctypes.c_size_t()
+    check(getattr(lib(), fn)(*args, ctypes.byref(n)))
+    return n.value
+
+
 def _scratch(nbytes, device):
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def _at(t):
+    return None if t is None else t.data_ptr()
 
 
 class memory4:
@@ -568,16 +585,16 @@ class memory4:
             scales = torch.empty(B, S_max, heads, g, dtype=torch.float16, device="cuda")
         self.codes = _dense(codes, "memory4: codes", torch.uint8, (B, S_max, heads, g * 16))
         self.scales = _dense(scales, "memory4: scales", torch.float16, (B, S_max, heads, g))
-        _here("memory4", self.codes, self.scales)
+        _here("memory4", codes, scales)
 
     def pack(self, hs, slot0=0):
         """hs [S, B, heads * d] (any strides but the last): slots slot0 .. slot0 + S - 1 of every column."""
         e = _elem(hs, "memory4.pack")
-        _here("memory4.pack", hs, self.codes)
+        stream = _here("memory4.pack", hs, self.codes)
         if hs.dim() != 3 or hs.size(1) != self.B or hs.size(2) != self.heads * self.d or (hs.size(2) > 1 and hs.stride(2) != 1):
             raise ValueError(f"memory4.pack: expected [S, {self.B}, {self.heads * self.d}] with contiguous vectors, got {tuple(hs.shape)}")
-        check(lib().zrnn_memory4_pack(e, _ptr(hs), hs.stride(0), hs.stride(1), hs.size(0), self.B, self.heads, self.d, slot0, self.S_max,
-                                      _ptr(self.codes), _ptr(self.scales), _stream()))
+        check(lib().zrnn_memory4_pack(e, hs.data_ptr(), hs.stride(0), hs.stride(1), hs.size(0), self.B, self.heads, self.d, slot0, self.S_max,
+                                      self.codes.data_ptr(), self.scales.data_ptr(), stream))
         return self
 
     def unpack(self, dtype=torch.float32, slot0=0, S=None):
@@ -585,9 +602,9 @@ class memory4:
         S = self.S_max - slot0 if S is None else S
         out = torch.empty(self.B, max(S, 0), self.heads, self.d, dtype=dtype, device=self.codes.device)
         e = _elem(out, "memory4.unpack")
-        _here("memory4.unpack", self.codes)
-        check(lib().zrnn_memory4_unpack(e, _ptr(self.codes), _ptr(self.scales), self.B, self.S_max, self.heads, self.d, slot0, S, _ptr(out),
-                                        _stream()))
+        stream = _here("memory4.unpack", self.codes)
+        check(lib().zrnn_memory4_unpack(e, self.codes.data_ptr(), self.scales.data_ptr(), self.B, self.S_max, self.heads, self.d, slot0, S,
+                                        out.data_ptr(), stream))
         return out
 
     def attend(self, q, lens, offsets=None, scale=1.0, mask01=None, out=None):
@@ -597,22 +614,23 @@ class memory4:
         N, ldq = _rows(q, "memory4.attend", self.heads * self.d)
         if N == 0 or N % self.B:
             raise ValueError(f"memory4.attend: {N} columns for {self.B} source columns")
+        B, heads, d = self.B, self.heads, self.d
         if out is None:
-            out = torch.empty(N, self.heads * self.d, dtype=q.dtype, device=q.device)
-        if out.dtype != q.dtype or out.size(0) != N:
-            raise ValueError("memory4.attend: out does not match q")
-        ldo = _rows(out, "memory4.attend: out", self.heads * self.d)[1]
-        _dense(lens, "memory4.attend: lens", torch.int32, (self.B,))
+            out, ldo = torch.empty(N, heads * d, dtype=q.dtype, device=q.device), heads * d
+        else:
+            if out.dtype != q.dtype or out.size(0) != N:
+                raise ValueError("memory4.attend: out does not match q")
+            ldo = _rows(out, "memory4.attend: out", heads * d)[1]
+        _dense(lens, "memory4.attend: lens", torch.int32, (B,))
         if offsets is not None:
-            _dense(offsets, "memory4.attend: offsets", torch.int32, (self.B,))
+            _dense(offsets, "memory4.attend: offsets", torch.int32, (B,))
         if mask01 is not None:
             _dense(mask01, "memory4.attend: mask01", torch.int32, (N,))
-        _here("memory4.attend", q, out, lens, offsets, mask01, self.codes)
-        L, n = lib(), ctypes.c_size_t()
-        check(L.zrnn_memory4_attend_workspace(self.B, N // self.B, self.S_max, self.heads, self.d, ctypes.byref(n)))
-        work = _scratch(n.value, q.device)
-        check(L.zrnn_memory4_attend(e, _ptr(self.codes), _ptr(self.scales), self.B, self.S_max, self.heads, self.d, _ptr(lens), _ptr(offsets),
-                                    _ptr(q), ldq, N // self.B, _ptr(mask01), scale, _ptr(out), ldo, _ptr(work), n.value, _stream()))
+        stream = _here("memory4.attend", q, out, lens, offsets, mask01, self.codes)
+        n = _work_bytes("zrnn_memory4_attend_workspace", q.get_device(), B, N // B, self.S_max, heads, d)
+        work = _scratch(n, q.device)
+        check(lib().zrnn_memory4_attend(e, self.codes.data_ptr(), self.scales.data_ptr(), B, self.S_max, heads, d, lens.data_ptr(), _at(offsets),
+                                        q.data_ptr(), ldq, N // B, _at(mask01), scale, out.data_ptr(), ldo, _at(work), n, stream))
         return out
 
 
@@ -627,22 +645,25 @@ def linear(W, X, bias=None, act="none", residual=None, out=None):
     if act not in ACTIVATIONS:
         raise ValueError(f"linear: act is one of {ACTIVATIONS}")
     if out is None:
-        out = torch.empty(N, n, dtype=X.dtype, device=X.device)
+        out, ldy = torch.empty(N, n, dtype=X.dtype, device=X.device), n
+    else:
+        if out.dtype != X.dtype or out.size(0) != N:
+            raise ValueError("linear: out does not match X")
+        ldy = _rows(out, "linear: out", n)[1]
     ldr = 0
-    for t, name in ((out, "out"), (residual, "residual")):
-        if t is not None and (t.dtype != X.dtype or t.size(0) != N):
-            raise ValueError(f"linear: {name} does not match X")
-    ldy = _rows(out, "linear: out", n)[1]
     if residual is not None:
+        if residual.dtype != X.dtype or residual.size(0) != N:
+            raise ValueError("linear: residual does not match X")
         ldr = _rows(residual, "linear: residual", n)[1]
     if bias is not None:
         _dense(bias, "linear: bias", torch.float32, (n,))
-    _here("linear", W, X, bias, residual, out)
-    L, nb = lib(), ctypes.c_size_t()
-    check(L.zrnn_linear_workspace(e, n, N, W.size(1), _ptr(W), ldw, _ptr(X), ldx, ctypes.byref(nb)))
-    work = _scratch(nb.value, X.device)
-    check(L.zrnn_linear(e, ACTIVATIONS.index(act), n, N, W.size(1), _ptr(W), ldw, _ptr(X), ldx, _ptr(bias), _ptr(residual), ldr, _ptr(out), ldy,
-                        _ptr(work), nb.value, _stream()))
+    stream = _here("linear", W, X, bias, residual, out)
+    K, w, x = W.size(1), W.data_ptr(), X.data_ptr()
+    # (of the addresses the answer depends on the alignment alone)
+    nb = _work_bytes("zrnn_linear_workspace", X.get_device(), e, n, N, K, 4096 + w % 256, ldw, 4096 + x % 256, ldx)
+    work = _scratch(nb, X.device)
+    check(lib().zrnn_linear(e, ACTIVATIONS.index(act), n, N, K, w, ldw, x, ldx, _at(bias), _at(residual), ldr, out.data_ptr(), ldy, _at(work), nb,
+                            stream))
     return out
 
 
@@ -658,15 +679,15 @@ def beam_select(logp, scores, beam, k, lse=None, done=None, eos=1):
     for t, name, dt in ((scores, "scores", torch.float32), (lse, "lse", torch.float32), (done, "done", torch.int32)):
         if t is not None and (t.dtype != dt or t.numel() != rows or not t.is_contiguous()):
             raise ValueError(f"beam_select: {name} must be a contiguous {dt} tensor of {rows} elements")
-    _here("beam_select", logp, scores, lse, done)
-    val = torch.empty(n, k, dtype=torch.float32, device=logp.device)
-    words = torch.empty(n, k, dtype=torch.int32, device=logp.device)
-    parents = torch.empty(n, k, dtype=torch.int32, device=logp.device)
-    L, nb = lib(), ctypes.c_size_t()
-    check(L.zrnn_beam_select_workspace(e, n, beam, logp.size(1), k, ctypes.byref(nb)))
-    work = _scratch(nb.value, logp.device)
-    check(L.zrnn_beam_select(e, _ptr(logp), ld, _ptr(lse), _ptr(scores), _ptr(done), n, beam, logp.size(1), k, eos, _ptr(val), _ptr(words),
-                             _ptr(parents), _ptr(work), nb.value, _stream()))
+    stream = _here("beam_select", logp, scores, lse, done)
+    device, V = logp.device, logp.size(1)
+    val = torch.empty(n, k, dtype=torch.float32, device=device)
+    words = torch.empty(n, k, dtype=torch.int32, device=device)
+    parents = torch.empty(n, k, dtype=torch.int32, device=device)
+    nb = _work_bytes("zrnn_beam_select_workspace", logp.get_device(), e, n, beam, V, k)
+    work = _scratch(nb, device)
+    check(lib().zrnn_beam_select(e, logp.data_ptr(), ld, _at(lse), scores.data_ptr(), _at(done), n, beam, V, k, eos, val.data_ptr(),
+                                 words.data_ptr(), parents.data_ptr(), _at(work), nb, stream))
     return val, words, parents
 
 
@@ -684,14 +705,16 @@ def beam_reorder(states, parents, out=None, group=1):
     if m == 0:
         return out
     n_src = states[0].size(0)
-    src, dst, size = (ctypes.c_void_p * m)(), (ctypes.c_void_p * m)(), (ctypes.c_size_t * m)()
-    for i, (s, o) in enumerate(zip(states, out)):
-        if not s.is_contiguous() or not o.is_contiguous() or s.dtype != o.dtype or s.size(0) != n_src or o.size(0) != n or s.shape[1:] != o.shape[1:]:
+    for s, o in zip(states, out):
+        a, b = s.shape, o.shape
+        if not s.is_contiguous() or not o.is_contiguous() or s.dtype != o.dtype or a[0] != n_src or b[0] != n or (a != b and a[1:] != b[1:]):
             raise ValueError("beam_reorder: states and outputs are contiguous [columns, ...] tensors of the same type and width")
-        src[i], dst[i], size[i] = s.data_ptr(), o.data_ptr(), (o.numel() // n if n else 0) * o.element_size()
-    _here("beam_reorder", parents, *states, *out)
-    check(lib().zrnn_beam_reorder(m, src, dst, size, _ptr(parents), n, n_src, group, _stream()))
+    stream = _here("beam_reorder", parents, *states, *out)
+    P = ctypes.c_void_p * m
+    check(lib().zrnn_beam_reorder(m, P(*[s.data_ptr() for s in states]), P(*[o.data_ptr() for o in out]),
+                                  (ctypes.c_size_t * m)(*[o.nbytes // n if n else 0 for o in out]), parents.data_ptr(), n, n_src, group, stream))
     return out
+
 
 def read_model_file_header(path):
     """(header ints [9], how many the file carried, source vocabulary lines, target vocabulary lines) of a

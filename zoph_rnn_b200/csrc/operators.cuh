@@ -91,6 +91,7 @@ struct BeamSelect {
   float* score_out;            // [n_sent][k]
   int *word_out, *parent_out;
   unsigned long long* work;    // beam_select_work(...) bytes
+  int first_row;               // what is added to the rows in parent_out
 };
 size_t beam_select_work(int elem, int n_sent, int beam, int V, int k);
 cudaError_t launch_beam_select(const BeamSelect& a, int elem, cudaStream_t st);

@@ -3217,7 +3217,7 @@ int zrnn_beam_select(int elem, const void* d_logp, long long ld, const float* d_
            "beam_select: the workspace must hold " + std::to_string(need) + " bytes (16-byte aligned)");
   ZR_TRY(check_device());
   zrnn::BeamSelect a{d_logp, ld, d_lse, d_scores, d_done, n_sent, beam, V, k, eos, d_score_out, d_word_out, d_parent_out,
-                     (unsigned long long*)d_workspace};
+                     (unsigned long long*)d_workspace, 0};
   KScope ks(KC_BEAM, (cudaStream_t)stream);
   ZR_CUDA(zrnn::launch_beam_select(a, elem, (cudaStream_t)stream));
   return ZRNN_OK;
