@@ -1,9 +1,11 @@
 // The source memory in 4 bits: packing, reading back, and attention over it.
 #include <algorithm>
 #include <cstring>
+#include <type_traits>
 
 #include "kernels.cuh"
 #include "operators.cuh"
+#include "tc_gemm.cuh"
 
 namespace zrnn {
 namespace {
@@ -62,43 +64,452 @@ __global__ void __launch_bounds__(256) mem4_unpack_kernel(const Mem4Unpack a) {
   }
 }
 
-__device__ __forceinline__ float mem4_value(const Mem4Attend& a, long long row, int i) {
-  const unsigned c = a.codes[(row + i / kMem4Group) * 16 + (i % kMem4Group) / 2];
-  return __half2float(__float2half_rn((float)((int)((i & 1) ? c >> 4 : c & 15) - 8) * __half2float(a.scales[row + i / kMem4Group])));
+// ---- attention
+// Per source column b, head and tile of 16 target columns: z = Q V^T and softmax(z) V over the slots, in one pass with a running maximum and
+// sum, on the warp-level tensor cores (m16n8k16, half precision in, 32 bits out).  The values q * s are half-precision numbers by
+// definition, so they enter a product exactly; in 32 bits Q and the weights are split into a half and a rest (times 2^11) that is another half.
+//
+// A warp owns NB blocks of 64 elements of the head for the scores and for the output, so that both read the same codes; a team of WT warps
+// covers the head and takes tiles of 32 slots, and a CTA has 16 / WT teams, each with slots of its own.  Per tile: the warps'
+// partial scores meet in shared memory, each warp finishes 16 / WT rows (a lane per slot: maximum, exponential, weights written as the
+// fragments of the second product), and all warps add weights x values to their registers.  Codes come three tiles ahead by
+// asynchronous copies.  What bounds it is the issue of instructions: turning 8 codes into 4 pairs of halves takes 13, twice per code.
+constexpr int kAttWarps = 16, kAttTile = 32, kAttStages = 3, kAttPartLd = 40;
+template <int PARTS, int WT, int NB>
+struct AttShape {
+  static constexpr int TEAMS = kAttWarps / WT, GP = 2 * NB * WT;  // groups that the team's warps have room for
+  static constexpr int ROW = (GP | 1) * 16;                       // bytes of a slot's codes in shared memory: an odd number of 16 spreads them over the banks
+  static constexpr int Q = GP * 2 * PARTS * 512;                  // Q as fragments
+  static constexpr int STAGE = kAttTile * ROW + GP * kAttTile * 2;
+  static constexpr int PART = WT * 16 * kAttPartLd * 4, W = 2 * PARTS * 512;
+  static constexpr int TEAM = kAttStages * STAGE + PART + W + 128;
+  static constexpr int OUT_LD = GP * 32 + 2;                      // floats; the teams' outputs take the place of all that
+  static constexpr int RUN = Q + TEAMS * TEAM, OUT = TEAMS * 16 * OUT_LD * 4;
+  static constexpr int ML = (RUN > OUT ? RUN : OUT), SMEM = ML + 3 * 16 * 16 * 4;
+  static_assert(SMEM <= 227 * 1024 && STAGE % 16 == 0 && TEAM % 16 == 0, "");
+};
+struct AttPlan {
+  int G, warps, blocks;       // groups of a head; WT and NB
+  int q_tiles, splits;
+};
+
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
 }
-// A CTA per column and head, a slot after the other.
-template <class T>
-__global__ void __launch_bounds__(256) mem4_attend_kernel(const Mem4Attend a) {
-  __shared__ float red[8];
-  const int c = blockIdx.x, h = blockIdx.y, b = c / a.cols, tid = threadIdx.x, G = mem4_groups(a.d);
-  const T* q = static_cast<const T*>(a.q) + c * a.ld_q + (long long)h * a.d;
-  T* out = static_cast<T*>(a.out) + c * a.ld_out + (long long)h * a.d;
+__device__ __forceinline__ void mma_f16_first(float (&c)[4], const uint4& a, uint32_t b0, uint32_t b1) {  // onto zeros
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+               : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+               : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ float exp2_approx(float x) {  // within 2 units of the last place
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float warp_max(float x) {
+  float y;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+__device__ __forceinline__ __half2 bits_h2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
+// Nibbles 0 .. 3 of each half of x, as pairs (low half, high half) of q * s: 1024 + u and 1024 + 16 u are halves made by or-ing u into a
+// mantissa, and what follows is exact but for the last product, whose rounding is the definition's.
+__device__ __forceinline__ void dequant4(uint32_t x, __half2 s, uint32_t (&v)[4]) {
+  const __half2 m1032 = __half2half2(__ushort_as_half(0xe408)), sixteenth = __half2half2(__ushort_as_half(0x2c00)), m72 = __half2half2(__ushort_as_half(0xd480));
+  const uint32_t y = x >> 8;
+  uint32_t a, b, c, d;
+  asm("lop3.b32 %0, %1, 0x000f000f, 0x64006400, 0xea;" : "=r"(a) : "r"(x));
+  asm("lop3.b32 %0, %1, 0x00f000f0, 0x64006400, 0xea;" : "=r"(b) : "r"(x));
+  asm("lop3.b32 %0, %1, 0x000f000f, 0x64006400, 0xea;" : "=r"(c) : "r"(y));
+  asm("lop3.b32 %0, %1, 0x00f000f0, 0x64006400, 0xea;" : "=r"(d) : "r"(y));
+  v[0] = h2_bits(__hmul2_rn(__hadd2_rn(bits_h2(a), m1032), s));
+  v[1] = h2_bits(__hmul2_rn(__hfma2(bits_h2(b), sixteenth, m72), s));
+  v[2] = h2_bits(__hmul2_rn(__hadd2_rn(bits_h2(c), m1032), s));
+  v[3] = h2_bits(__hmul2_rn(__hfma2(bits_h2(d), sixteenth, m72), s));
+}
+// x as a half and, times 2^11, what that leaves
+__device__ __forceinline__ void split_half(float x, __half& hi, __half& lo) {
+  hi = __float2half_rn(x);
+  lo = __float2half_rn((x - __half2float(hi)) * 2048.f);
+}
+__device__ __forceinline__ uint32_t shared_at(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void copy16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(shared_at(dst)), "l"(src) : "memory");
+}
+
+template <class T, int WT, int NB>
+__global__ void __launch_bounds__(kAttWarps * 32, 1) mem4_attend_kernel(const Mem4Attend a, const AttPlan pl) {
+  constexpr int PARTS = std::is_same<T, float>::value ? 2 : 1, ROWS = 16 / WT;
+  using Sh = AttShape<PARTS, WT, NB>;
+  constexpr int TEAMS = Sh::TEAMS, GP = Sh::GP, ROW = Sh::ROW;
+  extern __shared__ __align__(16) unsigned char smem[];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // (the combination waits for this launch's end before it reads anything)
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, team = warp / WT, wt = warp % WT;
+  const int g = lane >> 2, t = lane & 3, G = pl.G;
+  const int b = blockIdx.y / pl.q_tiles, c0 = blockIdx.y % pl.q_tiles * 16, h = blockIdx.z, split = blockIdx.x;
+  const int n_cols = min(16, a.cols - c0);
+  unsigned char* s_q = smem;
+  unsigned char* s_team = smem + Sh::Q + team * Sh::TEAM;
+  float* s_part = reinterpret_cast<float*>(s_team + kAttStages * Sh::STAGE);
+  unsigned char* s_w = s_team + kAttStages * Sh::STAGE + Sh::PART;
+  float* s_alpha = reinterpret_cast<float*>(s_w + Sh::W);
+  float* s_m = s_alpha + 16;  // running maxima
+  float* s_ml = reinterpret_cast<float*>(smem + Sh::ML);  // [team][16]: maxima, sums; then [16]: factors of the queries
+  float* s_fac = s_ml + 2 * 16 * 16;
+
+  // Q of row `warp`, all of it requested at once
+  const bool in = warp < n_cols;
+  float qx[GP];
+  {
+    const T* q = static_cast<const T*>(a.q) + ((long long)b * a.cols + c0 + (in ? warp : 0)) * a.ld_q + (long long)h * a.d + lane;
+#pragma unroll
+    for (int k = 0; k < GP; ++k) qx[k] = in && k * 32 + lane < a.d ? to_f32(__ldg(q + k * 32)) : 0.f;
+  }
+  // the slots of this CTA: whole tiles of 32 from the window's first slot on
   const long long off = a.offset ? a.offset[b] : 0;
-  const int lo = (int)max(off, 0ll), hi = (int)min(off + a.len[b], (long long)a.S_cap);
-  float m = -INFINITY, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f}, qv[4];
-  for (int u = 0; u < 4; ++u) qv[u] = tid + 256 * u < a.d ? to_f32(q[tid + 256 * u]) : 0.f;
-  if (!a.mask || a.mask[c] != 0)
-    for (int s = lo; s < hi; ++s) {
-      const long long row = (((long long)b * a.S_cap + s) * a.heads + h) * G;
-      float v[4], z = 0.f;
-      for (int u = 0; u < 4; ++u) {
-        v[u] = tid + 256 * u < a.d ? mem4_value(a, row, tid + 256 * u) : 0.f;
-        z += qv[u] * v[u];
+  const int lo = (int)max(off, 0ll), hi = (int)min(max(off + a.len[b], 0ll), (long long)a.S_cap);
+  const int tiles = hi > lo ? (hi - lo + kAttTile - 1) / kAttTile : 0;
+  const int t0 = (int)((long long)tiles * split / pl.splits), t1 = (int)((long long)tiles * (split + 1) / pl.splits);
+  const int my = t1 - t0 > team ? (t1 - t0 - team + TEAMS - 1) / TEAMS : 0;  // tiles t0 + team, + TEAMS, ...
+
+  // a thread copies chunk cq (16 bytes, one group) of the slots cp, cp + 8, .. + 24 of a tile (where the team has 128 threads per NB = 2; half
+  // of that: eight slots), and their scales, which lie as [group][slot % 8][slot / 8]
+  constexpr int CPY = kAttTile * GP / (WT * 32);  // 2 or 4 slots per thread
+  constexpr int STEP = kAttTile / CPY;
+  const int tw = wt * 32 + lane, cp = tw / GP, cq = tw % GP;
+  const bool copies = cq < G;
+  const size_t row_codes = (size_t)a.heads * G * 16, row_scales = (size_t)a.heads * G;
+  const uint8_t* codes = a.codes + ((size_t)b * a.S_cap + cp) * row_codes + (size_t)h * G * 16 + cq * 16;
+  const unsigned short* scales = reinterpret_cast<const unsigned short*>(a.scales) + ((size_t)b * a.S_cap + cp) * row_scales + (size_t)h * G + cq;
+  unsigned short sc_next[CPY];
+  auto request = [&](int it) {
+    if (it < my && copies) {
+      const int p0 = lo + (t0 + team + it * TEAMS) * kAttTile, n = hi - p0;
+      unsigned char* st = s_team + it % kAttStages * Sh::STAGE + cp * ROW + cq * 16;
+      const uint8_t* from = codes + (size_t)p0 * row_codes;
+      const unsigned short* sf = scales + (size_t)p0 * row_scales;
+#pragma unroll
+      for (int u = 0; u < CPY; ++u) {
+        if (cp + STEP * u < n) copy16(st + STEP * u * ROW, from + STEP * u * row_codes);
+        sc_next[u] = cp + STEP * u < n ? __ldg(sf + STEP * u * row_scales) : (unsigned short)0;
       }
-      for (int o = 16; o; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
-      __syncthreads();
-      if ((tid & 31) == 0) red[tid >> 5] = z;
-      __syncthreads();
-      z = 0.f;
-      for (int w = 0; w < 8; ++w) z += red[w];
-      z *= a.scale;
-      const float mn = fmaxf(m, z), al = m == -INFINITY ? 0.f : expf(m - mn), p = expf(z - mn);
-      m = mn;
-      l = l * al + p;
-      for (int u = 0; u < 4; ++u) acc[u] = acc[u] * al + p * v[u];
     }
-  for (int u = 0; u < 4; ++u)
-    if (tid + 256 * u < a.d) out[tid + 256 * u] = from_f32<T>(l == 0.f ? 0.f : acc[u] / l);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  auto keep_scales = [&](int it) {  // slots outside the window get 0: their codes, whatever they are, stand for 0
+    if (it < my && copies) {
+      unsigned short* st = reinterpret_cast<unsigned short*>(s_team + it % kAttStages * Sh::STAGE + kAttTile * ROW) + cq * kAttTile;
+#pragma unroll
+      for (int u = 0; u < CPY; ++u) {
+        const int p = cp + STEP * u;
+        st[(p & 7) * 4 + (p >> 3)] = sc_next[u];
+      }
+    }
+  };
+  auto team_sync = [&]() {
+    if (WT == 1) __syncwarp();
+    else asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "n"(WT * 32) : "memory");
+  };
+  request(0);
+  if (cq >= G)  // groups that the head does not have
+    for (int u = 0; u < CPY; ++u)
+      for (int k = 0; k < kAttStages; ++k) {
+        const int p = cp + STEP * u;
+        reinterpret_cast<unsigned short*>(s_team + k * Sh::STAGE + kAttTile * ROW)[cq * kAttTile + (p & 7) * 4 + (p >> 3)] = 0;
+      }
+
+  // Q scaled by a power of two to at most 1; element e of a thread's word of 8 is half e / 4 of register 2 (e % 2) (+ 1: rows 8 .. 15) of k-step
+  // (e % 4) / 2, so that a word of codes gives its fragments by masks alone
+  {
+    unsigned m = 0;
+#pragma unroll
+    for (int k = 0; k < GP; ++k) m = max(m, __float_as_uint(qx[k]) & 0x7fffffffu);
+    m = __reduce_max_sync(0xffffffffu, m);
+    int e = 0;
+    if (m != 0) frexpf(__uint_as_float(m), &e);
+    const float down1 = ldexpf(1.f, -(e / 2)), down2 = ldexpf(1.f, -(e - e / 2));
+    const int el = lane & 7, tt = lane >> 3;
+    unsigned char* at = s_q + ((el & 3) / 2 * PARTS) * 512 + ((warp & 7) * 4 + tt) * 16 + ((el & 1) * 2 + (warp >> 3)) * 4 + (el >> 2) * 2;
+#pragma unroll
+    for (int k = 0; k < GP; ++k) {
+      __half x0, x1;
+      split_half(qx[k] * down1 * down2, x0, x1);
+      *reinterpret_cast<__half*>(at + k * 2 * PARTS * 512) = x0;
+      if (PARTS == 2) *reinterpret_cast<__half*>(at + k * 2 * PARTS * 512 + 512) = x1;
+    }
+    if (lane == 0) s_fac[warp] = ldexpf(a.scale * 1.44269504f, e);  // (exponentials are powers of two)
+  }
+  keep_scales(0);
+  request(1);
+  __syncthreads();
+
+  float acc[NB][8][4], l[4] = {0.f, 0.f, 0.f, 0.f};  // l: the weights' sums, as a product with ones (columns alike)
+#pragma unroll
+  for (int x = 0; x < NB; ++x)
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) acc[x][j][u] = 0.f;
+  if (wt == 0 && lane < 16) s_m[lane] = -INFINITY;
+  keep_scales(1);
+
+  for (int it = 0; it < my; ++it) {
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    team_sync();  // the tile is there for all, and all are done with the one before
+    request(it + 2);
+    const unsigned char* st = s_team + it % kAttStages * Sh::STAGE;
+    const unsigned char* s_sc = st + kAttTile * ROW;
+    const int n = hi - (lo + (t0 + team + it * TEAMS) * kAttTile);
+    // scores of this warp's elements; n-tile j has slot 8 j + c in its column c
+    {
+      float z[PARTS][4][4];
+      const unsigned char* cw = st + g * ROW + wt * (2 * NB * 16) + t * 4;
+#pragma unroll
+      for (int k = 0; k < 2 * NB; ++k) {
+        uint4 q[2][PARTS];
+        const int kg = wt * 2 * NB + k;
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int x = 0; x < PARTS; ++x) q[s][x] = *reinterpret_cast<const uint4*>(s_q + ((kg * 2 + s) * PARTS + x) * 512 + lane * 16);
+        const uint2 sc4 = *reinterpret_cast<const uint2*>(s_sc + kg * (kAttTile * 2) + g * 8);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t w = *reinterpret_cast<const uint32_t*>(cw + 8 * j * ROW + k * 16);
+          uint32_t v[4];  // (elements 0, 4), (1, 5), (2, 6), (3, 7) of the word
+          dequant4(w, bits_h2(__byte_perm(j < 2 ? sc4.x : sc4.y, 0, j & 1 ? 0x3232 : 0x1010)), v);
+#pragma unroll
+          for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int x = 0; x < PARTS; ++x) {
+              if (k == 0 && s == 0) mma_f16_first(z[x][j], q[s][x], v[2 * s], v[2 * s + 1]);
+              else mma_f16(z[x][j], q[s][x], v[2 * s], v[2 * s + 1]);
+            }
+        }
+      }
+      float* at = s_part + (wt * 16 + g) * kAttPartLd + 2 * t;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float y[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) y[u] = PARTS == 2 ? fmaf(z[PARTS - 1][j][u], 1.f / 2048.f, z[0][j][u]) : z[0][j][u];
+        *reinterpret_cast<float2*>(at + 8 * j) = make_float2(y[0], y[1]);
+        *reinterpret_cast<float2*>(at + 8 * j + 8 * kAttPartLd) = make_float2(y[2], y[3]);
+      }
+    }
+    team_sync();
+    // softmax: row r of this warp, slot `lane`; as the second product's k, slot 8 j + c is half j % 2 of register 2 (j / 2) (+ 1: rows 8 .. 15) of lane
+    // c / 2 (of a row's four), k-step c % 2, so that a thread's four scales lie side by side
+    {
+      unsigned char* at0 = s_w + (lane & 1) * PARTS * 512 + (lane & 7) / 2 * 16 + (lane >> 4) * 8 + (lane >> 3 & 1) * 2;
+#pragma unroll
+      for (int rr = 0; rr < ROWS; ++rr) {
+        const int r = wt * ROWS + rr;
+        float z = 0.f;
+#pragma unroll
+        for (int w = 0; w < WT; ++w) z += s_part[(w * 16 + r) * kAttPartLd + lane];
+        z = lane < n ? z * s_fac[r] : -INFINITY;
+        const float m_old = s_m[r], m_new = fmaxf(m_old, warp_max(z)), ref = m_new == -INFINITY ? 0.f : m_new;
+        const float alpha = exp2_approx(m_old - ref), p = exp2_approx(z - ref);
+        __syncwarp();
+        if (lane == 0) {
+          s_alpha[r] = alpha;
+          s_m[r] = m_new;
+        }
+        __half p0h, p1h;
+        split_half(p, p0h, p1h);
+        unsigned char* at = at0 + (r & 7) * 64 + (r >> 3) * 4;
+        *reinterpret_cast<__half*>(at) = p0h;
+        if (PARTS == 2) *reinterpret_cast<__half*>(at + 512) = p1h;
+      }
+    }
+    team_sync();
+    // weights x values: n-tile j of a block has element 8 c + j of the block in its column c
+    {
+      uint4 w[2][PARTS];
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int x = 0; x < PARTS; ++x) w[s][x] = *reinterpret_cast<const uint4*>(s_w + (s * PARTS + x) * 512 + lane * 16);
+      const float al0 = s_alpha[g], al1 = s_alpha[g + 8];
+      // With 16-bit operands the products go straight onto the accumulators, which are rescaled where a maximum rose.  The tensor core cuts its
+      // sums off: 2^-23 per tile, which 32 bits of result would show, so those add the tile's sums in the ordinary way.
+      if (PARTS == 1 && __any_sync(0xffffffffu, al0 != 1.f || al1 != 1.f)) {
+#pragma unroll
+        for (int x = 0; x < NB; ++x)
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int u = 0; u < 4; ++u) acc[x][j][u] *= u < 2 ? al0 : al1;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) l[u] *= u < 2 ? al0 : al1;
+      }
+      {
+        constexpr uint32_t ones = 0x3c003c00u;
+        if (PARTS == 1) {
+          mma_f16(l, w[0][0], ones, ones);
+          mma_f16(l, w[1][0], ones, ones);
+        } else {
+          float y[4];
+          mma_f16_first(y, w[0][PARTS - 1], ones, ones);
+          mma_f16(y, w[1][PARTS - 1], ones, ones);
+#pragma unroll
+          for (int u = 0; u < 4; ++u) y[u] *= 1.f / 2048.f;
+          mma_f16(y, w[0][0], ones, ones);
+          mma_f16(y, w[1][0], ones, ones);
+#pragma unroll
+          for (int u = 0; u < 4; ++u) l[u] = fmaf(l[u], u < 2 ? al0 : al1, y[u]);
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < NB; ++x) {
+        const int blk = wt * NB + x;
+        const unsigned char* at = st + 2 * t * ROW + blk * 32 + g * 4;
+        uint32_t cw[2][4];
+        uint2 sc[2];
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+#pragma unroll
+          for (int u = 0; u < 4; ++u) cw[s][u] = *reinterpret_cast<const uint32_t*>(at + (s + 8 * u) * ROW);
+          sc[s] = *reinterpret_cast<const uint2*>(s_sc + (2 * blk + (g >> 2)) * (kAttTile * 2) + (2 * t + s) * 8);
+        }
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          uint32_t v[2][2][4];
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            dequant4(__byte_perm(cw[s][0], cw[s][1], half ? 0x7632 : 0x5410), bits_h2(sc[s].x), v[s][0]);
+            dequant4(__byte_perm(cw[s][2], cw[s][3], half ? 0x7632 : 0x5410), bits_h2(sc[s].y), v[s][1]);
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float (&o)[4] = acc[x][half * 4 + j];
+            if (PARTS == 1) {
+              mma_f16(o, w[0][0], v[0][0][j], v[0][1][j]);
+              mma_f16(o, w[1][0], v[1][0][j], v[1][1][j]);
+            } else {
+              float y[4];
+              mma_f16_first(y, w[0][PARTS - 1], v[0][0][j], v[0][1][j]);
+              mma_f16(y, w[1][PARTS - 1], v[1][0][j], v[1][1][j]);
+#pragma unroll
+              for (int u = 0; u < 4; ++u) y[u] *= 1.f / 2048.f;
+              mma_f16(y, w[0][0], v[0][0][j], v[0][1][j]);
+              mma_f16(y, w[1][0], v[1][0][j], v[1][1][j]);
+#pragma unroll
+              for (int u = 0; u < 4; ++u) o[u] = fmaf(o[u], u < 2 ? al0 : al1, y[u]);
+            }
+          }
+        }
+      }
+    }
+    keep_scales(it + 2);
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+
+  // the teams' maxima and sums, then their outputs side by side
+  team_sync();
+  if (wt == 0) {
+    if (lane < 16) s_ml[team * 16 + lane] = s_m[lane];
+    if (t == 0) {
+      s_ml[256 + team * 16 + g] = l[0];
+      s_ml[256 + team * 16 + g + 8] = l[2];
+    }
+  }
+  __syncthreads();  // (also: nobody reads the fragments and stages any more)
+  float* s_out = reinterpret_cast<float*>(smem);
+  const int busy = min(TEAMS, t1 - t0);
+  if (team < busy) {
+    float* o = s_out + (team * 16 + g) * Sh::OUT_LD + 16 * t;
+#pragma unroll
+    for (int x = 0; x < NB; ++x)
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) o[(u >> 1) * 8 * Sh::OUT_LD + (wt * NB + x) * 64 + 8 * (u & 1) + j] = acc[x][j][u];
+  }
+  __syncthreads();
+  // row r: warp r
+  if (!in) return;
+  float m = -INFINITY, sum = 0.f, f[TEAMS];
+#pragma unroll
+  for (int k = 0; k < TEAMS; ++k) m = fmaxf(m, s_ml[k * 16 + warp]);
+#pragma unroll
+  for (int k = 0; k < TEAMS; ++k) {
+    f[k] = k < busy ? exp2f(s_ml[k * 16 + warp] - (m == -INFINITY ? 0.f : m)) : 0.f;
+    if (k < busy) sum += s_ml[256 + k * 16 + warp] * f[k];
+  }
+  const long long c = (long long)b * a.cols + c0 + warp;
+  const bool part = pl.splits > 1, on = sum != 0.f && (!a.mask || a.mask[c] != 0);
+  const int dp = G * 32;
+  float* w = part ? a.work + (((long long)blockIdx.y * a.heads + h) * pl.splits + split) * 16 * (dp + 2) + warp * (dp + 2) : nullptr;
+  T* out = static_cast<T*>(a.out) + c * a.ld_out + (long long)h * a.d;
+  if (part && lane == 0) { w[0] = m; w[1] = sum; }
+#pragma unroll 4
+  for (int k0 = 0; k0 < GP; ++k0) {
+    const int i = k0 * 32 + lane;
+    float y = 0.f;
+#pragma unroll
+    for (int k = 0; k < TEAMS; ++k)
+      if (k < busy) y = fmaf(s_out[(k * 16 + warp) * Sh::OUT_LD + i], f[k], y);
+    if (part) {
+      if (i < dp) w[2 + i] = y;
+    } else if (i < a.d) {
+      out[i] = from_f32<T>(on ? y / sum : 0.f);
+    }
+  }
+}
+// The parts of a column and head: their weights first, then a thread per element
+constexpr int kMostSplits = 1024;
+template <class T>
+__global__ void __launch_bounds__(256) mem4_combine_kernel(const Mem4Attend a, const AttPlan pl) {
+  __shared__ float s_f[kMostSplits], s_red[8];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int tid = threadIdx.x, h = blockIdx.y, dp = pl.G * 32;
+  const long long c = blockIdx.x, b = c / a.cols;
+  const int at = (int)(c - b * a.cols);
+  const float* w = a.work + ((b * pl.q_tiles + at / 16) * a.heads + h) * pl.splits * 16 * (dp + 2) + (at % 16) * (dp + 2);
+  const long long step = 16ll * (dp + 2);
+  float m = -INFINITY;
+  for (int s = tid; s < pl.splits; s += 256) {
+    const float x = __ldcg(w + s * step);
+    s_f[s] = x;
+    m = fmaxf(m, x);
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if ((tid & 31) == 0) s_red[tid >> 5] = m;
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 8; ++k) m = fmaxf(m, s_red[k]);
+  __syncthreads();
+  float l = 0.f;
+  for (int s = tid; s < pl.splits; s += 256) {
+    const float f = exp2f(s_f[s] - (m == -INFINITY ? 0.f : m));
+    s_f[s] = f;
+    if (f != 0.f) l += __ldcg(w + s * step + 1) * f;
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+  if ((tid & 31) == 0) s_red[tid >> 5] = l;
+  __syncthreads();
+  l = 0.f;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) l += s_red[k];
+  // (l is 0 only where no part had a slot: a NaN among the weights is one here, too)
+  const bool on = l != 0.f && (!a.mask || a.mask[c] != 0);
+  T* out = static_cast<T*>(a.out) + c * a.ld_out + (long long)h * a.d;
+  for (int i = tid; i < a.d; i += 256) {
+    float y = 0.f;
+#pragma unroll 4
+    for (int s = 0; s < pl.splits; ++s) {
+      const float x = __ldcg(w + s * step + 2 + i), f = s_f[s];
+      y = f != 0.f ? fmaf(x, f, y) : y;
+    }
+    out[i] = from_f32<T>(on ? y / l : 0.f);
+  }
 }
 
 }  // namespace
@@ -127,17 +538,86 @@ cudaError_t launch_mem4_unpack(const Mem4Unpack& a, int elem, cudaStream_t st) {
   }
   return cudaGetLastError();
 }
-size_t mem4_attend_work(int, int, int, int, int) { return 0; }
+namespace {
+
+// Splits: CTAs for every multiprocessor, but at least two tiles for each team of a part.
+AttPlan att_plan(int B, int cols, int S_cap, int heads, int d) {
+  AttPlan pl;
+  pl.G = mem4_groups(d);
+  pl.warps = pl.G <= 4 ? 1 : pl.G <= 8 ? 2 : pl.G <= 16 ? 4 : 8;
+  pl.blocks = pl.G <= 2 ? 1 : 2;
+  pl.q_tiles = (cols + 15) / 16;
+  const long long units = (long long)B * pl.q_tiles * heads, most = S_cap / (kAttTile * 2 * (kAttWarps / pl.warps));
+  pl.splits = (int)std::max<long long>(1, std::min<long long>(std::min<long long>(device_sms() / units, kMostSplits), most));
+  return pl;
+}
+template <class T, int WT, int NB>
+cudaError_t attend_launch(const Mem4Attend& a, const AttPlan& pl, cudaStream_t st) {
+  constexpr int smem = AttShape<std::is_same<T, float>::value ? 2 : 1, WT, NB>::SMEM;
+  static bool configured[64] = {false};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
+  if (!configured[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(mem4_attend_kernel<T, WT, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    configured[dev] = true;
+  }
+  mem4_attend_kernel<T, WT, NB><<<dim3(pl.splits, (unsigned)(a.B * pl.q_tiles), (unsigned)a.heads), kAttWarps * 32, smem, st>>>(a, pl);
+  return cudaGetLastError();
+}
+template <class T>
+cudaError_t attend_type(const Mem4Attend& all, cudaStream_t st) {
+  const AttPlan pl = att_plan(all.B, all.cols, all.S_cap, all.heads, all.d);
+  const int most = 65535 / pl.q_tiles;  // source columns of a launch
+  if (most < 1) return cudaErrorInvalidValue;
+  for (int at = 0; at < all.B; at += most) {
+    Mem4Attend a = all;
+    a.B = std::min(most, all.B - at);
+    const size_t rows = (size_t)at * a.S_cap * a.heads * pl.G;
+    const long long cols = (long long)at * a.cols;
+    a.codes += rows * 16;
+    a.scales += rows;
+    a.len += at;
+    if (a.offset) a.offset += at;
+    if (a.mask) a.mask += cols;
+    a.q = static_cast<const T*>(a.q) + cols * a.ld_q;
+    a.out = static_cast<T*>(a.out) + cols * a.ld_out;
+    count_launch();
+    const cudaError_t e = pl.blocks == 1 ? attend_launch<T, 1, 1>(a, pl, st) : pl.warps == 1 ? attend_launch<T, 1, 2>(a, pl, st)
+                          : pl.warps == 2 ? attend_launch<T, 2, 2>(a, pl, st) : pl.warps == 4 ? attend_launch<T, 4, 2>(a, pl, st)
+                                                                                             : attend_launch<T, 8, 2>(a, pl, st);
+    if (e != cudaSuccess) return e;
+    if (pl.splits == 1) continue;
+    cudaLaunchConfig_t cfg;
+    std::memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim = dim3((unsigned)(a.B * a.cols), a.heads);
+    cfg.blockDim = dim3(256);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    count_launch();
+    const cudaError_t e2 = cudaLaunchKernelEx(&cfg, mem4_combine_kernel<T>, a, pl);
+    if (e2 != cudaSuccess) return e2;
+  }
+  return cudaSuccess;
+}
+
+}  // namespace
+
+size_t mem4_attend_work(int B, int cols, int S_cap, int heads, int d) {
+  const AttPlan pl = att_plan(B, cols, S_cap, heads, d);
+  return pl.splits > 1 ? (size_t)B * pl.q_tiles * heads * pl.splits * 16 * (pl.G * 32 + 2) : 0;
+}
 cudaError_t launch_mem4_attend(const Mem4Attend& a, int elem, cudaStream_t st) {
   if (a.B == 0 || a.cols == 0) return cudaSuccess;
-  const dim3 grid((unsigned)(a.B * a.cols), (unsigned)a.heads);
-  count_launch();
   switch (elem) {
-    case ELEM_F32: mem4_attend_kernel<float><<<grid, 256, 0, st>>>(a); break;
-    case ELEM_BF16: mem4_attend_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(a); break;
-    default: mem4_attend_kernel<__half><<<grid, 256, 0, st>>>(a);
+    case ELEM_F32: return attend_type<float>(a, st);
+    case ELEM_BF16: return attend_type<__nv_bfloat16>(a, st);
   }
-  return cudaGetLastError();
+  return attend_type<__half>(a, st);
 }
 
 }  // namespace zrnn

@@ -3107,7 +3107,7 @@ int zrnn_memory4_unpack(int elem, const void* d_codes, const void* d_scales, int
 int zrnn_memory4_attend_workspace(int B, int cols_per_sentence, int S_cap, int heads, int d, size_t* bytes) {
   ZR_CHECK(bytes, "memory4_attend_workspace: null argument");
   ZR_TRY(mem4_check("memory4_attend_workspace", ZRNN_ELEM_F32, B, S_cap, heads, d));
-  ZR_CHECK(cols_per_sentence >= 1, "memory4_attend_workspace: cols_per_sentence must be positive");
+  ZR_CHECK(cols_per_sentence >= 1 && cols_per_sentence <= 1000000, "memory4_attend_workspace: cols_per_sentence must be in [1, 1000000]");
   ZR_CHECK(d <= zrnn::kMem4MaxHead, "memory4_attend_workspace: a head of more than 1024 elements");
   *bytes = zrnn::mem4_attend_work(B, cols_per_sentence, S_cap, heads, d) * sizeof(float);
   return ZRNN_OK;
@@ -3117,7 +3117,8 @@ int zrnn_memory4_attend(int elem, const void* d_codes, const void* d_scales, int
                         long long ld_out, void* d_workspace, size_t workspace_bytes, void* stream) {
   ZR_TRY(mem4_check("memory4_attend", elem, B, S_cap, heads, d));
   ZR_CHECK(d <= zrnn::kMem4MaxHead, "memory4_attend: a head of more than 1024 elements");
-  ZR_CHECK(cols_per_sentence >= 1 && (long long)B * cols_per_sentence <= 0x7fffffff, "memory4_attend: bad number of columns");
+  ZR_CHECK(cols_per_sentence >= 1 && cols_per_sentence <= 1000000 && (long long)B * cols_per_sentence <= 0x7fffffff,
+           "memory4_attend: bad number of columns");
   ZR_CHECK(d_codes && d_scales && d_len && d_q && d_out, "memory4_attend: null pointer");
   const long long width = (long long)heads * d, N = (long long)B * cols_per_sentence;
   ZR_CHECK(ld_q >= width && ld_out >= width, "memory4_attend: leading dimension too small");
