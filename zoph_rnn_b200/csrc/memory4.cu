@@ -172,7 +172,8 @@ __global__ void __launch_bounds__(kAttWarps * 32, 1) mem4_attend_kernel(const Me
   const long long off = a.offset ? a.offset[b] : 0;
   const int lo = (int)max(off, 0ll), hi = (int)min(max(off + a.len[b], 0ll), (long long)a.S_cap);
   const int tiles = hi > lo ? (hi - lo + kAttTile - 1) / kAttTile : 0;
-  const int t0 = (int)((long long)tiles * split / pl.splits), t1 = (int)((long long)tiles * (split + 1) / pl.splits);
+  const int share = pl.splits == 1 ? tiles : tiles / pl.splits, more = tiles - share * pl.splits;
+  const int t0 = split * share + min(split, more), t1 = t0 + share + (split < more);
   const int my = t1 - t0 > team ? (t1 - t0 - team + TEAMS - 1) / TEAMS : 0;  // tiles t0 + team, + TEAMS, ...
 
   // a thread copies chunk cq (16 bytes, one group) of the slots cp, cp + 8, .. + 24 of a tile (where the team has 128 threads per NB = 2; half
@@ -232,7 +233,8 @@ __global__ void __launch_bounds__(kAttWarps * 32, 1) mem4_attend_kernel(const Me
     if (m != 0) frexpf(__uint_as_float(m), &e);
     const float down1 = ldexpf(1.f, -(e / 2)), down2 = ldexpf(1.f, -(e - e / 2));
     const int el = lane & 7, tt = lane >> 3;
-    unsigned char* at = s_q + ((el & 3) / 2 * PARTS) * 512 + ((warp & 7) * 4 + tt) * 16 + ((el & 1) * 2 + (warp >> 3)) * 4 + (el >> 2) * 2;
+    // (the fragments of odd k-steps have neighbouring rows exchanged: the two k-steps that a warp writes at once fall on different banks)
+    unsigned char* at = s_q + ((el & 3) / 2 * PARTS) * 512 + (((warp & 7) * 4 + tt) ^ ((el & 2) * 2)) * 16 + ((el & 1) * 2 + (warp >> 3)) * 4 + (el >> 2) * 2;
 #pragma unroll
     for (int k = 0; k < GP; ++k) {
       __half x0, x1;
@@ -274,7 +276,7 @@ __global__ void __launch_bounds__(kAttWarps * 32, 1) mem4_attend_kernel(const Me
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
-          for (int x = 0; x < PARTS; ++x) q[s][x] = *reinterpret_cast<const uint4*>(s_q + ((kg * 2 + s) * PARTS + x) * 512 + lane * 16);
+          for (int x = 0; x < PARTS; ++x) q[s][x] = *reinterpret_cast<const uint4*>(s_q + ((kg * 2 + s) * PARTS + x) * 512 + (lane ^ (4 * s)) * 16);
         const uint2 sc4 = *reinterpret_cast<const uint2*>(s_sc + kg * (kAttTile * 2) + g * 8);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -447,17 +449,26 @@ __global__ void __launch_bounds__(kAttWarps * 32, 1) mem4_attend_kernel(const Me
   float* w = part ? a.work + (((long long)blockIdx.y * a.heads + h) * pl.splits + split) * 16 * (dp + 2) + warp * (dp + 2) : nullptr;
   T* out = static_cast<T*>(a.out) + c * a.ld_out + (long long)h * a.d;
   if (part && lane == 0) { w[0] = m; w[1] = sum; }
-#pragma unroll 4
-  for (int k0 = 0; k0 < GP; ++k0) {
-    const int i = k0 * 32 + lane;
-    float y = 0.f;
+  const float inv = on ? 1.f / sum : 0.f;
+  constexpr int AT_ONCE = GP < 8 ? GP : 8;
+  for (int k0 = 0; k0 < GP; k0 += AT_ONCE) {
+    float y[AT_ONCE];
 #pragma unroll
-    for (int k = 0; k < TEAMS; ++k)
-      if (k < busy) y = fmaf(s_out[(k * 16 + warp) * Sh::OUT_LD + i], f[k], y);
-    if (part) {
-      if (i < dp) w[2 + i] = y;
-    } else if (i < a.d) {
-      out[i] = from_f32<T>(on ? y / sum : 0.f);
+    for (int u = 0; u < AT_ONCE; ++u) y[u] = 0.f;
+#pragma unroll
+    for (int k = 0; k < TEAMS; ++k) {
+      if (k >= busy) break;
+#pragma unroll
+      for (int u = 0; u < AT_ONCE; ++u) y[u] = fmaf(s_out[(k * 16 + warp) * Sh::OUT_LD + (k0 + u) * 32 + lane], f[k], y[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < AT_ONCE; ++u) {
+      const int i = (k0 + u) * 32 + lane;
+      if (part) {
+        if (i < dp) w[2 + i] = y[u];
+      } else if (i < a.d) {
+        out[i] = from_f32<T>(on ? y[u] * inv : 0.f);
+      }
     }
   }
 }
