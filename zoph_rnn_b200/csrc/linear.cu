@@ -1,56 +1,429 @@
-// Y = act(W X + bias) + R.
+// Y = act(W X + bias) + R for more than a few columns, on tcgen05.
+//
+// A tile is 128 outputs (the M side: a lane of tensor memory per output, so that a warp stores 32 consecutive ones of a column) x nb columns, on one
+// CTA; where there are enough of them, 256 x nb on a pair of CTAs that share the MMAs and hold half of the columns' operand each
+// (tc_pair_device.cuh).  One warp brings the k-blocks of 128 bytes by TMA, one issues the MMAs, sixteen take the accumulators
+// through bias, activation and residual while the next tile's MMAs run; persistent.
+//
+// 32-bit operands go as two tf32 parts each and three products (hi hi; lo hi and hi lo into an accumulator of their own).  The tensor cores
+// ignore the bits below tf32, so the tile that TMA brought is the hi part as it is; four warps write the lo part of each stage beside
+// it, element by element, whatever the swizzle.  A tensor-core accumulator cuts its sums off, so the hi products of four k-blocks
+// (16 additions) go into a fresh one, two in turn, and the sixteen warps add those up in ordinary 32-bit arithmetic.
+//
+// A CTA asks for all of an SM's shared memory, so that a pair's allocation of tensor memory waits for nobody that could wait for it in turn.
 #include <algorithm>
+#include <cstdint>
 #include <cstring>
 
 #include "kernels.cuh"
 #include "linear_device.cuh"
 #include "operators.cuh"
+#include "tc_pair_device.cuh"
 
 namespace zrnn {
 namespace {
 
-// 32 outputs x 32 columns per CTA of 256 threads, four columns per thread
-template <class T>
-__global__ void __launch_bounds__(256) linear_simple_kernel(const LinearArgs a) {
-  __shared__ float w[32][33], x[32][33];
-  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  const long long i0 = (long long)blockIdx.x * 32, c0 = (long long)blockIdx.y * 32;
-  float acc[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int k0 = 0; k0 < a.K; k0 += 32) {
-    for (int r = ty; r < 32; r += 8) {
-      w[r][tx] = i0 + r < a.n && k0 + tx < a.K ? to_f32(static_cast<const T*>(a.W)[(i0 + r) * a.ldw + k0 + tx]) : 0.f;
-      x[r][tx] = c0 + r < a.N && k0 + tx < a.K ? to_f32(static_cast<const T*>(a.X)[(c0 + r) * a.ldx + k0 + tx]) : 0.f;
+enum { LIN_F32 = ELEM_F32, LIN_BF16 = ELEM_BF16, LIN_F16 = ELEM_F16 };
+constexpr int kEpiWarps = 16, kLoadWarp = 16, kMmaWarp = 17, kSplitWarp0 = 18, kSplitWarps = 4;
+constexpr int kSmem = 227 * 1024, kMaxStages = 8, kRound = 4;  // kRound: k-blocks per fresh accumulator (32 bits)
+static_assert(fills_sm(kSmem), "both CTAs of a pair hold all of the tensor memory");
+__host__ __device__ constexpr int lin_threads(int mode) { return mode == LIN_F32 ? 32 * (kSplitWarp0 + kSplitWarps) : 32 * kSplitWarp0; }
+__host__ __device__ constexpr int lin_max_nb(int mode) { return mode == LIN_F32 ? 128 : 256; }
+__host__ __device__ constexpr uint32_t lin_fmt(int mode) { return mode == LIN_BF16 ? 1u : mode == LIN_F16 ? 0u : 2u; }
+struct LinParams {
+  CUtensorMap w, x;  // boxes of 128 rows and of nb / CG columns
+  LinearArgs a;
+  int nb, n_ct, r_tiles, kb, stages;
+};
+struct alignas(16) LinCtrl {
+  uint64_t full[kMaxStages], split[kMaxStages], empty[kMaxStages];
+  uint64_t acc_full[2], acc_empty[2], cross_empty;
+  uint32_t tmem_base;
+  int abort;
+};
+template <int MODE> struct LinElem { using T = float; };
+template <> struct LinElem<LIN_BF16> { using T = __nv_bfloat16; };
+template <> struct LinElem<LIN_F16> { using T = __half; };
+
+template <int CG>
+__device__ __forceinline__ void lin_tma(void* dst, const CUtensorMap* map, uint32_t bar, int k, int row) {
+  if constexpr (CG == 2)
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                 :: "r"(smem_u32(dst)), "l"(map), "r"(bar), "r"(k), "r"(row) : "memory");
+  else
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                 :: "r"(smem_u32(dst)), "l"(map), "r"(bar), "r"(k), "r"(row) : "memory");
+}
+template <int CG, int TF32>
+__device__ __forceinline__ void lin_mma(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate) {
+  if constexpr (CG == 2) umma_pair<TF32>(d, da, db, idesc, accumulate);
+  else umma<TF32>(d, da, db, idesc, accumulate);
+}
+template <int CG>
+__device__ __forceinline__ void lin_commit(uint64_t* bar) {
+  if constexpr (CG == 2) umma_commit_pair(bar);
+  else umma_commit(bar);
+}
+// arrival on the leader's barrier (a CTA alone leads itself)
+template <int CG>
+__device__ __forceinline__ void lin_arrive(uint64_t* bar) {
+  if constexpr (CG == 2) mbar_arrive_leader(bar);
+  else mbar_arrive(bar);
+}
+
+template <int MODE, int CG, int ACT>
+__global__ void __launch_bounds__(lin_threads(MODE), 1) linear_tc_kernel(const __grid_constant__ LinParams p) {
+  using T = typename LinElem<MODE>::T;
+  constexpr bool F32 = MODE == LIN_F32;
+  constexpr int EPK = 128 / (int)sizeof(T), GROUPS = lin_max_nb(MODE) / 32;
+  extern __shared__ __align__(1024) uint8_t lin_smem[];
+  const int warp = uniform_warp(), lane = threadIdx.x & 31;
+  const int rank = CG == 2 ? (int)(blockIdx.x & 1) : 0, unit = blockIdx.x / CG, n_units = gridDim.x / CG;
+  const int nb = p.nb, x_rows = nb / CG, w_bytes = 128 * 128, x_bytes = x_rows * 128, raw = w_bytes + x_bytes, stage = raw * (F32 ? 2 : 1);
+  LinCtrl& ct = *reinterpret_cast<LinCtrl*>(lin_smem + (size_t)p.stages * stage);
+  const int n_tiles = p.r_tiles * p.n_ct, rounds = F32 ? (p.kb + kRound - 1) / kRound : 1;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < p.stages; ++s) {
+      mbar_init(&ct.full[s], 1);                       // the stage's bytes: 32 bits, of this CTA; else the leader's, of both
+      mbar_init(&ct.split[s], CG * kSplitWarps);       // (the leader's) the lo parts are written
+      mbar_init(&ct.empty[s], 1);
     }
-    __syncthreads();
-    for (int k = 0; k < 32; ++k)
-      for (int u = 0; u < 4; ++u) acc[u] = fmaf(w[tx][k], x[ty + 8 * u][k], acc[u]);
-    __syncthreads();
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&ct.acc_full[b], 1);
+      mbar_init(&ct.acc_empty[b], CG * kEpiWarps);
+    }
+    mbar_init(&ct.cross_empty, CG * kEpiWarps);
+    ct.abort = (smem_u32(lin_smem) & 1023) ? 1 : 0;
+    if (ct.abort && p.a.err) atomicExch(p.a.err, 8);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  const long long i = i0 + tx;
-  if (i >= a.n) return;
-  const float b = a.bias ? a.bias[i] : 0.f;
-  for (int u = 0; u < 4; ++u) {
-    const long long c = c0 + ty + 8 * u;
-    if (c >= a.N) continue;
-    float y = linear_act(acc[u] + b, a.act);
-    if (a.R) y += to_f32(static_cast<const T*>(a.R)[c * a.ldr + i]);
-    static_cast<T*>(a.Y)[c * a.ldy + i] = from_f32<T>(y);
+  if (warp == kMmaWarp) {
+    if constexpr (CG == 2) tmem_alloc_pair(&ct.tmem_base, 512);
+    else lin_tmem_alloc(&ct.tmem_base, 512);
   }
+  tc_fence_before();
+  __syncthreads();
+  if constexpr (CG == 2) cluster_sync_all();
+  tc_fence_after();
+  const uint32_t tmem_base = ct.tmem_base;
+  const bool sound = __all_sync(0xffffffffu, ct.abort == 0);
+
+  if (warp == kLoadWarp) {
+    // ------------------------------------------------------------ loads
+    const bool one = elect_one();
+    bool ok = sound;
+    int st = 0, it = 0;
+    uint32_t ph = 0;
+    for (int tile = unit; tile < n_tiles && ok; tile += n_units) {
+      const int col = tile % p.n_ct * nb + rank * x_rows, row = (tile / p.n_ct * CG + rank) * 128;
+      for (int k = 0; k < p.kb; ++k, ++it) {
+        if (it >= p.stages && !mbar_wait_warp(&ct.empty[st], ph ^ 1u, &ct.abort, p.a.err, 1)) { ok = false; break; }
+        uint8_t* dst = lin_smem + (size_t)st * stage;
+        if (one) {
+          // 32 bits: counted here, for the warps that split; else on the leader's barrier, which expects both CTAs' bytes
+          const uint32_t bar = CG == 2 && !F32 ? cluster_map(smem_u32(&ct.full[st]), 0) : smem_u32(&ct.full[st]);
+          if (F32 || rank == 0) mbar_expect_tx(&ct.full[st], (uint32_t)(F32 ? raw : CG * raw));
+          lin_tma<F32 ? 1 : CG>(dst, &p.w, bar, k * EPK, row);
+          lin_tma<F32 ? 1 : CG>(dst + w_bytes, &p.x, bar, k * EPK, col);
+        }
+        __syncwarp();
+        if (++st == p.stages) { st = 0; ph ^= 1u; }
+      }
+    }
+    if (sound && !ok) settle_copies();
+  } else if (warp == kMmaWarp) {
+    // ------------------------------------------------------------ MMAs
+    if (rank == 0 && sound) {
+      const bool one = elect_one();
+      const uint32_t idesc = CG == 2 ? make_idesc_pair(lin_fmt(MODE), (uint32_t)nb) : make_idesc(lin_fmt(MODE), (uint32_t)nb);
+      int st = 0, use = 0, ti = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      for (int tile = unit; tile < n_tiles && ok; tile += n_units, ++ti) {
+        uint32_t d = 0;
+        const uint32_t x_acc = tmem_base + 2u * nb;
+        for (int k = 0; k < p.kb; ++k) {
+          const bool fresh = F32 ? k % kRound == 0 : k == 0;
+          if (fresh) {
+            if (!mbar_wait_warp(&ct.acc_empty[use & 1], (uint32_t)(((use >> 1) & 1) ^ 1), &ct.abort, p.a.err, 4)) { ok = false; break; }
+            d = tmem_base + (uint32_t)((use & 1) * nb);
+          }
+          if (F32 && k == 0 && !mbar_wait_warp(&ct.cross_empty, (uint32_t)((ti & 1) ^ 1), &ct.abort, p.a.err, 5)) { ok = false; break; }
+          if (!(F32 && CG == 2 ? __all_sync(0xffffffffu, mbar_wait_cluster(&ct.split[st], ph, &ct.abort, p.a.err, 2))
+                               : mbar_wait_warp(F32 ? &ct.split[st] : &ct.full[st], ph, &ct.abort, p.a.err, 2))) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t w_addr = smem_u32(lin_smem + (size_t)st * stage), x_addr = w_addr + w_bytes;
+          const uint64_t dw = make_smem_desc(w_addr), dx = make_smem_desc(x_addr);
+          if (one) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) lin_mma<CG, F32>(d, dw + 2 * i, dx + 2 * i, idesc, (!fresh || i > 0) ? 1u : 0u);
+            if (F32) {
+              const uint64_t dwl = make_smem_desc(w_addr + raw), dxl = make_smem_desc(x_addr + raw);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                lin_mma<CG, F32>(x_acc, dwl + 2 * i, dx + 2 * i, idesc, (k > 0 || i > 0) ? 1u : 0u);
+                lin_mma<CG, F32>(x_acc, dw + 2 * i, dxl + 2 * i, idesc, 1u);
+              }
+            }
+            lin_commit<CG>(&ct.empty[st]);
+          }
+          __syncwarp();
+          if (++st == p.stages) { st = 0; ph ^= 1u; }
+          if (F32 ? (k % kRound == kRound - 1 || k == p.kb - 1) : k == p.kb - 1) {
+            if (one) lin_commit<CG>(&ct.acc_full[use & 1]);
+            __syncwarp();
+            ++use;
+          }
+        }
+      }
+      if (!ok) settle_copies();
+    }
+  } else if (warp < kEpiWarps) {
+    // ------------------------------------------------------------ epilogue: outputs 32 quad .. +31 of the CTA's 128, every fourth group of 8 columns
+    const int quad = warp & 3, cg = warp >> 2;
+    const LinearArgs& a = p.a;
+    int use = 0;
+    bool ready = sound;
+    for (int tile = unit; tile < n_tiles && ready; tile += n_units) {
+      const int col = tile % p.n_ct * nb, cols = min(nb, a.N - col), i = (tile / p.n_ct * CG + rank) * 128 + quad * 32 + lane;
+      const bool in = i < a.n;
+      const float bias = in && a.bias ? __ldg(a.bias + i) : 0.f;
+      float z[GROUPS][8];
+      const uint32_t lanes = tmem_base + ((uint32_t)(quad * 32) << 16) + 8u * cg;
+      for (int r = 0; r < rounds && ready; ++r, ++use) {
+        ready = __all_sync(0xffffffffu, mbar_wait(&ct.acc_full[use & 1], (uint32_t)((use >> 1) & 1), &ct.abort, a.err, 3));
+        if (!ready) break;
+        tc_fence_after();
+        const uint32_t at = lanes + (uint32_t)((use & 1) * nb);
+        if (r == 0) {
+#pragma unroll
+          for (int j = 0; j < GROUPS; ++j)
+            if (32 * j + 8 * cg < nb) tmem_ld8(at + 32 * j, z[j]);
+          tmem_wait_ld();
+        } else {
+#pragma unroll
+          for (int j = 0; j < GROUPS; j += 2) {
+            float y[2][8];
+            if (32 * j + 8 * cg < nb) tmem_ld8(at + 32 * j, y[0]);
+            if (j + 1 < GROUPS && 32 * (j + 1) + 8 * cg < nb) tmem_ld8(at + 32 * (j + 1), y[1]);
+            tmem_wait_ld();
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+              if (32 * j + 8 * cg < nb) z[j][u] += y[0][u];
+              if (j + 1 < GROUPS && 32 * (j + 1) + 8 * cg < nb) z[j + 1][u] += y[1][u];
+            }
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) lin_arrive<CG>(&ct.acc_empty[use & 1]);
+      }
+      if (!ready) break;
+      if (F32) {  // the last round's commit covers the cross products
+#pragma unroll
+        for (int j = 0; j < GROUPS; ++j) {
+          if (32 * j + 8 * cg < nb) {
+            float y[8];
+            tmem_ld8(lanes + 2u * nb + 32 * j, y);
+            tmem_wait_ld();
+#pragma unroll
+            for (int u = 0; u < 8; ++u) z[j][u] += y[u];
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) lin_arrive<CG>(&ct.cross_empty);
+      }
+      if (in) {
+#pragma unroll
+        for (int j = 0; j < GROUPS; ++j) {
+          const int c0 = 32 * j + 8 * cg;
+          if (c0 >= cols) break;
+          const long long c = col + c0;
+          T* y = static_cast<T*>(a.Y) + c * a.ldy + i;
+          const T* res = static_cast<const T*>(a.R) + c * a.ldr + i;
+          float rv[8];
+          if (a.R) {
+#pragma unroll
+            for (int u = 0; u < 8; ++u) rv[u] = c0 + u < cols ? to_f32(res[u * a.ldr]) : 0.f;
+          }
+#pragma unroll
+          for (int u = 0; u < 8; ++u) {
+            float v = linear_act(z[j][u] + bias, ACT);
+            if (a.R) v += rv[u];
+            if (c0 + u < cols) y[u * a.ldy] = from_f32<T>(v);
+          }
+        }
+      }
+      __syncwarp();
+    }
+  } else if (F32) {
+    // ------------------------------------------------------------ the lo parts of a stage: what tf32 cuts off of the tile beside it
+    int st = 0;
+    uint32_t ph = 0;
+    bool ok = sound;
+    const int me = (warp - kSplitWarp0) * 32 + lane;
+    for (int tile = unit; tile < n_tiles && ok; tile += n_units)
+      for (int k = 0; k < p.kb; ++k) {
+        if (!mbar_wait_warp(&ct.full[st], ph, &ct.abort, p.a.err, 6)) { ok = false; break; }
+        const uint4* src = reinterpret_cast<const uint4*>(lin_smem + (size_t)st * stage);
+        uint4* dst = reinterpret_cast<uint4*>(lin_smem + (size_t)st * stage + raw);
+#pragma unroll 4
+        for (int e = me; e < raw / 16; e += kSplitWarps * 32) {
+          const uint4 x = src[e];
+          dst[e] = make_uint4(tf32_rest(x.x), tf32_rest(x.y), tf32_rest(x.z), tf32_rest(x.w));
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) {
+          if constexpr (CG == 2) mbar_arrive_remote(&ct.split[st], 0);
+          else mbar_arrive(&ct.split[st]);
+        }
+        if (++st == p.stages) { st = 0; ph ^= 1u; }
+      }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if constexpr (CG == 2) cluster_sync_all();  // neither CTA ends while the other one's MMAs read its tiles or its arrivals come in
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    if constexpr (CG == 2) tmem_free_pair(tmem_base, 512);
+    else lin_tmem_free(tmem_base, 512);
+  }
+}
+
+// Rows that no 16-byte copy can start at, moved to where one can: one element per thread and step
+template <class T>
+__global__ void __launch_bounds__(256) linear_align_kernel(const T* src, long long ld, int rows, int K, T* dst, long long ld_dst) {
+  for (long long r = blockIdx.y; r < rows; r += gridDim.y)
+    for (int k = blockIdx.x * 256 + threadIdx.x; k < K; k += gridDim.x * 256) dst[r * ld_dst + k] = src[r * ld + k];
+}
+
+struct LinPlan {
+  bool few;
+  int cg, nb, n_ct;
+  bool align_w, align_x;
+  long long ld_pad;         // elements of a row that was moved
+  size_t w_bytes, x_bytes;  // of the workspace
+};
+LinPlan lin_plan(const LinearArgs& a, int elem) {
+  LinPlan pl;
+  std::memset(&pl, 0, sizeof(pl));
+  const int eb = elem_bytes(elem), sms = device_sms(), kb = (a.K * eb + 127) / 128;
+  const long long rows1 = (a.n + 127) / 128, rows2 = (a.n + 255) / 256;
+  pl.few = a.N <= 32 || a.n <= 16;
+  if (pl.few) return pl;
+  // the time of a launch: tiles of the busiest unit x (columns of a tile, at least what the issue of an MMA takes)
+  double best = 0;
+  for (int cg = 1; cg <= 2; ++cg)
+    for (int w = lin_max_nb(elem); w >= 32; w -= 32) {
+      const int n_ct = (a.N - 1) / w + 1, nb = ((a.N - 1) / n_ct + 32) / 32 * 32;
+      if ((long long)nb * (n_ct - 1) >= a.N) continue;
+      const long long tiles = (cg == 2 ? rows2 : rows1) * n_ct, waves = (tiles + sms / cg - 1) / (sms / cg);
+      const double cost = waves * (kb * (elem == ELEM_F32 ? 3.0 : 1.0) * std::max(nb * (cg == 2 ? 1.0 : 1.25), 48.0) + 600.0);
+      if (pl.nb == 0 || cost < best) {
+        best = cost;
+        pl.cg = cg; pl.nb = nb; pl.n_ct = n_ct;
+      }
+    }
+  const auto off16 = [&](const void* p, long long ld) { return ((uintptr_t)p & 15) != 0 || (ld * eb) % 16 != 0; };
+  pl.align_w = off16(a.W, a.ldw);
+  pl.align_x = off16(a.X, a.ldx);
+  pl.ld_pad = (a.K * eb + 15) / 16 * 16 / eb;
+  const auto whole = [](size_t b) { return (b + 255) / 256 * 256; };
+  pl.w_bytes = pl.align_w ? whole((size_t)a.n * pl.ld_pad * eb) : 0;
+  pl.x_bytes = pl.align_x ? whole((size_t)a.N * pl.ld_pad * eb) : 0;
+  return pl;
+}
+
+template <int MODE, int CG, int ACT>
+cudaError_t lin_launch(LinParams& p, cudaStream_t st) {
+  const int raw = (128 + p.nb / CG) * 128, stage = raw * (MODE == LIN_F32 ? 2 : 1);
+  p.stages = std::min((kSmem - (int)sizeof(LinCtrl)) / stage, (int)kMaxStages);
+  static bool configured[64] = {false};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
+  if (!configured[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(linear_tc_kernel<MODE, CG, ACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    if (e != cudaSuccess) return e;
+    configured[dev] = true;
+  }
+  cudaLaunchConfig_t cfg;
+  std::memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3((unsigned)(CG * std::min<long long>((long long)p.r_tiles * p.n_ct, device_sms() / CG)));
+  cfg.blockDim = dim3(lin_threads(MODE));
+  cfg.dynamicSmemBytes = kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = CG;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = CG == 2 ? 1 : 0;
+  count_launch();
+  return cudaLaunchKernelEx(&cfg, linear_tc_kernel<MODE, CG, ACT>, p);
+}
+template <int MODE, int CG>
+cudaError_t lin_act(LinParams& p, cudaStream_t st) {
+  switch (p.a.act) {
+    case ACT_TANH: return lin_launch<MODE, CG, ACT_TANH>(p, st);
+    case ACT_SIGMOID: return lin_launch<MODE, CG, ACT_SIGMOID>(p, st);
+    case ACT_RELU: return lin_launch<MODE, CG, ACT_RELU>(p, st);
+    case ACT_GELU: return lin_launch<MODE, CG, ACT_GELU>(p, st);
+    case ACT_SILU: return lin_launch<MODE, CG, ACT_SILU>(p, st);
+  }
+  return lin_launch<MODE, CG, ACT_NONE>(p, st);
+}
+template <int MODE>
+cudaError_t lin_type(const LinearArgs& all, const LinPlan& pl, cudaStream_t st) {
+  using T = typename LinElem<MODE>::T;
+  LinParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.a = all;
+  char* work = static_cast<char*>(all.work);
+  const auto move = [&](const void* src, long long ld, int rows, char* dst) {
+    count_launch();
+    linear_align_kernel<T><<<dim3((unsigned)((all.K + 255) / 256), (unsigned)std::min(rows, 8192)), 256, 0, st>>>(static_cast<const T*>(src), ld, rows, all.K,
+                                                                                                               reinterpret_cast<T*>(dst), pl.ld_pad);
+    return cudaGetLastError();
+  };
+  if (pl.align_w) {
+    const cudaError_t e = move(all.W, all.ldw, all.n, work);
+    if (e != cudaSuccess) return e;
+    p.a.W = work;
+    p.a.ldw = pl.ld_pad;
+  }
+  if (pl.align_x) {
+    const cudaError_t e = move(all.X, all.ldx, all.N, work + pl.w_bytes);
+    if (e != cudaSuccess) return e;
+    p.a.X = work + pl.w_bytes;
+    p.a.ldx = pl.ld_pad;
+  }
+  p.nb = pl.nb;
+  p.n_ct = pl.n_ct;
+  p.r_tiles = (all.n + 128 * pl.cg - 1) / (128 * pl.cg);
+  p.kb = (int)((all.K * (long long)sizeof(T) + 127) / 128);
+  if (!make_kmajor_map(&p.w, p.a.W, sizeof(T), all.K, all.n, p.a.ldw, 128) || !make_kmajor_map(&p.x, p.a.X, sizeof(T), all.K, all.N, p.a.ldx, pl.nb / pl.cg))
+    return cudaErrorInvalidValue;
+  return pl.cg == 2 ? lin_act<MODE, 2>(p, st) : lin_act<MODE, 1>(p, st);
 }
 
 }  // namespace
 
-size_t linear_work(const LinearArgs&, int) { return 0; }
+size_t linear_work(const LinearArgs& a, int elem) {
+  const LinPlan pl = lin_plan(a, elem);
+  return pl.w_bytes + pl.x_bytes;
+}
 cudaError_t launch_linear(const LinearArgs& a, int elem, cudaStream_t st) {
   if (a.n == 0 || a.N == 0) return cudaSuccess;
-  const dim3 grid((a.n + 31) / 32, (a.N + 31) / 32);
-  count_launch();
+  const LinPlan pl = lin_plan(a, elem);
+  if (pl.few) return launch_linear_few(a, elem, st);
   switch (elem) {
-    case ELEM_F32: linear_simple_kernel<float><<<grid, 256, 0, st>>>(a); break;
-    case ELEM_BF16: linear_simple_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(a); break;
-    default: linear_simple_kernel<__half><<<grid, 256, 0, st>>>(a);
+    case ELEM_F32: return lin_type<LIN_F32>(a, pl, st);
+    case ELEM_BF16: return lin_type<LIN_BF16>(a, pl, st);
   }
-  return cudaGetLastError();
+  return lin_type<LIN_F16>(a, pl, st);
 }
 
 }  // namespace zrnn

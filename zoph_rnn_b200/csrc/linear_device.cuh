@@ -18,5 +18,27 @@ __device__ __forceinline__ float linear_act(float x, int act) {
   return x;
 }
 
+// x in 32 bits as two tf32 operands, of which the tensor cores take the upper 19 bits: hi is x cut off there, lo what that leaves, rounded to
+// nearest (cut off, too, it would shrink every product a little: 2^-22 in the same direction).  Together 11 + 11 bits.  Of an
+// infinity or a NaN lo is NaN.
+__device__ __forceinline__ uint32_t tf32_rest(uint32_t x) {
+  const float lo = __uint_as_float(x) - __uint_as_float(x & 0xffffe000u);
+  const uint32_t b = __float_as_uint(lo);
+  return lo == lo ? b + 0x1000u : b;
+}
+__device__ __forceinline__ void split_tf32(uint32_t x, uint32_t& hi, uint32_t& lo) {
+  hi = x;
+  lo = tf32_rest(x);
+}
+
+// tensor memory for a CTA without a partner, by one warp
+__device__ __forceinline__ void lin_tmem_alloc(uint32_t* base, uint32_t cols) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"((uint32_t)__cvta_generic_to_shared(base)), "r"(cols) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void lin_tmem_free(uint32_t base, uint32_t cols) {
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(cols) : "memory");
+}
+
 }  // namespace
 }  // namespace zrnn
