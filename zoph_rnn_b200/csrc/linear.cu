@@ -5,10 +5,12 @@
 // (tc_pair_device.cuh).  One warp brings the k-blocks of 128 bytes by TMA, one issues the MMAs, sixteen take the accumulators
 // through bias, activation and residual while the next tile's MMAs run; persistent.
 //
-// 32-bit operands go as two tf32 parts each and three products (hi hi; lo hi and hi lo into an accumulator of their own).  The tensor cores
+// 32-bit operands go as two tf32 parts each and three products (hi hi; hi lo and lo hi into an accumulator of their own).  The tensor cores
 // ignore the bits below tf32, so the tile that TMA brought is the hi part as it is; four warps write the lo part of each stage beside
-// it, element by element, whatever the swizzle.  A tensor-core accumulator cuts its sums off, so the hi products of four k-blocks
-// (16 additions) go into a fresh one, two in turn, and the sixteen warps add those up in ordinary 32-bit arithmetic.
+// it, element by element, whatever the swizzle.  hi and lo of the columns lie one behind the other, so that W's hi part is read once for both.
+// A tensor-core accumulator cuts its sums off, so the products of four k-blocks (16 additions) go into a fresh pair, two
+// pairs in turn, and the sixteen warps add those up in ordinary 32-bit arithmetic.  What bounds it is shared memory: per k-block of
+// 256 x 128, a CTA's TMA writes, the splitting's reads and writes and the MMAs' reads are 131 KB, 1024 cycles for MMAs of 768.
 //
 // A CTA asks for all of an SM's shared memory, so that a pair's allocation of tensor memory waits for nobody that could wait for it in turn.
 #include <algorithm>
@@ -24,10 +26,10 @@ namespace zrnn {
 namespace {
 
 enum { LIN_F32 = ELEM_F32, LIN_BF16 = ELEM_BF16, LIN_F16 = ELEM_F16 };
-constexpr int kEpiWarps = 16, kLoadWarp = 16, kMmaWarp = 17, kSplitWarp0 = 18, kSplitWarps = 4;
+constexpr int kEpiWarps = 16, kLoadWarp = 16, kMmaWarp = 17, kSplitWarp0 = 18, kSplitWarps = 4, kSplitTeams = 2;
 constexpr int kSmem = 227 * 1024, kMaxStages = 8, kRound = 4;  // kRound: k-blocks per fresh accumulator (32 bits)
 static_assert(fills_sm(kSmem), "both CTAs of a pair hold all of the tensor memory");
-__host__ __device__ constexpr int lin_threads(int mode) { return mode == LIN_F32 ? 32 * (kSplitWarp0 + kSplitWarps) : 32 * kSplitWarp0; }
+__host__ __device__ constexpr int lin_threads(int mode) { return mode == LIN_F32 ? 32 * (kSplitWarp0 + kSplitTeams * kSplitWarps) : 32 * kSplitWarp0; }
 __host__ __device__ constexpr int lin_max_nb(int mode) { return mode == LIN_F32 ? 128 : 256; }
 __host__ __device__ constexpr uint32_t lin_fmt(int mode) { return mode == LIN_BF16 ? 1u : mode == LIN_F16 ? 0u : 2u; }
 struct LinParams {
@@ -37,7 +39,7 @@ struct LinParams {
 };
 struct alignas(16) LinCtrl {
   uint64_t full[kMaxStages], split[kMaxStages], empty[kMaxStages];
-  uint64_t acc_full[2], acc_empty[2], cross_empty;
+  uint64_t acc_full[2], acc_empty[2];
   uint32_t tmem_base;
   int abort;
 };
@@ -80,6 +82,8 @@ __global__ void __launch_bounds__(lin_threads(MODE), 1) linear_tc_kernel(const _
   const int warp = uniform_warp(), lane = threadIdx.x & 31;
   const int rank = CG == 2 ? (int)(blockIdx.x & 1) : 0, unit = blockIdx.x / CG, n_units = gridDim.x / CG;
   const int nb = p.nb, x_rows = nb / CG, w_bytes = 128 * 128, x_bytes = x_rows * 128, raw = w_bytes + x_bytes, stage = raw * (F32 ? 2 : 1);
+  // a stage: W, X; in 32 bits also X lo and W lo, in that order: X and its rest are one operand of twice the columns
+  const int w_off = w_bytes + 2 * x_bytes, acc = nb * (F32 ? 2 : 1);
   LinCtrl& ct = *reinterpret_cast<LinCtrl*>(lin_smem + (size_t)p.stages * stage);
   const int n_tiles = p.r_tiles * p.n_ct, rounds = F32 ? (p.kb + kRound - 1) / kRound : 1;
   if (threadIdx.x == 0) {
@@ -92,7 +96,6 @@ __global__ void __launch_bounds__(lin_threads(MODE), 1) linear_tc_kernel(const _
       mbar_init(&ct.acc_full[b], 1);
       mbar_init(&ct.acc_empty[b], CG * kEpiWarps);
     }
-    mbar_init(&ct.cross_empty, CG * kEpiWarps);
     ct.abort = (smem_u32(lin_smem) & 1023) ? 1 : 0;
     if (ct.abort && p.a.err) atomicExch(p.a.err, 8);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -136,34 +139,34 @@ __global__ void __launch_bounds__(lin_threads(MODE), 1) linear_tc_kernel(const _
     if (rank == 0 && sound) {
       const bool one = elect_one();
       const uint32_t idesc = CG == 2 ? make_idesc_pair(lin_fmt(MODE), (uint32_t)nb) : make_idesc(lin_fmt(MODE), (uint32_t)nb);
-      int st = 0, use = 0, ti = 0;
+      const uint32_t idesc2 = CG == 2 ? 0u : make_idesc(lin_fmt(MODE), 2u * nb);
+      int st = 0, use = 0;
       uint32_t ph = 0;
       bool ok = true;
-      for (int tile = unit; tile < n_tiles && ok; tile += n_units, ++ti) {
+      for (int tile = unit; tile < n_tiles && ok; tile += n_units) {
         uint32_t d = 0;
-        const uint32_t x_acc = tmem_base + 2u * nb;
         for (int k = 0; k < p.kb; ++k) {
           const bool fresh = F32 ? k % kRound == 0 : k == 0;
           if (fresh) {
             if (!mbar_wait_warp(&ct.acc_empty[use & 1], (uint32_t)(((use >> 1) & 1) ^ 1), &ct.abort, p.a.err, 4)) { ok = false; break; }
-            d = tmem_base + (uint32_t)((use & 1) * nb);
+            d = tmem_base + (uint32_t)((use & 1) * acc);
           }
-          if (F32 && k == 0 && !mbar_wait_warp(&ct.cross_empty, (uint32_t)((ti & 1) ^ 1), &ct.abort, p.a.err, 5)) { ok = false; break; }
           if (!(F32 && CG == 2 ? __all_sync(0xffffffffu, mbar_wait_cluster(&ct.split[st], ph, &ct.abort, p.a.err, 2))
                                : mbar_wait_warp(F32 ? &ct.split[st] : &ct.full[st], ph, &ct.abort, p.a.err, 2))) { ok = false; break; }
           tc_fence_after();
           const uint32_t w_addr = smem_u32(lin_smem + (size_t)st * stage), x_addr = w_addr + w_bytes;
-          const uint64_t dw = make_smem_desc(w_addr), dx = make_smem_desc(x_addr);
+          const uint64_t dw = make_smem_desc(w_addr), dx = make_smem_desc(x_addr), dwl = make_smem_desc(w_addr + w_off), dxl = make_smem_desc(x_addr + x_bytes);
           if (one) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) lin_mma<CG, F32>(d, dw + 2 * i, dx + 2 * i, idesc, (!fresh || i > 0) ? 1u : 0u);
-            if (F32) {
-              const uint64_t dwl = make_smem_desc(w_addr + raw), dxl = make_smem_desc(x_addr + raw);
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                lin_mma<CG, F32>(x_acc, dwl + 2 * i, dx + 2 * i, idesc, (k > 0 || i > 0) ? 1u : 0u);
-                lin_mma<CG, F32>(x_acc, dw + 2 * i, dxl + 2 * i, idesc, 1u);
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t more = !fresh || i > 0 ? 1u : 0u;
+              if (F32 && CG == 1) {  // hi times [hi lo] of the columns, twice as wide
+                lin_mma<CG, F32>(d, dw + 2 * i, dx + 2 * i, idesc2, more);
+              } else {               // (of a pair, each CTA has half of the columns' operand: it would be hi lo hi lo)
+                lin_mma<CG, F32>(d, dw + 2 * i, dx + 2 * i, idesc, more);
+                if (F32) lin_mma<CG, F32>(d + nb, dw + 2 * i, dxl + 2 * i, idesc, more);
               }
+              if (F32) lin_mma<CG, F32>(d + nb, dwl + 2 * i, dx + 2 * i, idesc, 1u);
             }
             lin_commit<CG>(&ct.empty[st]);
           }
@@ -194,23 +197,22 @@ __global__ void __launch_bounds__(lin_threads(MODE), 1) linear_tc_kernel(const _
         ready = __all_sync(0xffffffffu, mbar_wait(&ct.acc_full[use & 1], (uint32_t)((use >> 1) & 1), &ct.abort, a.err, 3));
         if (!ready) break;
         tc_fence_after();
-        const uint32_t at = lanes + (uint32_t)((use & 1) * nb);
-        if (r == 0) {
+        const uint32_t at = lanes + (uint32_t)((use & 1) * acc);
+        if (!F32) {
 #pragma unroll
           for (int j = 0; j < GROUPS; ++j)
             if (32 * j + 8 * cg < nb) tmem_ld8(at + 32 * j, z[j]);
           tmem_wait_ld();
-        } else {
+        } else {  // this round's sums and, beside them, the cross products
 #pragma unroll
-          for (int j = 0; j < GROUPS; j += 2) {
-            float y[2][8];
-            if (32 * j + 8 * cg < nb) tmem_ld8(at + 32 * j, y[0]);
-            if (j + 1 < GROUPS && 32 * (j + 1) + 8 * cg < nb) tmem_ld8(at + 32 * (j + 1), y[1]);
-            tmem_wait_ld();
+          for (int j = 0; j < GROUPS; ++j) {
+            if (32 * j + 8 * cg < nb) {
+              float y[2][8];
+              tmem_ld8(at + 32 * j, y[0]);
+              tmem_ld8(at + nb + 32 * j, y[1]);
+              tmem_wait_ld();
 #pragma unroll
-            for (int u = 0; u < 8; ++u) {
-              if (32 * j + 8 * cg < nb) z[j][u] += y[0][u];
-              if (j + 1 < GROUPS && 32 * (j + 1) + 8 * cg < nb) z[j + 1][u] += y[1][u];
+              for (int u = 0; u < 8; ++u) z[j][u] = r == 0 ? y[0][u] + y[1][u] : z[j][u] + (y[0][u] + y[1][u]);
             }
           }
         }
@@ -219,21 +221,6 @@ __global__ void __launch_bounds__(lin_threads(MODE), 1) linear_tc_kernel(const _
         if (lane == 0) lin_arrive<CG>(&ct.acc_empty[use & 1]);
       }
       if (!ready) break;
-      if (F32) {  // the last round's commit covers the cross products
-#pragma unroll
-        for (int j = 0; j < GROUPS; ++j) {
-          if (32 * j + 8 * cg < nb) {
-            float y[8];
-            tmem_ld8(lanes + 2u * nb + 32 * j, y);
-            tmem_wait_ld();
-#pragma unroll
-            for (int u = 0; u < 8; ++u) z[j][u] += y[u];
-          }
-        }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) lin_arrive<CG>(&ct.cross_empty);
-      }
       if (in) {
 #pragma unroll
         for (int j = 0; j < GROUPS; ++j) {
@@ -259,28 +246,35 @@ __global__ void __launch_bounds__(lin_threads(MODE), 1) linear_tc_kernel(const _
     }
   } else if (F32) {
     // ------------------------------------------------------------ the lo parts of a stage: what tf32 cuts off of the tile beside it
-    int st = 0;
-    uint32_t ph = 0;
-    bool ok = sound;
-    const int me = (warp - kSplitWarp0) * 32 + lane;
-    for (int tile = unit; tile < n_tiles && ok; tile += n_units)
-      for (int k = 0; k < p.kb; ++k) {
-        if (!mbar_wait_warp(&ct.full[st], ph, &ct.abort, p.a.err, 6)) { ok = false; break; }
-        const uint4* src = reinterpret_cast<const uint4*>(lin_smem + (size_t)st * stage);
-        uint4* dst = reinterpret_cast<uint4*>(lin_smem + (size_t)st * stage + raw);
+    // Two teams of four warps take every other k-block each: one's waits are filled by the other.
+    const int team = (warp - kSplitWarp0) / kSplitWarps, me = (warp - kSplitWarp0) % kSplitWarps * 32 + lane;
+    const int wv = w_bytes / 16, xv = x_bytes / 16;
+    long long its = 0;
+    for (int tile = unit; tile < n_tiles; tile += n_units) its += p.kb;
+    int st = team % p.stages;
+    uint32_t ph = (uint32_t)(team / p.stages) & 1u;
+    for (long long it = team; it < its && sound; it += kSplitTeams) {
+      if (!mbar_wait_warp(&ct.full[st], ph, &ct.abort, p.a.err, 6)) break;
+      uint4* tiles = reinterpret_cast<uint4*>(lin_smem + (size_t)st * stage);
 #pragma unroll 4
-        for (int e = me; e < raw / 16; e += kSplitWarps * 32) {
-          const uint4 x = src[e];
-          dst[e] = make_uint4(tf32_rest(x.x), tf32_rest(x.y), tf32_rest(x.z), tf32_rest(x.w));
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) {
-          if constexpr (CG == 2) mbar_arrive_remote(&ct.split[st], 0);
-          else mbar_arrive(&ct.split[st]);
-        }
-        if (++st == p.stages) { st = 0; ph ^= 1u; }
+      for (int e = me; e < wv; e += kSplitWarps * 32) {
+        const uint4 x = tiles[e];
+        tiles[w_off / 16 + e] = make_uint4(tf32_rest(x.x), tf32_rest(x.y), tf32_rest(x.z), tf32_rest(x.w));
       }
+#pragma unroll 2
+      for (int e = wv + me; e < wv + xv; e += kSplitWarps * 32) {
+        const uint4 x = tiles[e];
+        tiles[xv + e] = make_uint4(tf32_rest(x.x), tf32_rest(x.y), tf32_rest(x.z), tf32_rest(x.w));
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (CG == 2) mbar_arrive_remote(&ct.split[st], 0);
+        else mbar_arrive(&ct.split[st]);
+      }
+      st += kSplitTeams;
+      if (st >= p.stages) { st -= p.stages; ph ^= 1u; }
+    }
   }
   __syncwarp();
   tc_fence_before();

@@ -18,14 +18,10 @@ __device__ __forceinline__ float linear_act(float x, int act) {
   return x;
 }
 
-// x in 32 bits as two tf32 operands, of which the tensor cores take the upper 19 bits: hi is x cut off there, lo what that leaves, rounded to
-// nearest (cut off, too, it would shrink every product a little: 2^-22 in the same direction).  Together 11 + 11 bits.  Of an
-// infinity or a NaN lo is NaN.
-__device__ __forceinline__ uint32_t tf32_rest(uint32_t x) {
-  const float lo = __uint_as_float(x) - __uint_as_float(x & 0xffffe000u);
-  const uint32_t b = __float_as_uint(lo);
-  return lo == lo ? b + 0x1000u : b;
-}
+// x in 32 bits as two tf32 operands, of which the tensor cores take the upper 19 bits: hi is x as it is, cut off there; lo what that leaves,
+// 13 bits of which 11 count.  What lo loses makes an operand smaller by some 1e-7 of itself; rounding it instead would take three more
+// instructions per element, and the splitting of a stage takes as long as its products.  Of an infinity lo is NaN.
+__device__ __forceinline__ uint32_t tf32_rest(uint32_t x) { return __float_as_uint(__uint_as_float(x) - __uint_as_float(x & 0xffffe000u)); }
 __device__ __forceinline__ void split_tf32(uint32_t x, uint32_t& hi, uint32_t& lo) {
   hi = x;
   lo = tf32_rest(x);
