@@ -26,16 +26,17 @@ namespace zrnn {
 namespace {
 
 enum { LIN_F32 = ELEM_F32, LIN_BF16 = ELEM_BF16, LIN_F16 = ELEM_F16 };
-constexpr int kEpiWarps = 16, kLoadWarp = 16, kMmaWarp = 17, kSplitWarp0 = 18, kSplitWarps = 4, kSplitTeams = 2;
+constexpr int kEpiWarps = 16, kLoadWarp = 16, kMmaWarp = 17, kSplitWarp0 = 18, kSplitWarps = 4, kSplitTeams = 3;
 constexpr int kSmem = 227 * 1024, kMaxStages = 8, kRound = 4;  // kRound: k-blocks per fresh accumulator (32 bits)
 static_assert(fills_sm(kSmem), "both CTAs of a pair hold all of the tensor memory");
 __host__ __device__ constexpr int lin_threads(int mode) { return mode == LIN_F32 ? 32 * (kSplitWarp0 + kSplitTeams * kSplitWarps) : 32 * kSplitWarp0; }
-__host__ __device__ constexpr int lin_max_nb(int mode) { return mode == LIN_F32 ? 128 : 256; }
+__host__ __device__ constexpr int lin_max_nb(int mode, bool cut) { return mode == LIN_F32 || cut ? 128 : 256; }
 __host__ __device__ constexpr uint32_t lin_fmt(int mode) { return mode == LIN_BF16 ? 1u : mode == LIN_F16 ? 0u : 2u; }
 struct LinParams {
   CUtensorMap w, x;  // boxes of 128 rows and of nb / CG columns
   LinearArgs a;
   int nb, n_ct, r_tiles, kb, stages;
+  int cut;  // CTAs of a cluster that share a tile's K axis (1: none; not with pairs)
 };
 struct alignas(16) LinCtrl {
   uint64_t full[kMaxStages], split[kMaxStages], empty[kMaxStages];
@@ -73,19 +74,22 @@ __device__ __forceinline__ void lin_arrive(uint64_t* bar) {
   else mbar_arrive(bar);
 }
 
-template <int MODE, int CG, int ACT>
+template <int MODE, int CG, int ACT, bool CUT>
 __global__ void __launch_bounds__(lin_threads(MODE), 1) linear_tc_kernel(const __grid_constant__ LinParams p) {
   using T = typename LinElem<MODE>::T;
   constexpr bool F32 = MODE == LIN_F32;
-  constexpr int EPK = 128 / (int)sizeof(T), GROUPS = lin_max_nb(MODE) / 32;
+  constexpr int EPK = 128 / (int)sizeof(T), GROUPS = lin_max_nb(MODE, CUT) / 32;
+  static_assert(!CUT || CG == 1, "a pair's tiles are not cut");
   extern __shared__ __align__(1024) uint8_t lin_smem[];
   const int warp = uniform_warp(), lane = threadIdx.x & 31;
-  const int rank = CG == 2 ? (int)(blockIdx.x & 1) : 0, unit = blockIdx.x / CG, n_units = gridDim.x / CG;
+  const int rank = CG == 2 ? (int)(blockIdx.x & 1) : 0, cut = CUT ? p.cut : 1, unit = blockIdx.x / (CG * cut), n_units = gridDim.x / (CG * cut);
+  const int part = CUT ? (int)blockIdx.x % cut : 0;
+  const int kb0 = CUT ? (int)((long long)p.kb * part / cut) : 0, kb = CUT ? (int)((long long)p.kb * (part + 1) / cut) - kb0 : p.kb;  // this CTA's k-blocks
   const int nb = p.nb, x_rows = nb / CG, w_bytes = 128 * 128, x_bytes = x_rows * 128, raw = w_bytes + x_bytes, stage = raw * (F32 ? 2 : 1);
   // a stage: W, X; in 32 bits also X lo and W lo, in that order: X and its rest are one operand of twice the columns
   const int w_off = w_bytes + 2 * x_bytes, acc = nb * (F32 ? 2 : 1);
   LinCtrl& ct = *reinterpret_cast<LinCtrl*>(lin_smem + (size_t)p.stages * stage);
-  const int n_tiles = p.r_tiles * p.n_ct, rounds = F32 ? (p.kb + kRound - 1) / kRound : 1;
+  const int n_tiles = p.r_tiles * p.n_ct, rounds = F32 ? (kb + kRound - 1) / kRound : 1;
   if (threadIdx.x == 0) {
     for (int s = 0; s < p.stages; ++s) {
       mbar_init(&ct.full[s], 1);                       // the stage's bytes: 32 bits, of this CTA; else the leader's, of both
@@ -106,7 +110,7 @@ __global__ void __launch_bounds__(lin_threads(MODE), 1) linear_tc_kernel(const _
   }
   tc_fence_before();
   __syncthreads();
-  if constexpr (CG == 2) cluster_sync_all();
+  if (CG == 2 || CUT) cluster_sync_all();
   tc_fence_after();
   const uint32_t tmem_base = ct.tmem_base;
   const bool sound = __all_sync(0xffffffffu, ct.abort == 0);
@@ -119,7 +123,7 @@ __global__ void __launch_bounds__(lin_threads(MODE), 1) linear_tc_kernel(const _
     uint32_t ph = 0;
     for (int tile = unit; tile < n_tiles && ok; tile += n_units) {
       const int col = tile % p.n_ct * nb + rank * x_rows, row = (tile / p.n_ct * CG + rank) * 128;
-      for (int k = 0; k < p.kb; ++k, ++it) {
+      for (int k = kb0; k < kb0 + kb; ++k, ++it) {
         if (it >= p.stages && !mbar_wait_warp(&ct.empty[st], ph ^ 1u, &ct.abort, p.a.err, 1)) { ok = false; break; }
         uint8_t* dst = lin_smem + (size_t)st * stage;
         if (one) {
@@ -145,7 +149,7 @@ __global__ void __launch_bounds__(lin_threads(MODE), 1) linear_tc_kernel(const _
       bool ok = true;
       for (int tile = unit; tile < n_tiles && ok; tile += n_units) {
         uint32_t d = 0;
-        for (int k = 0; k < p.kb; ++k) {
+        for (int k = 0; k < kb; ++k) {
           const bool fresh = F32 ? k % kRound == 0 : k == 0;
           if (fresh) {
             if (!mbar_wait_warp(&ct.acc_empty[use & 1], (uint32_t)(((use >> 1) & 1) ^ 1), &ct.abort, p.a.err, 4)) { ok = false; break; }
@@ -172,7 +176,7 @@ __global__ void __launch_bounds__(lin_threads(MODE), 1) linear_tc_kernel(const _
           }
           __syncwarp();
           if (++st == p.stages) { st = 0; ph ^= 1u; }
-          if (F32 ? (k % kRound == kRound - 1 || k == p.kb - 1) : k == p.kb - 1) {
+          if (F32 ? (k % kRound == kRound - 1 || k == kb - 1) : k == kb - 1) {
             if (one) lin_commit<CG>(&ct.acc_full[use & 1]);
             __syncwarp();
             ++use;
@@ -187,7 +191,7 @@ __global__ void __launch_bounds__(lin_threads(MODE), 1) linear_tc_kernel(const _
     const LinearArgs& a = p.a;
     int use = 0;
     bool ready = sound;
-    for (int tile = unit; tile < n_tiles && ready; tile += n_units) {
+    for (int tile = unit; tile < n_tiles && (ready || CUT); tile += n_units) {
       const int col = tile % p.n_ct * nb, cols = min(nb, a.N - col), i = (tile / p.n_ct * CG + rank) * 128 + quad * 32 + lane;
       const bool in = i < a.n;
       const float bias = in && a.bias ? __ldg(a.bias + i) : 0.f;
@@ -220,12 +224,44 @@ __global__ void __launch_bounds__(lin_threads(MODE), 1) linear_tc_kernel(const _
         __syncwarp();
         if (lane == 0) lin_arrive<CG>(&ct.acc_empty[use & 1]);
       }
+      if (CUT) {
+        // The CTAs of the cluster each finish every cut-th group of 8 columns: the other ones' sums of it go into that CTA's shared memory, where
+        // the operands were (one tile per cluster), and are added to its own in the order of the CTAs.
+        cluster_sync_all();  // all MMAs of all of them are over
+        const int per = (nb / 8 + cut - 1) / cut;
+        auto slot = [&](int from, int group) { return (uint32_t)((((from * 4 + quad) * per + group / cut) * 256 + lane) * 4); };
+        if (ready) {
+#pragma unroll
+          for (int j = 0; j < GROUPS; ++j) {
+            const int group = 4 * j + cg, to = group % cut;
+            if (8 * group >= nb || to == part) continue;
+            const uint32_t at = cluster_map(smem_u32(lin_smem) + slot(part, group), (uint32_t)to);
+#pragma unroll
+            for (int u = 0; u < 8; ++u) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at + u * 128), "f"(z[j][u]) : "memory");
+          }
+        }
+        cluster_sync_all();
+        if (ready) {
+#pragma unroll
+          for (int j = 0; j < GROUPS; ++j) {
+            const int group = 4 * j + cg;
+            if (8 * group >= nb || group % cut != part) continue;
+            for (int from = 0; from < cut; ++from) {
+              if (from == part) continue;
+              const float* got = reinterpret_cast<const float*>(lin_smem + slot(from, group));
+#pragma unroll
+              for (int u = 0; u < 8; ++u) z[j][u] += got[u * 32];
+            }
+          }
+        }
+      }
       if (!ready) break;
       if (in) {
 #pragma unroll
         for (int j = 0; j < GROUPS; ++j) {
           const int c0 = 32 * j + 8 * cg;
           if (c0 >= cols) break;
+          if (CUT && (4 * j + cg) % cut != part) continue;
           const long long c = col + c0;
           T* y = static_cast<T*>(a.Y) + c * a.ldy + i;
           const T* res = static_cast<const T*>(a.R) + c * a.ldr + i;
@@ -250,7 +286,7 @@ __global__ void __launch_bounds__(lin_threads(MODE), 1) linear_tc_kernel(const _
     const int team = (warp - kSplitWarp0) / kSplitWarps, me = (warp - kSplitWarp0) % kSplitWarps * 32 + lane;
     const int wv = w_bytes / 16, xv = x_bytes / 16;
     long long its = 0;
-    for (int tile = unit; tile < n_tiles; tile += n_units) its += p.kb;
+    for (int tile = unit; tile < n_tiles; tile += n_units) its += kb;
     int st = team % p.stages;
     uint32_t ph = (uint32_t)(team / p.stages) & 1u;
     for (long long it = team; it < its && sound; it += kSplitTeams) {
@@ -277,6 +313,10 @@ __global__ void __launch_bounds__(lin_threads(MODE), 1) linear_tc_kernel(const _
     }
   }
   __syncwarp();
+  if (CUT && warp >= kEpiWarps) {  // (the epilogue's two cluster barriers are everybody's)
+    cluster_sync_all();
+    cluster_sync_all();
+  }
   tc_fence_before();
   __syncthreads();
   if constexpr (CG == 2) cluster_sync_all();  // neither CTA ends while the other one's MMAs read its tiles or its arrivals come in
@@ -296,7 +336,7 @@ __global__ void __launch_bounds__(256) linear_align_kernel(const T* src, long lo
 
 struct LinPlan {
   bool few;
-  int cg, nb, n_ct;
+  int cg, nb, n_ct, cut;
   bool align_w, align_x;
   long long ld_pad;         // elements of a row that was moved
   size_t w_bytes, x_bytes;  // of the workspace
@@ -308,17 +348,26 @@ LinPlan lin_plan(const LinearArgs& a, int elem) {
   const long long rows1 = (a.n + 127) / 128, rows2 = (a.n + 255) / 256;
   pl.few = a.N <= 32 || a.n <= 16;
   if (pl.few) return pl;
-  // the time of a launch: tiles of the busiest unit x (columns of a tile, at least what the issue of an MMA takes)
+  // The time of a launch in cycles: the tiles of the busiest unit, each its k-blocks and a start and an end.  A k-block takes the longest of its MMAs,
+  // what goes through shared memory at 128 bytes per cycle (TMA's writes and the MMAs' reads of w and x columns; in 32 bits the
+  // splitting's reads and writes, too), and its way from the L2 at 70.
   double best = 0;
+  const bool f32 = elem == ELEM_F32;
   for (int cg = 1; cg <= 2; ++cg)
-    for (int w = lin_max_nb(elem); w >= 32; w -= 32) {
+    for (int w = lin_max_nb(elem, false); w >= 32; w -= 32) {
       const int n_ct = (a.N - 1) / w + 1, nb = ((a.N - 1) / n_ct + 32) / 32 * 32;
       if ((long long)nb * (n_ct - 1) >= a.N) continue;
-      const long long tiles = (cg == 2 ? rows2 : rows1) * n_ct, waves = (tiles + sms / cg - 1) / (sms / cg);
-      const double cost = waves * (kb * (elem == ELEM_F32 ? 3.0 : 1.0) * std::max(nb * (cg == 2 ? 1.0 : 1.25), 48.0) + 600.0);
-      if (pl.nb == 0 || cost < best) {
-        best = cost;
-        pl.cg = cg; pl.nb = nb; pl.n_ct = n_ct;
+      const long long tiles = (cg == 2 ? rows2 : rows1) * n_ct;
+      const double x = (double)nb / cg, mma = nb * (f32 ? 6.0 : 2.0), fill = (128 + x) * 128 / 70;
+      const double smem = f32 ? 3 * (128 + x) + (cg == 2 ? 384 + 3 * x : 256 + 3 * x) : 256 + 2 * x, block = std::max(mma, std::max(smem, fill));
+      for (int cut = 1; cut <= 8; cut *= 2) {
+        if (cut > 1 && (cg == 2 || tiles * cut > sms || kb < 4 * cut || nb / 8 < cut || nb > lin_max_nb(elem, true))) break;
+        const long long waves = (tiles * cut + sms / cg - 1) / (sms / cg);
+        const double cost = waves * (block * ((kb + cut - 1) / cut) + 12.0 * nb / cut) + 3000 + (cut > 1 ? 2000 + 4 * nb : 0);
+        if (pl.nb == 0 || cost < best) {
+          best = cost;
+          pl.cg = cg; pl.nb = nb; pl.n_ct = n_ct; pl.cut = cut;
+        }
       }
     }
   const auto off16 = [&](const void* p, long long ld) { return ((uintptr_t)p & 15) != 0 || (ld * eb) % 16 != 0; };
@@ -331,7 +380,7 @@ LinPlan lin_plan(const LinearArgs& a, int elem) {
   return pl;
 }
 
-template <int MODE, int CG, int ACT>
+template <int MODE, int CG, int ACT, bool CUT>
 cudaError_t lin_launch(LinParams& p, cudaStream_t st) {
   const int raw = (128 + p.nb / CG) * 128, stage = raw * (MODE == LIN_F32 ? 2 : 1);
   p.stages = std::min((kSmem - (int)sizeof(LinCtrl)) / stage, (int)kMaxStages);
@@ -339,35 +388,35 @@ cudaError_t lin_launch(LinParams& p, cudaStream_t st) {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
   if (!configured[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(linear_tc_kernel<MODE, CG, ACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    const cudaError_t e = cudaFuncSetAttribute(linear_tc_kernel<MODE, CG, ACT, CUT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
     if (e != cudaSuccess) return e;
     configured[dev] = true;
   }
   cudaLaunchConfig_t cfg;
   std::memset(&cfg, 0, sizeof(cfg));
-  cfg.gridDim = dim3((unsigned)(CG * std::min<long long>((long long)p.r_tiles * p.n_ct, device_sms() / CG)));
+  cfg.gridDim = dim3((unsigned)(CG * p.cut * std::min<long long>((long long)p.r_tiles * p.n_ct, p.cut > 1 ? (1ll << 30) : device_sms() / CG)));
   cfg.blockDim = dim3(lin_threads(MODE));
   cfg.dynamicSmemBytes = kSmem;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = CG;
+  attr[0].val.clusterDim.x = CG * p.cut;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = CG == 2 ? 1 : 0;
+  cfg.numAttrs = CG * p.cut > 1 ? 1 : 0;
   count_launch();
-  return cudaLaunchKernelEx(&cfg, linear_tc_kernel<MODE, CG, ACT>, p);
+  return cudaLaunchKernelEx(&cfg, linear_tc_kernel<MODE, CG, ACT, CUT>, p);
 }
-template <int MODE, int CG>
+template <int MODE, int CG, bool CUT>
 cudaError_t lin_act(LinParams& p, cudaStream_t st) {
   switch (p.a.act) {
-    case ACT_TANH: return lin_launch<MODE, CG, ACT_TANH>(p, st);
-    case ACT_SIGMOID: return lin_launch<MODE, CG, ACT_SIGMOID>(p, st);
-    case ACT_RELU: return lin_launch<MODE, CG, ACT_RELU>(p, st);
-    case ACT_GELU: return lin_launch<MODE, CG, ACT_GELU>(p, st);
-    case ACT_SILU: return lin_launch<MODE, CG, ACT_SILU>(p, st);
+    case ACT_TANH: return lin_launch<MODE, CG, ACT_TANH, CUT>(p, st);
+    case ACT_SIGMOID: return lin_launch<MODE, CG, ACT_SIGMOID, CUT>(p, st);
+    case ACT_RELU: return lin_launch<MODE, CG, ACT_RELU, CUT>(p, st);
+    case ACT_GELU: return lin_launch<MODE, CG, ACT_GELU, CUT>(p, st);
+    case ACT_SILU: return lin_launch<MODE, CG, ACT_SILU, CUT>(p, st);
   }
-  return lin_launch<MODE, CG, ACT_NONE>(p, st);
+  return lin_launch<MODE, CG, ACT_NONE, CUT>(p, st);
 }
 template <int MODE>
 cudaError_t lin_type(const LinearArgs& all, const LinPlan& pl, cudaStream_t st) {
@@ -396,11 +445,12 @@ cudaError_t lin_type(const LinearArgs& all, const LinPlan& pl, cudaStream_t st) 
   }
   p.nb = pl.nb;
   p.n_ct = pl.n_ct;
+  p.cut = pl.cut;
   p.r_tiles = (all.n + 128 * pl.cg - 1) / (128 * pl.cg);
   p.kb = (int)((all.K * (long long)sizeof(T) + 127) / 128);
   if (!make_kmajor_map(&p.w, p.a.W, sizeof(T), all.K, all.n, p.a.ldw, 128) || !make_kmajor_map(&p.x, p.a.X, sizeof(T), all.K, all.N, p.a.ldx, pl.nb / pl.cg))
     return cudaErrorInvalidValue;
-  return pl.cg == 2 ? lin_act<MODE, 2>(p, st) : lin_act<MODE, 1>(p, st);
+  return pl.cg == 2 ? lin_act<MODE, 2, false>(p, st) : pl.cut > 1 ? lin_act<MODE, 1, true>(p, st) : lin_act<MODE, 1, false>(p, st);
 }
 
 }  // namespace
