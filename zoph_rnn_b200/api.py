@@ -569,14 +569,20 @@ def _at(t):
     return None if t is None else t.data_ptr()
 
 
+@functools.lru_cache(maxsize=1024)
+def _memory4_sizes(B, S_max, heads, d):
+    nc, ns = ctypes.c_size_t(), ctypes.c_size_t()
+    check(lib().zrnn_memory4_sizes(B, S_max, heads, d, ctypes.byref(nc), ctypes.byref(ns)))
+    return nc.value, ns.value
+
+
 class memory4:
     """The states that attention reads, held in 4 bits (zrnn_memory4_* in include/zrnn.h): B source columns of S_max slots with
     `heads` vectors of d elements each (heads = 1, d = H for this library's models).  codes [B, S_max, heads, groups * 16] uint8 and
     scales [B, S_max, heads, groups] float16 may be given; otherwise they are made, uninitialised."""
 
     def __init__(self, B, S_max, d, heads=1, codes=None, scales=None):
-        nc, ns = ctypes.c_size_t(), ctypes.c_size_t()
-        check(lib().zrnn_memory4_sizes(B, S_max, heads, d, ctypes.byref(nc), ctypes.byref(ns)))
+        _memory4_sizes(B, S_max, heads, d)  # (refuses what the library does not take)
         self.B, self.S_max, self.heads, self.d = B, S_max, heads, d
         g = -(-d // 32)
         if codes is None:

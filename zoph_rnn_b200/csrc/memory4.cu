@@ -13,54 +13,188 @@ namespace {
 constexpr float kSeventh = 0.14285714924335479736328125f;  // 1/7 rounded to 32 bits
 constexpr float kMaxScale = 9352.0f;                       // the largest half that times 7 is finite
 
-// A warp per group, a lane per element.  The scale is fp16(a / 7) of the largest magnitude a (a product with 1/7 in 32 bits).  The code is the
-// integer nearest to x / s, ties to even: the rounded quotient can be off by one only where 32 bits end up on the middle between two codes,
-// which the remainder x - q s (exact: at most 24 bits) tells apart.
-template <class T>
-__global__ void __launch_bounds__(256) mem4_pack_kernel(const Mem4Pack a) {
-  const int G = mem4_groups(a.d), lane = threadIdx.x & 31;
-  const long long total = (long long)a.S * a.B * a.heads * G;
-  for (long long w = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); w < total; w += (long long)gridDim.x * 8) {
-    const int g = (int)(w % G);
-    long long r = w / G;
-    const int h = (int)(r % a.heads);
-    r /= a.heads;
-    const int b = (int)(r % a.B), s = (int)(r / a.B);
-    const int i = g * kMem4Group + lane;
-    const float x = i < a.d ? to_f32(static_cast<const T*>(a.x)[s * a.ld_slot + b * a.ld_col + (long long)h * a.d + i]) : 0.f;
-    unsigned m = __float_as_uint(x) & 0x7fffffffu;  // (as integers: a NaN is the largest)
-    m = __reduce_max_sync(0xffffffffu, m);
-    const __half sh = m < 0x7f800000u ? __float2half_rn(fminf(__uint_as_float(m) * kSeventh, kMaxScale)) : __ushort_as_half(0x7e00);
-    const float sc = __half2float(sh);
-    int q = 0;
-    if (sc > 0.f) {
-      float f = rintf(__fdiv_rn(x, sc));
-      const float rem = 2.f * fmaf(-f, sc, x);
-      if (fabsf(f) <= 16.f) f += rem > sc ? 1.f : (rem < -sc ? -1.f : 0.f);
-      q = (int)fminf(fmaxf(f, -7.f), 7.f);
+// The scale is fp16(a / 7) of the group's largest magnitude a (a product with 1/7 in 32 bits).
+__device__ __forceinline__ __half mem4_scale(float a) {
+  return a < INFINITY ? __float2half_rn(fminf(a * kSeventh, kMaxScale)) : __ushort_as_half(0x7e00);
+}
+// Eight codes: the integer nearest to x / s, ties to even, plus 8.  An addition of 1.5 * 2^23 rounds x times the reciprocal to a whole number, and
+// four of them are put together by multiplications with powers of 16.  The product may lie on the wrong side of the middle between two
+// numbers, by some 2^-20: next to the middle the remainder x - f s decides (exact: at most 24 bits), a tie being one where twice that is s.
+constexpr float kWhole = 12582912.f;
+__device__ __forceinline__ float mem4_near(float x, float s, float f) {
+  const float rem = 2.f * fmaf(-f, s, x);
+  const bool odd = ((int)f & 1) != 0;
+  if (rem > s || (rem == s && odd)) return f + 1.f;
+  if (rem < -s || (rem == -s && odd)) return f - 1.f;
+  return f;
+}
+// two 32-bit operations in one instruction
+__device__ __forceinline__ unsigned long long pair_of(float x, float y) {
+  unsigned long long r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void of_pair(unsigned long long p, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(p)); }
+__device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigned long long b) {
+  unsigned long long r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b) {
+  unsigned long long r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ unsigned mem4_codes(const float (&x)[8], float s) {
+  float inv;  // (s is no less than 2^-24; an approximation will do)
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+  const unsigned long long inv2 = pair_of(inv, inv), whole = pair_of(kWhole, kWhole), less = pair_of(-kWhole, -kWhole);
+  float f[8], far = 0.f;
+#pragma unroll
+  for (int u = 0; u < 8; u += 2) {
+    float t0, t1, d0, d1;
+    of_pair(mul2(pair_of(x[u], x[u + 1]), inv2), t0, t1);
+    t0 = fminf(fmaxf(t0, -7.25f), 7.25f);  // (beyond: 7)
+    t1 = fminf(fmaxf(t1, -7.25f), 7.25f);
+    const unsigned long long t = pair_of(t0, t1), r = add2(add2(t, whole), less);
+    of_pair(r, f[u], f[u + 1]);
+    of_pair(add2(t, pair_of(-f[u], -f[u + 1])), d0, d1);
+    far = fmaxf(far, fmaxf(fabsf(d0), fabsf(d1)));
+  }
+  if (far > 0.4999f) {
+#pragma unroll
+    for (int u = 0; u < 8; ++u) f[u] = fminf(fmaxf(mem4_near(x[u], s, f[u]), -7.f), 7.f);
+  }
+  constexpr float eights = 8.f + 128.f + 2048.f + 32768.f;
+  const float lo = fmaf(f[3], 4096.f, fmaf(f[2], 256.f, fmaf(f[1], 16.f, f[0]))) + (kWhole + eights);
+  const float hi = fmaf(f[7], 4096.f, fmaf(f[6], 256.f, fmaf(f[5], 16.f, f[4]))) + (kWhole + eights);
+  return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x5410);
+}
+__device__ __forceinline__ float max_nan(float x, float y) {  // NaN if one of them is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+__device__ __forceinline__ __half2 bits_h2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
+// Nibbles 0 .. 3 of each half of x, as pairs (low half, high half) of q * s: 1024 + u and 1024 + 16 u are halves made by or-ing u into a
+// mantissa, and what follows is exact but for the last product, whose rounding is the definition's.
+__device__ __forceinline__ void dequant4(uint32_t x, __half2 s, uint32_t (&v)[4]) {
+  const __half2 m1032 = __half2half2(__ushort_as_half(0xe408)), sixteenth = __half2half2(__ushort_as_half(0x2c00)), m72 = __half2half2(__ushort_as_half(0xd480));
+  const uint32_t y = x >> 8;
+  uint32_t a, b, c, d;
+  asm("lop3.b32 %0, %1, 0x000f000f, 0x64006400, 0xea;" : "=r"(a) : "r"(x));
+  asm("lop3.b32 %0, %1, 0x00f000f0, 0x64006400, 0xea;" : "=r"(b) : "r"(x));
+  asm("lop3.b32 %0, %1, 0x000f000f, 0x64006400, 0xea;" : "=r"(c) : "r"(y));
+  asm("lop3.b32 %0, %1, 0x00f000f0, 0x64006400, 0xea;" : "=r"(d) : "r"(y));
+  v[0] = h2_bits(__hmul2_rn(__hadd2_rn(bits_h2(a), m1032), s));
+  v[1] = h2_bits(__hmul2_rn(__hfma2(bits_h2(b), sixteenth, m72), s));
+  v[2] = h2_bits(__hmul2_rn(__hadd2_rn(bits_h2(c), m1032), s));
+  v[3] = h2_bits(__hmul2_rn(__hfma2(bits_h2(d), sixteenth, m72), s));
+}
+template <class T> struct Mem4Vec;  // 8 elements
+template <> struct Mem4Vec<float> {
+  static __device__ void load(const float* p, float (&x)[8]) {
+    const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+  }
+  static __device__ void store(float* p, const float (&x)[8]) {
+    reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+  }
+};
+template <class T> struct Mem4Vec {
+  static __device__ void load(const T* p, float (&x)[8]) {
+    const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
+    const unsigned w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (std::is_same<T, __half>::value) {
+        x[2 * i] = __half2float(__ushort_as_half((unsigned short)w[i]));
+        x[2 * i + 1] = __half2float(__ushort_as_half((unsigned short)(w[i] >> 16)));
+      } else {
+        x[2 * i] = __uint_as_float(w[i] << 16);
+        x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      }
     }
-    const unsigned u = (unsigned)(q + 8);
-    const unsigned pair = u | (__shfl_down_sync(0xffffffffu, u, 1) << 4);
-    const long long row = (((long long)b * a.S_cap + a.slot0 + s) * a.heads + h) * G + g;
-    if ((lane & 1) == 0) a.codes[row * 16 + (lane >> 1)] = (uint8_t)pair;
-    if (lane == 0) a.scales[row] = sh;
+  }
+  static __device__ void store(T* p, const float (&x)[8]) {
+    unsigned w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const T a = from_f32<T>(x[2 * i]), b = from_f32<T>(x[2 * i + 1]);
+      w[i] = (unsigned)*reinterpret_cast<const unsigned short*>(&a) | (unsigned)*reinterpret_cast<const unsigned short*>(&b) << 16;
+    }
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+};
+
+// A lane takes 8 elements, four lanes a group, a team of lanes one source column, whose slots it walks through: all indices are computed once
+// per thread (divided per vector, they were two thirds of the instructions).  ALIGNED: vectors lie on 16 bytes and a head is a
+// multiple of 8 elements.
+template <class T, bool ALIGNED>
+__global__ void __launch_bounds__(256) mem4_pack_kernel(const Mem4Pack a, int team) {
+  const int G = mem4_groups(a.d), lane = threadIdx.x % team, sub = threadIdx.x / team, q = blockIdx.z * team + lane, quads = a.heads * G * 4;
+  const long long b = (long long)blockIdx.x * (256 / team) + sub;
+  if (sub >= 256 / team || b >= a.B || q >= quads) return;  // (whole groups of four leave)
+  const int g = q >> 2, h = g / G, i = (q - h * G * 4) * 8;
+  const T* x = static_cast<const T*>(a.x) + b * a.ld_col + (long long)h * a.d + i + blockIdx.y * a.ld_slot;
+  const long long row = (long long)a.heads * G, to = (b * a.S_cap + a.slot0 + blockIdx.y) * row + g;
+  unsigned* codes = reinterpret_cast<unsigned*>(a.codes) + to * 4 + (q & 3);
+  __half* scales = a.scales + to;
+  const unsigned four = 0xfu << (threadIdx.x & 28);
+  const long long x_step = gridDim.y * a.ld_slot, step = gridDim.y * row;
+#pragma unroll 2
+  for (int s = blockIdx.y; s < a.S; s += gridDim.y, x += x_step, codes += step * 4, scales += step) {
+    float v[8];
+    if (ALIGNED) {
+#pragma unroll
+      for (int u = 0; u < 8; ++u) v[u] = 0.f;
+      if (i < a.d) Mem4Vec<T>::load(x, v);
+    } else {
+#pragma unroll
+      for (int u = 0; u < 8; ++u) v[u] = i + u < a.d ? to_f32(__ldg(x + u)) : 0.f;
+    }
+    float m = fabsf(v[0]);
+#pragma unroll
+    for (int u = 1; u < 8; ++u) m = max_nan(m, fabsf(v[u]));
+    m = max_nan(m, __shfl_xor_sync(four, m, 1));
+    m = max_nan(m, __shfl_xor_sync(four, m, 2));
+    const __half sh = mem4_scale(m);
+    const float sc = __half2float(sh);
+    *codes = sc > 0.f ? mem4_codes(v, sc) : 0x88888888u;
+    if ((q & 3) == 0) *scales = sh;
   }
 }
-
-template <class T>
-__global__ void __launch_bounds__(256) mem4_unpack_kernel(const Mem4Unpack a) {
-  const int G = mem4_groups(a.d);
-  const long long total = (long long)a.B * a.S * a.heads * a.d;
-  for (long long e = (long long)blockIdx.x * 256 + threadIdx.x; e < total; e += (long long)gridDim.x * 256) {
-    const int i = (int)(e % a.d);
-    long long r = e / a.d;
-    const int h = (int)(r % a.heads);
-    r /= a.heads;
-    const int s = (int)(r % a.S), b = (int)(r / a.S);
-    const long long row = (((long long)b * a.S_cap + a.slot0 + s) * a.heads + h) * G + i / kMem4Group;
-    const unsigned c = a.codes[row * 16 + (i % kMem4Group) / 2];
-    const int q = (int)((i & 1) ? c >> 4 : c & 15) - 8;
-    static_cast<T*>(a.out)[e] = from_f32<T>(__half2float(__float2half_rn((float)q * __half2float(a.scales[row]))));
+template <class T, bool ALIGNED>
+__global__ void __launch_bounds__(256) mem4_unpack_kernel(const Mem4Unpack a, int team) {
+  const int G = mem4_groups(a.d), lane = threadIdx.x % team, sub = threadIdx.x / team, q = blockIdx.z * team + lane, quads = a.heads * G * 4;
+  const long long b = (long long)blockIdx.x * (256 / team) + sub;
+  const int g = q >> 2, h = g / G, i = (q - h * G * 4) * 8;
+  if (sub >= 256 / team || b >= a.B || q >= quads || i >= a.d) return;
+  const long long row = (long long)a.heads * G, from = (b * a.S_cap + a.slot0 + blockIdx.y) * row + g, width = (long long)a.heads * a.d;
+  const unsigned* codes = reinterpret_cast<const unsigned*>(a.codes) + from * 4 + (q & 3);
+  const __half* scales = a.scales + from;
+  T* out = static_cast<T*>(a.out) + (b * a.S + blockIdx.y) * width + (long long)h * a.d + i;
+  const long long step = gridDim.y * row;
+#pragma unroll 4
+  for (int s = blockIdx.y; s < a.S; s += gridDim.y, codes += step * 4, scales += step, out += gridDim.y * width) {
+    uint32_t p[4];  // (elements 0, 4), (1, 5), (2, 6), (3, 7)
+    dequant4(__ldg(codes), __half2half2(__ldg(scales)), p);
+    float v[8];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const float2 f = __half22float2(bits_h2(p[u]));
+      v[u] = f.x;
+      v[u + 4] = f.y;
+    }
+    if (ALIGNED) {
+      Mem4Vec<T>::store(out, v);
+    } else {
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (i + u < a.d) out[u] = from_f32<T>(v[u]);
+    }
   }
 }
 
@@ -112,23 +246,6 @@ __device__ __forceinline__ float warp_max(float x) {
   float y;
   asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
   return y;
-}
-__device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
-__device__ __forceinline__ __half2 bits_h2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
-// Nibbles 0 .. 3 of each half of x, as pairs (low half, high half) of q * s: 1024 + u and 1024 + 16 u are halves made by or-ing u into a
-// mantissa, and what follows is exact but for the last product, whose rounding is the definition's.
-__device__ __forceinline__ void dequant4(uint32_t x, __half2 s, uint32_t (&v)[4]) {
-  const __half2 m1032 = __half2half2(__ushort_as_half(0xe408)), sixteenth = __half2half2(__ushort_as_half(0x2c00)), m72 = __half2half2(__ushort_as_half(0xd480));
-  const uint32_t y = x >> 8;
-  uint32_t a, b, c, d;
-  asm("lop3.b32 %0, %1, 0x000f000f, 0x64006400, 0xea;" : "=r"(a) : "r"(x));
-  asm("lop3.b32 %0, %1, 0x00f000f0, 0x64006400, 0xea;" : "=r"(b) : "r"(x));
-  asm("lop3.b32 %0, %1, 0x000f000f, 0x64006400, 0xea;" : "=r"(c) : "r"(y));
-  asm("lop3.b32 %0, %1, 0x00f000f0, 0x64006400, 0xea;" : "=r"(d) : "r"(y));
-  v[0] = h2_bits(__hmul2_rn(__hadd2_rn(bits_h2(a), m1032), s));
-  v[1] = h2_bits(__hmul2_rn(__hfma2(bits_h2(b), sixteenth, m72), s));
-  v[2] = h2_bits(__hmul2_rn(__hadd2_rn(bits_h2(c), m1032), s));
-  v[3] = h2_bits(__hmul2_rn(__hfma2(bits_h2(d), sixteenth, m72), s));
 }
 // x as a half and, times 2^11, what that leaves
 __device__ __forceinline__ void split_half(float x, __half& hi, __half& lo) {
@@ -525,29 +642,45 @@ __global__ void __launch_bounds__(256) mem4_combine_kernel(const Mem4Attend a, c
 
 }  // namespace
 
-cudaError_t launch_mem4_pack(const Mem4Pack& a, int elem, cudaStream_t st) {
-  const long long warps = (long long)a.S * a.B * a.heads * mem4_groups(a.d);
-  if (warps == 0) return cudaSuccess;
-  const unsigned grid = (unsigned)std::min<long long>((warps + 7) / 8, 1 << 20);
-  count_launch();
-  switch (elem) {
-    case ELEM_F32: mem4_pack_kernel<float><<<grid, 256, 0, st>>>(a); break;
-    case ELEM_BF16: mem4_pack_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(a); break;
-    default: mem4_pack_kernel<__half><<<grid, 256, 0, st>>>(a);
-  }
+namespace {
+
+// Teams of as many lanes as a vector has (256 at most, then several CTAs share it); CTAs along the slots: eight per multiprocessor in all
+dim3 mem4_grid(int B, int S, int heads, int d, int* team) {
+  const int quads = heads * mem4_groups(d) * 4;
+  *team = std::min(quads, 256);
+  const long long x = (B + 256 / *team - 1) / (256 / *team), z = (quads + *team - 1) / *team;
+  const long long y = std::max<long long>(1, std::min<long long>(S, (16ll * device_sms() + x * z - 1) / (x * z)));
+  return dim3((unsigned)x, (unsigned)std::min<long long>(y, 65535), (unsigned)z);
+}
+template <class T>
+cudaError_t pack_type(const Mem4Pack& a, cudaStream_t st) {
+  int team;
+  const dim3 grid = mem4_grid(a.B, a.S, a.heads, a.d, &team);
+  const bool aligned = ((uintptr_t)a.x & 15) == 0 && a.ld_slot * sizeof(T) % 16 == 0 && a.ld_col * sizeof(T) % 16 == 0 && a.d % 8 == 0;
+  if (aligned) mem4_pack_kernel<T, true><<<grid, 256, 0, st>>>(a, team);
+  else mem4_pack_kernel<T, false><<<grid, 256, 0, st>>>(a, team);
   return cudaGetLastError();
 }
-cudaError_t launch_mem4_unpack(const Mem4Unpack& a, int elem, cudaStream_t st) {
-  const long long total = (long long)a.B * a.S * a.heads * a.d;
-  if (total == 0) return cudaSuccess;
-  const unsigned grid = (unsigned)std::min<long long>((total + 255) / 256, 1 << 20);
-  count_launch();
-  switch (elem) {
-    case ELEM_F32: mem4_unpack_kernel<float><<<grid, 256, 0, st>>>(a); break;
-    case ELEM_BF16: mem4_unpack_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(a); break;
-    default: mem4_unpack_kernel<__half><<<grid, 256, 0, st>>>(a);
-  }
+template <class T>
+cudaError_t unpack_type(const Mem4Unpack& a, cudaStream_t st) {
+  int team;
+  const dim3 grid = mem4_grid(a.B, a.S, a.heads, a.d, &team);
+  if (((uintptr_t)a.out & 15) == 0 && a.d % 8 == 0) mem4_unpack_kernel<T, true><<<grid, 256, 0, st>>>(a, team);
+  else mem4_unpack_kernel<T, false><<<grid, 256, 0, st>>>(a, team);
   return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_mem4_pack(const Mem4Pack& a, int elem, cudaStream_t st) {
+  if (a.S == 0) return cudaSuccess;
+  count_launch();
+  return elem == ELEM_F32 ? pack_type<float>(a, st) : elem == ELEM_BF16 ? pack_type<__nv_bfloat16>(a, st) : pack_type<__half>(a, st);
+}
+cudaError_t launch_mem4_unpack(const Mem4Unpack& a, int elem, cudaStream_t st) {
+  if (a.S == 0) return cudaSuccess;
+  count_launch();
+  return elem == ELEM_F32 ? unpack_type<float>(a, st) : elem == ELEM_BF16 ? unpack_type<__nv_bfloat16>(a, st) : unpack_type<__half>(a, st);
 }
 namespace {
 
