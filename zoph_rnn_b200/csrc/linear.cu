@@ -36,7 +36,7 @@ struct LinParams {
   CUtensorMap w, x;  // boxes of 128 rows and of nb / CG columns
   LinearArgs a;
   int nb, n_ct, r_tiles, kb, stages;
-  int cut;  // CTAs of a cluster that share a tile's K axis (1: none; not with pairs)
+  int cut_log2;  // 2^cut_log2 CTAs of a cluster share a tile's K axis (0: none; not with pairs)
 };
 struct alignas(16) LinCtrl {
   uint64_t full[kMaxStages], split[kMaxStages], empty[kMaxStages];
@@ -82,9 +82,9 @@ __global__ void __launch_bounds__(lin_threads(MODE), 1) linear_tc_kernel(const _
   static_assert(!CUT || CG == 1, "a pair's tiles are not cut");
   extern __shared__ __align__(1024) uint8_t lin_smem[];
   const int warp = uniform_warp(), lane = threadIdx.x & 31;
-  const int rank = CG == 2 ? (int)(blockIdx.x & 1) : 0, cut = CUT ? p.cut : 1, unit = blockIdx.x / (CG * cut), n_units = gridDim.x / (CG * cut);
-  const int part = CUT ? (int)blockIdx.x % cut : 0;
-  const int kb0 = CUT ? (int)((long long)p.kb * part / cut) : 0, kb = CUT ? (int)((long long)p.kb * (part + 1) / cut) - kb0 : p.kb;  // this CTA's k-blocks
+  const int rank = CG == 2 ? (int)(blockIdx.x & 1) : 0, cut = CUT ? 1 << p.cut_log2 : 1, unit = blockIdx.x / CG >> (CUT ? p.cut_log2 : 0), n_units = gridDim.x / CG >> (CUT ? p.cut_log2 : 0);
+  const int part = CUT ? (int)blockIdx.x & (cut - 1) : 0;
+  const int kb0 = CUT ? (int)((long long)p.kb * part >> p.cut_log2) : 0, kb = CUT ? (int)((long long)p.kb * (part + 1) >> p.cut_log2) - kb0 : p.kb;  // this CTA's k-blocks
   const int nb = p.nb, x_rows = nb / CG, w_bytes = 128 * 128, x_bytes = x_rows * 128, raw = w_bytes + x_bytes, stage = raw * (F32 ? 2 : 1);
   // a stage: W, X; in 32 bits also X lo and W lo, in that order: X and its rest are one operand of twice the columns
   const int w_off = w_bytes + 2 * x_bytes, acc = nb * (F32 ? 2 : 1);
@@ -228,29 +228,30 @@ __global__ void __launch_bounds__(lin_threads(MODE), 1) linear_tc_kernel(const _
         // The CTAs of the cluster each finish every cut-th group of 8 columns: the other ones' sums of it go into that CTA's shared memory, where
         // the operands were (one tile per cluster), and are added to its own in the order of the CTAs.
         cluster_sync_all();  // all MMAs of all of them are over
-        const int per = (nb / 8 + cut - 1) / cut;
-        auto slot = [&](int from, int group) { return (uint32_t)((((from * 4 + quad) * per + group / cut) * 256 + lane) * 4); };
+        const int per = (nb / 8 + cut - 1) >> p.cut_log2;
+        auto slot = [&](int from, int group) { return (uint32_t)((((from * 4 + quad) * per + (group >> p.cut_log2)) * 64 + lane) * 16); };
         if (ready) {
 #pragma unroll
           for (int j = 0; j < GROUPS; ++j) {
-            const int group = 4 * j + cg, to = group % cut;
-            if (8 * group >= nb || to == part) continue;
+            const int group = cg * (nb / 32) + j, to = group & (cut - 1);  // (a warp's groups go to different CTAs)
+            if (32 * j >= nb || to == part) continue;
             const uint32_t at = cluster_map(smem_u32(lin_smem) + slot(part, group), (uint32_t)to);
-#pragma unroll
-            for (int u = 0; u < 8; ++u) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at + u * 128), "f"(z[j][u]) : "memory");
+            st_cluster_v4(at, z[j][0], z[j][1], z[j][2], z[j][3]);
+            st_cluster_v4(at + 512, z[j][4], z[j][5], z[j][6], z[j][7]);
           }
         }
         cluster_sync_all();
         if (ready) {
 #pragma unroll
           for (int j = 0; j < GROUPS; ++j) {
-            const int group = 4 * j + cg;
-            if (8 * group >= nb || group % cut != part) continue;
+            const int group = cg * (nb / 32) + j;
+            if (32 * j >= nb || (group & (cut - 1)) != part) continue;
             for (int from = 0; from < cut; ++from) {
               if (from == part) continue;
-              const float* got = reinterpret_cast<const float*>(lin_smem + slot(from, group));
-#pragma unroll
-              for (int u = 0; u < 8; ++u) z[j][u] += got[u * 32];
+              const float4* got = reinterpret_cast<const float4*>(lin_smem + slot(from, group));
+              const float4 lo = got[0], hi = got[32];
+              z[j][0] += lo.x; z[j][1] += lo.y; z[j][2] += lo.z; z[j][3] += lo.w;
+              z[j][4] += hi.x; z[j][5] += hi.y; z[j][6] += hi.z; z[j][7] += hi.w;
             }
           }
         }
@@ -261,7 +262,7 @@ __global__ void __launch_bounds__(lin_threads(MODE), 1) linear_tc_kernel(const _
         for (int j = 0; j < GROUPS; ++j) {
           const int c0 = 32 * j + 8 * cg;
           if (c0 >= cols) break;
-          if (CUT && (4 * j + cg) % cut != part) continue;
+          if (CUT && ((cg * (nb / 32) + j) & (cut - 1)) != part) continue;
           const long long c = col + c0;
           T* y = static_cast<T*>(a.Y) + c * a.ldy + i;
           const T* res = static_cast<const T*>(a.R) + c * a.ldr + i;
@@ -327,11 +328,15 @@ __global__ void __launch_bounds__(lin_threads(MODE), 1) linear_tc_kernel(const _
   }
 }
 
-// Rows that no 16-byte copy can start at, moved to where one can: one element per thread and step
+// Rows that no 16-byte copy can start at, moved to where one can: 16 bytes of the new row per thread, from the words that hold them
 template <class T>
 __global__ void __launch_bounds__(256) linear_align_kernel(const T* src, long long ld, int rows, int K, T* dst, long long ld_dst) {
-  for (long long r = blockIdx.y; r < rows; r += gridDim.y)
-    for (int k = blockIdx.x * 256 + threadIdx.x; k < K; k += gridDim.x * 256) dst[r * ld_dst + k] = src[r * ld + k];
+  constexpr int V = 16 / (int)sizeof(T);
+  const int vecs = (K + V - 1) / V, lanes = min(vecs, 256), per = 256 / lanes, lane = threadIdx.x % lanes, sub = threadIdx.x / lanes;
+  if (sub >= per) return;
+  for (long long r = (long long)blockIdx.x * per + sub; r < rows; r += (long long)gridDim.x * per)
+    for (int q = blockIdx.y * lanes + lane; q < vecs; q += gridDim.y * lanes)
+      reinterpret_cast<uint4*>(dst + r * ld_dst)[q] = load16<T, false>(src + r * ld, q * V, K, true);
 }
 
 struct LinPlan {
@@ -346,11 +351,10 @@ LinPlan lin_plan(const LinearArgs& a, int elem) {
   std::memset(&pl, 0, sizeof(pl));
   const int eb = elem_bytes(elem), sms = device_sms(), kb = (a.K * eb + 127) / 128;
   const long long rows1 = (a.n + 127) / 128, rows2 = (a.n + 255) / 256;
-  pl.few = a.N <= 32 || a.n <= 16;
-  if (pl.few) return pl;
-  // The time of a launch in cycles: the tiles of the busiest unit, each its k-blocks and a start and an end.  A k-block takes the longest of its MMAs,
-  // what goes through shared memory at 128 bytes per cycle (TMA's writes and the MMAs' reads of w and x columns; in 32 bits the
-  // splitting's reads and writes, too), and its way from the L2 at 70.
+  // The time of a launch in ns, as measured with all multiprocessors at work: a start and an end (6 us, with a cut 8), and for the busiest unit's
+  // tiles the k-blocks or the epilogue, whichever takes longer.  A k-block of 16-bit operands takes the MMAs' time, but no less than
+  // 200 ns (its way from the L2); of 32 bits the splitting's and what shared memory lets through: a CTA 365 / 435 / 500 / 690 ns with 32 / 64 / 96 /
+  // 128 columns, a pair 510 up to 96 and 700 with 128 (four stages instead of five).
   double best = 0;
   const bool f32 = elem == ELEM_F32;
   for (int cg = 1; cg <= 2; ++cg)
@@ -358,12 +362,13 @@ LinPlan lin_plan(const LinearArgs& a, int elem) {
       const int n_ct = (a.N - 1) / w + 1, nb = ((a.N - 1) / n_ct + 32) / 32 * 32;
       if ((long long)nb * (n_ct - 1) >= a.N) continue;
       const long long tiles = (cg == 2 ? rows2 : rows1) * n_ct;
-      const double x = (double)nb / cg, mma = nb * (f32 ? 6.0 : 2.0), fill = (128 + x) * 128 / 70;
-      const double smem = f32 ? 3 * (128 + x) + (cg == 2 ? 384 + 3 * x : 256 + 3 * x) : 256 + 2 * x, block = std::max(mma, std::max(smem, fill));
+      const double block = !f32 ? std::max(200.0, 1.1 * nb) : cg == 2 ? (nb > 96 ? 700.0 : 510.0) : 300 + 2.1 * nb + (nb > 96 ? 120.0 : 0.0), end = 14.0 * nb;
       for (int cut = 1; cut <= 8; cut *= 2) {
-        if (cut > 1 && (cg == 2 || tiles * cut > sms || kb < 4 * cut || nb / 8 < cut || nb > lin_max_nb(elem, true))) break;
-        const long long waves = (tiles * cut + sms / cg - 1) / (sms / cg);
-        const double cost = waves * (block * ((kb + cut - 1) / cut) + 12.0 * nb / cut) + 3000 + (cut > 1 ? 2000 + 4 * nb : 0);
+        if (cut > 1 && (cg == 2 || kb < 4 * cut || nb / 8 < cut || nb > lin_max_nb(elem, true))) break;
+        // clusters of 4 and 8 CTAs that take whole multiprocessors do not fill the processing clusters: 33 and 15 of them on 148
+        const long long units = cut == 1 ? sms / cg : cut == 2 ? sms / 2 : cut == 4 ? sms * 33 / 148 : sms * 15 / 148, waves = (tiles + units - 1) / units;
+        if (cut > 1 && waves > 1) break;
+        const double cost = waves * std::max(block * ((kb + cut - 1) / cut), end) + end / cut + (cut > 1 ? 8000 : 6000);
         if (pl.nb == 0 || cost < best) {
           best = cost;
           pl.cg = cg; pl.nb = nb; pl.n_ct = n_ct; pl.cut = cut;
@@ -373,6 +378,18 @@ LinPlan lin_plan(const LinearArgs& a, int elem) {
   const auto off16 = [&](const void* p, long long ld) { return ((uintptr_t)p & 15) != 0 || (ld * eb) % 16 != 0; };
   pl.align_w = off16(a.W, a.ldw);
   pl.align_x = off16(a.X, a.ldx);
+  if (pl.align_w) best += 3000 + (double)a.n * a.K * eb / 1500;
+  if (pl.align_x) best += 3000 + (double)a.N * a.K * eb / 1500;
+  // The kernel for few columns: 4 us, and per chunk of a warp (64 bytes of K) its latency or its share of a multiprocessor that has many CTAs (both in ns, with
+  // tiles of 8, 16 and 32 columns).  Up to 8 columns it is ahead, up to 32 with few weights or rows that would have to be moved first.
+  static const double lat[2][3] = {{300, 460, 550}, {270, 460, 840}}, thr[2][3] = {{232, 390, 520}, {154, 230, 380}};
+  const int t = a.N <= 8 ? 0 : a.N <= 16 ? 1 : 2, cols = 8 << t;
+  const double ctas = (double)((a.n + 15) / 16) * ((a.N + cols - 1) / cols), chunks = (((long long)a.K * eb + 63) / 64 + 7) / 8;
+  pl.few = 4000 + chunks * std::max(lat[!f32][t], thr[!f32][t] * ctas / sms) <= best;
+  if (pl.few) {
+    pl.align_w = pl.align_x = false;
+    return pl;
+  }
   pl.ld_pad = (a.K * eb + 15) / 16 * 16 / eb;
   const auto whole = [](size_t b) { return (b + 255) / 256 * 256; };
   pl.w_bytes = pl.align_w ? whole((size_t)a.n * pl.ld_pad * eb) : 0;
@@ -394,16 +411,16 @@ cudaError_t lin_launch(LinParams& p, cudaStream_t st) {
   }
   cudaLaunchConfig_t cfg;
   std::memset(&cfg, 0, sizeof(cfg));
-  cfg.gridDim = dim3((unsigned)(CG * p.cut * std::min<long long>((long long)p.r_tiles * p.n_ct, p.cut > 1 ? (1ll << 30) : device_sms() / CG)));
+  cfg.gridDim = dim3((unsigned)((CG << p.cut_log2) * std::min<long long>((long long)p.r_tiles * p.n_ct, CUT ? (1ll << 30) : device_sms() / CG)));
   cfg.blockDim = dim3(lin_threads(MODE));
   cfg.dynamicSmemBytes = kSmem;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = CG * p.cut;
+  attr[0].val.clusterDim.x = CG << p.cut_log2;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = CG * p.cut > 1 ? 1 : 0;
+  cfg.numAttrs = CG == 2 || CUT ? 1 : 0;
   count_launch();
   return cudaLaunchKernelEx(&cfg, linear_tc_kernel<MODE, CG, ACT, CUT>, p);
 }
@@ -427,8 +444,9 @@ cudaError_t lin_type(const LinearArgs& all, const LinPlan& pl, cudaStream_t st) 
   char* work = static_cast<char*>(all.work);
   const auto move = [&](const void* src, long long ld, int rows, char* dst) {
     count_launch();
-    linear_align_kernel<T><<<dim3((unsigned)((all.K + 255) / 256), (unsigned)std::min(rows, 8192)), 256, 0, st>>>(static_cast<const T*>(src), ld, rows, all.K,
-                                                                                                               reinterpret_cast<T*>(dst), pl.ld_pad);
+    const int vecs = (int)((all.K * (long long)sizeof(T) + 15) / 16), lanes = std::min(vecs, 256), per = 256 / lanes;
+    linear_align_kernel<T><<<dim3((unsigned)std::min((rows + per - 1) / per, 16 * device_sms()), (unsigned)((vecs + lanes - 1) / lanes)), 256, 0, st>>>(
+        static_cast<const T*>(src), ld, rows, all.K, reinterpret_cast<T*>(dst), pl.ld_pad);
     return cudaGetLastError();
   };
   if (pl.align_w) {
@@ -445,7 +463,7 @@ cudaError_t lin_type(const LinearArgs& all, const LinPlan& pl, cudaStream_t st) 
   }
   p.nb = pl.nb;
   p.n_ct = pl.n_ct;
-  p.cut = pl.cut;
+  while (1 << p.cut_log2 < pl.cut) ++p.cut_log2;
   p.r_tiles = (all.n + 128 * pl.cg - 1) / (128 * pl.cg);
   p.kb = (int)((all.K * (long long)sizeof(T) + 127) / 128);
   if (!make_kmajor_map(&p.w, p.a.W, sizeof(T), all.K, all.n, p.a.ldw, 128) || !make_kmajor_map(&p.x, p.a.X, sizeof(T), all.K, all.N, p.a.ldx, pl.nb / pl.cg))

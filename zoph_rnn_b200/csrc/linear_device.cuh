@@ -2,6 +2,7 @@
 #pragma once
 #include <cuda_runtime.h>
 
+#include "att_device.cuh"
 #include "operators.cuh"
 
 namespace zrnn {
@@ -9,11 +10,11 @@ namespace {
 
 __device__ __forceinline__ float linear_act(float x, int act) {
   switch (act) {
-    case ACT_TANH: return tanhf(x);
-    case ACT_SIGMOID: return 1.0f / (1.0f + expf(-x));
+    case ACT_TANH: return tanh_f32(x);  // (the gates' functions: within 1.2e-7, in a third of tanhf's and an IEEE division's instructions)
+    case ACT_SIGMOID: return sigmoid_f32(x);
     case ACT_RELU: return x > 0.f ? x : (x != x ? x : 0.f);  // (a NaN stays one)
     case ACT_GELU: return 0.5f * x * (1.0f + erff(x * 0.70710678118654752f));
-    case ACT_SILU: return x / (1.0f + expf(-x));
+    case ACT_SILU: return x * sigmoid_f32(x);
   }
   return x;
 }
@@ -25,6 +26,40 @@ __device__ __forceinline__ uint32_t tf32_rest(uint32_t x) { return __float_as_ui
 __device__ __forceinline__ void split_tf32(uint32_t x, uint32_t& hi, uint32_t& lo) {
   hi = x;
   lo = tf32_rest(x);
+}
+
+// 16 bytes of a row from element k on, zeros from K on.  Rows that lie on 16 bytes with K a multiple of a vector: one load.
+template <class T, bool ALIGNED>
+__device__ __forceinline__ uint4 load16(const T* row, int k, int K, bool in) {
+  constexpr int V = 16 / sizeof(T);
+  uint4 r = make_uint4(0u, 0u, 0u, 0u);
+  if (!in || k >= K) return r;
+  if (ALIGNED) return __ldg(reinterpret_cast<const uint4*>(row + k));
+  if constexpr (sizeof(T) == 4) {
+    const unsigned* p = reinterpret_cast<const unsigned*>(row + k);
+    r.x = __ldg(p);
+    if (k + 1 < K) r.y = __ldg(p + 1);
+    if (k + 2 < K) r.z = __ldg(p + 2);
+    if (k + 3 < K) r.w = __ldg(p + 3);
+  } else {
+    const unsigned short* p = reinterpret_cast<const unsigned short*>(row + k);
+    if (k + V < K) {  // (not the row's last element: the fifth word ends inside the row)
+      const unsigned* q = reinterpret_cast<const unsigned*>((uintptr_t)p & ~(uintptr_t)3);
+      const unsigned odd = ((uintptr_t)p & 2) * 8;
+      unsigned w[5];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = __ldg(q + i);
+      w[4] = odd ? __ldg(q + 4) : 0u;
+      r = make_uint4(__funnelshift_r(w[0], w[1], odd), __funnelshift_r(w[1], w[2], odd), __funnelshift_r(w[2], w[3], odd), __funnelshift_r(w[3], w[4], odd));
+    } else {
+      unsigned w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (k + i < K) w[i / 2] |= (unsigned)__ldg(p + i) << (16 * (i & 1));
+      r = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+  return r;
 }
 
 // tensor memory for a CTA without a partner, by one warp

@@ -28,40 +28,6 @@ __device__ __forceinline__ void mma8(float (&c)[4], uint32_t a0, uint32_t a1, ui
   asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// 16 bytes of a row from element k on, zeros from K on.  Rows that lie on 16 bytes with K a multiple of a vector: one load.
-template <class T, bool ALIGNED>
-__device__ __forceinline__ uint4 load16(const T* row, int k, int K, bool in) {
-  constexpr int V = 16 / sizeof(T);
-  uint4 r = make_uint4(0u, 0u, 0u, 0u);
-  if (!in || k >= K) return r;
-  if (ALIGNED) return __ldg(reinterpret_cast<const uint4*>(row + k));
-  if constexpr (sizeof(T) == 4) {
-    const unsigned* p = reinterpret_cast<const unsigned*>(row + k);
-    r.x = __ldg(p);
-    if (k + 1 < K) r.y = __ldg(p + 1);
-    if (k + 2 < K) r.z = __ldg(p + 2);
-    if (k + 3 < K) r.w = __ldg(p + 3);
-  } else {
-    const unsigned short* p = reinterpret_cast<const unsigned short*>(row + k);
-    if (k + V < K) {  // (not the row's last element: the fifth word ends inside the row)
-      const unsigned* q = reinterpret_cast<const unsigned*>((uintptr_t)p & ~(uintptr_t)3);
-      const unsigned odd = ((uintptr_t)p & 2) * 8;
-      unsigned w[5];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = __ldg(q + i);
-      w[4] = odd ? __ldg(q + 4) : 0u;
-      r = make_uint4(__funnelshift_r(w[0], w[1], odd), __funnelshift_r(w[1], w[2], odd), __funnelshift_r(w[2], w[3], odd), __funnelshift_r(w[3], w[4], odd));
-    } else {
-      unsigned w[4] = {0u, 0u, 0u, 0u};
-#pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (k + i < K) w[i / 2] |= (unsigned)__ldg(p + i) << (16 * (i & 1));
-      r = make_uint4(w[0], w[1], w[2], w[3]);
-    }
-  }
-  return r;
-}
-
 constexpr int kFewWarps = 8;
 template <class T, int NT, bool ALIGNED>
 __global__ void __launch_bounds__(kFewWarps * 32) linear_few_kernel(const LinearArgs a) {
