@@ -34,13 +34,15 @@ __host__ __device__ constexpr int lin_max_nb(int mode, bool cut) { return mode =
 __host__ __device__ constexpr uint32_t lin_fmt(int mode) { return mode == LIN_BF16 ? 1u : mode == LIN_F16 ? 0u : 2u; }
 struct LinParams {
   CUtensorMap w, x;  // boxes of 128 rows and of nb / CG columns
+  CUtensorMap y, r;  // bulk: 128 outputs x nb columns
+  int bulk;          // outputs and residual go through shared memory, as whole tiles
   LinearArgs a;
   int nb, n_ct, r_tiles, kb, stages;
   int cut_log2;  // 2^cut_log2 CTAs of a cluster share a tile's K axis (0: none; not with pairs)
 };
 struct alignas(16) LinCtrl {
   uint64_t full[kMaxStages], split[kMaxStages], empty[kMaxStages];
-  uint64_t acc_full[2], acc_empty[2];
+  uint64_t acc_full[2], acc_empty[2], res_full;
   uint32_t tmem_base;
   int abort;
 };
@@ -100,6 +102,7 @@ __global__ void __launch_bounds__(lin_threads(MODE), 1) linear_tc_kernel(const _
       mbar_init(&ct.acc_full[b], 1);
       mbar_init(&ct.acc_empty[b], CG * kEpiWarps);
     }
+    mbar_init(&ct.res_full, 1);
     ct.abort = (smem_u32(lin_smem) & 1023) ? 1 : 0;
     if (ct.abort && p.a.err) atomicExch(p.a.err, 8);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -191,7 +194,19 @@ __global__ void __launch_bounds__(lin_threads(MODE), 1) linear_tc_kernel(const _
     const LinearArgs& a = p.a;
     int use = 0;
     bool ready = sound;
-    for (int tile = unit; tile < n_tiles && (ready || CUT); tile += n_units) {
+    // bulk: one thread brings a tile's residual and takes its outputs away; both lie at `out`, 128 outputs per column
+    constexpr bool BULK = !F32 && !CUT;
+    T* out = reinterpret_cast<T*>(lin_smem + (size_t)p.stages * stage + ((sizeof(LinCtrl) + 127) / 128) * 128);
+    const bool one = BULK && threadIdx.x == 0;
+    uint32_t res_ph = 0;
+    auto bring_residual = [&](int tile) {
+      const int row = (tile / p.n_ct * CG + rank) * 128;
+      if (tile >= n_tiles || row >= a.n) return;
+      mbar_expect_tx(&ct.res_full, (uint32_t)(128 * nb * sizeof(T)));
+      tma_load_2d(out, &p.r, &ct.res_full, row, tile % p.n_ct * nb);
+    };
+    if (BULK && p.bulk && a.R && one && sound) bring_residual(unit);
+    for (int tile = unit; tile < n_tiles && (ready || CUT || (BULK && p.bulk)); tile += n_units) {  // (to the end even after a wait that gave up: barriers)
       const int col = tile % p.n_ct * nb, cols = min(nb, a.N - col), i = (tile / p.n_ct * CG + rank) * 128 + quad * 32 + lane;
       const bool in = i < a.n;
       const float bias = in && a.bias ? __ldg(a.bias + i) : 0.f;
@@ -256,6 +271,37 @@ __global__ void __launch_bounds__(lin_threads(MODE), 1) linear_tc_kernel(const _
           }
         }
       }
+      if (BULK && p.bulk) {
+        const int row = (tile / p.n_ct * CG + rank) * 128;
+        if (row < a.n) {  // (the same for the whole CTA)
+          if (a.R && ready) {
+            ready = __all_sync(0xffffffffu, mbar_wait(&ct.res_full, res_ph, &ct.abort, a.err, 7));
+            res_ph ^= 1u;
+          }
+          T* o = out + quad * 32 + lane;
+#pragma unroll
+          for (int j = 0; j < GROUPS; ++j) {
+            const int c0 = 32 * j + 8 * cg;
+            if (c0 >= nb || !ready) break;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+              float v = linear_act(z[j][u] + bias, ACT);
+              if (a.R) v += to_f32(o[(c0 + u) * 128]);
+              o[(c0 + u) * 128] = from_f32<T>(v);
+            }
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          asm volatile("bar.sync 1, %0;" ::"n"(kEpiWarps * 32) : "memory");
+          if (one && ready) {
+            asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(&p.y), "r"(smem_u32(out)), "r"(row), "r"(col) : "memory");
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+            asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+            if (a.R) bring_residual(tile + n_units);
+          }
+          asm volatile("bar.sync 1, %0;" ::"n"(kEpiWarps * 32) : "memory");  // the tile's place is free again
+        }
+        continue;
+      }
       if (!ready) break;
       if (in) {
 #pragma unroll
@@ -281,6 +327,7 @@ __global__ void __launch_bounds__(lin_threads(MODE), 1) linear_tc_kernel(const _
       }
       __syncwarp();
     }
+    if (BULK && p.bulk && one) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   } else if (F32) {
     // ------------------------------------------------------------ the lo parts of a stage: what tf32 cuts off of the tile beside it
     // Two teams of four warps take every other k-block each: one's waits are filled by the other.
@@ -352,9 +399,9 @@ LinPlan lin_plan(const LinearArgs& a, int elem) {
   const int eb = elem_bytes(elem), sms = device_sms(), kb = (a.K * eb + 127) / 128;
   const long long rows1 = (a.n + 127) / 128, rows2 = (a.n + 255) / 256;
   // The time of a launch in ns, as measured with all multiprocessors at work: a start and an end (6 us, with a cut 8), and for the busiest unit's
-  // tiles the k-blocks or the epilogue, whichever takes longer.  A k-block of 16-bit operands takes the MMAs' time, but no less than
-  // 200 ns (its way from the L2); of 32 bits the splitting's and what shared memory lets through: a CTA 365 / 435 / 500 / 690 ns with 32 / 64 / 96 /
-  // 128 columns, a pair 510 up to 96 and 700 with 128 (four stages instead of five).
+  // tiles the k-blocks or the epilogue, whichever takes longer.  A k-block of 16-bit operands takes a pair the MMAs' time, a CTA that of
+  // its shared memory (450 ns with 224 columns), but no less than 200 ns (its way from the L2); of 32 bits the splitting's and what shared memory lets through: a CTA 400 / 480 / 550 / 760 ns with 32 / 64 / 96 /
+  // 128 columns, a pair 640 up to 96 and 780 with 128 (a stage less).
   double best = 0;
   const bool f32 = elem == ELEM_F32;
   for (int cg = 1; cg <= 2; ++cg)
@@ -362,7 +409,7 @@ LinPlan lin_plan(const LinearArgs& a, int elem) {
       const int n_ct = (a.N - 1) / w + 1, nb = ((a.N - 1) / n_ct + 32) / 32 * 32;
       if ((long long)nb * (n_ct - 1) >= a.N) continue;
       const long long tiles = (cg == 2 ? rows2 : rows1) * n_ct;
-      const double block = !f32 ? std::max(200.0, 1.1 * nb) : cg == 2 ? (nb > 96 ? 700.0 : 510.0) : 300 + 2.1 * nb + (nb > 96 ? 120.0 : 0.0), end = 14.0 * nb;
+      const double block = !f32 ? (cg == 2 ? std::max(200.0, 1.1 * nb) : std::max(200.0, 140 + 1.4 * nb)) : cg == 2 ? (nb > 96 ? 780.0 : 640.0) : 330 + 2.3 * nb + (nb > 96 ? 130.0 : 0.0), end = 14.0 * nb;
       for (int cut = 1; cut <= 8; cut *= 2) {
         if (cut > 1 && (cg == 2 || kb < 4 * cut || nb / 8 < cut || nb > lin_max_nb(elem, true))) break;
         // clusters of 4 and 8 CTAs that take whole multiprocessors do not fill the processing clusters: 33 and 15 of them on 148
@@ -400,7 +447,8 @@ LinPlan lin_plan(const LinearArgs& a, int elem) {
 template <int MODE, int CG, int ACT, bool CUT>
 cudaError_t lin_launch(LinParams& p, cudaStream_t st) {
   const int raw = (128 + p.nb / CG) * 128, stage = raw * (MODE == LIN_F32 ? 2 : 1);
-  p.stages = std::min((kSmem - (int)sizeof(LinCtrl)) / stage, (int)kMaxStages);
+  const int out = p.bulk ? 128 * p.nb * 2 : 0;
+  p.stages = std::min((kSmem - ((int)sizeof(LinCtrl) + 127) / 128 * 128 - out) / stage, (int)kMaxStages);
   static bool configured[64] = {false};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
@@ -466,6 +514,10 @@ cudaError_t lin_type(const LinearArgs& all, const LinPlan& pl, cudaStream_t st) 
   while (1 << p.cut_log2 < pl.cut) ++p.cut_log2;
   p.r_tiles = (all.n + 128 * pl.cg - 1) / (128 * pl.cg);
   p.kb = (int)((all.K * (long long)sizeof(T) + 127) / 128);
+  // Whole tiles of 16-bit outputs through shared memory, where TMA can address them and the residual and the product is no shorter than a ring:
+  // with stores of 64 bytes per warp and a residual that a warp waits for, 8192 x 2048 x 16384 took 574 us.
+  p.bulk = sizeof(T) == 2 && pl.cut == 1 && p.kb >= 8 && make_plain_map(&p.y, all.Y, 2, all.n, all.N, all.ldy, 128, pl.nb) &&
+           (!all.R || make_plain_map(&p.r, all.R, 2, all.n, all.N, all.ldr, 128, pl.nb));
   if (!make_kmajor_map(&p.w, p.a.W, sizeof(T), all.K, all.n, p.a.ldw, 128) || !make_kmajor_map(&p.x, p.a.X, sizeof(T), all.K, all.N, p.a.ldx, pl.nb / pl.cg))
     return cudaErrorInvalidValue;
   return pl.cg == 2 ? lin_act<MODE, 2, false>(p, st) : pl.cut > 1 ? lin_act<MODE, 1, true>(p, st) : lin_act<MODE, 1, false>(p, st);

@@ -333,6 +333,16 @@ static bool encode_map(CUtensorMap* out, const void* base, int elem_bytes, int r
   return fn(out, dt, rank, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
+bool make_plain_map(CUtensorMap* out, const void* base, int elem_bytes, long long inner, long long outer, long long ld, int box_inner, int box_outer) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn || !base || ((uintptr_t)base & 15) != 0 || (ld * elem_bytes) % 16 != 0 || box_inner > 256 || box_outer > 256) return false;
+  const cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)outer};
+  const cuuint64_t strides[1] = {(cuuint64_t)(ld * elem_bytes)};
+  const cuuint32_t box[2] = {(cuuint32_t)box_inner, (cuuint32_t)box_outer}, estr[2] = {1, 1};
+  const CUtensorMapDataType dt = elem_bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
+  return fn(out, dt, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
 bool make_rows_map(CUtensorMap* out, const void* base, int elem_bytes, long long row_bytes, long long rows, int parts,
                    long long part_bytes, int kblocks, int box_rows, int box_kb) {
   const cuuint64_t dims[4] = {(cuuint64_t)(128 / elem_bytes), (cuuint64_t)rows, (cuuint64_t)parts, (cuuint64_t)kblocks};

@@ -52,6 +52,9 @@ int device_sms();
 bool make_kmajor_map(CUtensorMap* out, const void* base, int elem_bytes, long long k, long long rows, long long ld,
                      int box_rows);
 
+// 2-D map without swizzle: rows of `inner` elements, ld apart; a box lies in shared memory row after row
+bool make_plain_map(CUtensorMap* out, const void* base, int elem_bytes, long long inner, long long outer, long long ld, int box_inner, int box_outer);
+
 // round fp32 to the nearest value representable in tf32 (10 mantissa bits), ties away from zero on the bit pattern
 inline float tf32_round_host(float x) {
   unsigned u;
