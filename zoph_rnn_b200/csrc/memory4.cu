@@ -207,24 +207,26 @@ __global__ void __launch_bounds__(256) mem4_unpack_kernel(const Mem4Unpack a, in
 // covers the head and takes tiles of 32 slots, and a CTA has 16 / WT teams, each with slots of its own.  Per tile: the warps'
 // partial scores meet in shared memory, each warp finishes 16 / WT rows (a lane per slot: maximum, exponential, weights written as the
 // fragments of the second product), and all warps add weights x values to their registers.  Codes come three tiles ahead by
-// asynchronous copies.  What bounds it is the issue of instructions: turning 8 codes into 4 pairs of halves takes 13, twice per code.
+// asynchronous copies.  Many short heads (SOLO, one warp per team): each team has a column tile and head of its own, all of its slots, and
+// nothing to put together at the end; 481 x 16 heads of 32, one slot: 200 us with a CTA each.  What bounds it is the issue of instructions: turning 8 codes into 4 pairs of halves takes 13, twice per code.
 constexpr int kAttWarps = 16, kAttTile = 32, kAttStages = 3, kAttPartLd = 40;
-template <int PARTS, int WT, int NB>
+template <int PARTS, int WT, int NB, bool SOLO>
 struct AttShape {
-  static constexpr int TEAMS = kAttWarps / WT, GP = 2 * NB * WT;  // groups that the team's warps have room for
+  static constexpr int WARPS = SOLO ? 8 : kAttWarps, TEAMS = WARPS / WT, GP = 2 * NB * WT;  // groups that the team's warps have room for
   static constexpr int ROW = (GP | 1) * 16;                       // bytes of a slot's codes in shared memory: an odd number of 16 spreads them over the banks
   static constexpr int Q = GP * 2 * PARTS * 512;                  // Q as fragments
   static constexpr int STAGE = kAttTile * ROW + GP * kAttTile * 2;
   static constexpr int PART = WT * 16 * kAttPartLd * 4, W = 2 * PARTS * 512;
-  static constexpr int TEAM = kAttStages * STAGE + PART + W + 128;
+  static constexpr int TEAM = kAttStages * STAGE + PART + W + 192 + (SOLO ? Q : 0);
   static constexpr int OUT_LD = GP * 32 + 2;                      // floats; the teams' outputs take the place of all that
-  static constexpr int RUN = Q + TEAMS * TEAM, OUT = TEAMS * 16 * OUT_LD * 4;
-  static constexpr int ML = (RUN > OUT ? RUN : OUT), SMEM = ML + 3 * 16 * 16 * 4;
+  static constexpr int RUN = (SOLO ? 0 : Q) + TEAMS * TEAM, OUT = SOLO ? 0 : TEAMS * 16 * OUT_LD * 4;
+  static constexpr int ML = (RUN > OUT ? RUN : OUT), SMEM = ML + (SOLO ? 0 : 2 * 16 * 16 * 4);
   static_assert(SMEM <= 227 * 1024 && STAGE % 16 == 0 && TEAM % 16 == 0, "");
 };
 struct AttPlan {
   int G, warps, blocks;       // groups of a head; WT and NB
   int q_tiles, splits;
+  bool solo;
 };
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint4& a, uint32_t b0, uint32_t b1) {
@@ -257,41 +259,60 @@ __device__ __forceinline__ void copy16(void* dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(shared_at(dst)), "l"(src) : "memory");
 }
 
-template <class T, int WT, int NB>
-__global__ void __launch_bounds__(kAttWarps * 32, 1) mem4_attend_kernel(const Mem4Attend a, const AttPlan pl) {
+template <class T, int WT, int NB, bool SOLO>
+__global__ void __launch_bounds__((SOLO ? 8 : kAttWarps) * 32, SOLO && NB == 1 ? 2 : 1) mem4_attend_kernel(const Mem4Attend a, const AttPlan pl) {
   constexpr int PARTS = std::is_same<T, float>::value ? 2 : 1, ROWS = 16 / WT;
-  using Sh = AttShape<PARTS, WT, NB>;
+  using Sh = AttShape<PARTS, WT, NB, SOLO>;
+  static_assert(!SOLO || WT == 1, "");
   constexpr int TEAMS = Sh::TEAMS, GP = Sh::GP, ROW = Sh::ROW;
   extern __shared__ __align__(16) unsigned char smem[];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // (the combination waits for this launch's end before it reads anything)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, team = warp / WT, wt = warp % WT;
   const int g = lane >> 2, t = lane & 3, G = pl.G;
-  const int b = blockIdx.y / pl.q_tiles, c0 = blockIdx.y % pl.q_tiles * 16, h = blockIdx.z, split = blockIdx.x;
+  int b, c0, h, split = 0;
+  if constexpr (SOLO) {
+    const long long unit = (long long)blockIdx.x * TEAMS + team;
+    if (unit >= (long long)a.B * pl.q_tiles * a.heads) return;  // (teams of one warp: no barrier is missed)
+    h = (int)(unit % a.heads);
+    const int bq = (int)(unit / a.heads);
+    b = bq / pl.q_tiles;
+    c0 = (bq - b * pl.q_tiles) * 16;
+  } else {
+    b = blockIdx.y / pl.q_tiles;
+    c0 = (blockIdx.y - b * pl.q_tiles) * 16;
+    h = blockIdx.z;
+    split = blockIdx.x;
+  }
   const int n_cols = min(16, a.cols - c0);
-  unsigned char* s_q = smem;
-  unsigned char* s_team = smem + Sh::Q + team * Sh::TEAM;
+  unsigned char* s_team = smem + (SOLO ? 0 : Sh::Q) + team * Sh::TEAM;
+  unsigned char* s_q = SOLO ? s_team + Sh::TEAM - Sh::Q : smem;
   float* s_part = reinterpret_cast<float*>(s_team + kAttStages * Sh::STAGE);
   unsigned char* s_w = s_team + kAttStages * Sh::STAGE + Sh::PART;
   float* s_alpha = reinterpret_cast<float*>(s_w + Sh::W);
   float* s_m = s_alpha + 16;  // running maxima
-  float* s_ml = reinterpret_cast<float*>(smem + Sh::ML);  // [team][16]: maxima, sums; then [16]: factors of the queries
-  float* s_fac = s_ml + 2 * 16 * 16;
+  float* s_fac = s_m + 16;    // factors of the queries
+  float* s_ml = reinterpret_cast<float*>(smem + Sh::ML);  // [team][16]: maxima, sums
 
-  // Q of row `warp`, all of it requested at once
-  const bool in = warp < n_cols;
-  float qx[GP];
-  {
-    const T* q = static_cast<const T*>(a.q) + ((long long)b * a.cols + c0 + (in ? warp : 0)) * a.ld_q + (long long)h * a.d + lane;
+  // Q, a row per warp (of a team on its own, one row after the other), a row's elements requested at once
+  auto fetch_row = [&](int r, float (&x)[GP]) {
+    const bool in = r < n_cols;
+    const T* q = static_cast<const T*>(a.q) + ((long long)b * a.cols + c0 + (in ? r : 0)) * a.ld_q + (long long)h * a.d + lane;
 #pragma unroll
-    for (int k = 0; k < GP; ++k) qx[k] = in && k * 32 + lane < a.d ? to_f32(__ldg(q + k * 32)) : 0.f;
-  }
+    for (int k = 0; k < GP; ++k) x[k] = in && k * 32 + lane < a.d ? to_f32(__ldg(q + k * 32)) : 0.f;
+  };
+  const bool in = SOLO || warp < n_cols;
+  constexpr int ROWS_AT_ONCE = SOLO ? 4 : 1;
+  float qx[ROWS_AT_ONCE][GP];
+#pragma unroll
+  for (int r = 0; r < ROWS_AT_ONCE; ++r) fetch_row(SOLO ? r : warp, qx[r]);
   // the slots of this CTA: whole tiles of 32 from the window's first slot on
   const long long off = a.offset ? a.offset[b] : 0;
   const int lo = (int)max(off, 0ll), hi = (int)min(max(off + a.len[b], 0ll), (long long)a.S_cap);
   const int tiles = hi > lo ? (hi - lo + kAttTile - 1) / kAttTile : 0;
   const int share = pl.splits == 1 ? tiles : tiles / pl.splits, more = tiles - share * pl.splits;
   const int t0 = split * share + min(split, more), t1 = t0 + share + (split < more);
-  const int my = t1 - t0 > team ? (t1 - t0 - team + TEAMS - 1) / TEAMS : 0;  // tiles t0 + team, + TEAMS, ...
+  constexpr int STRIDE = SOLO ? 1 : TEAMS;
+  const int tile0 = t0 + (SOLO ? 0 : team), my = t1 > tile0 ? (t1 - tile0 + STRIDE - 1) / STRIDE : 0;  // tiles tile0, + STRIDE, ...
 
   // a thread copies chunk cq (16 bytes, one group) of the slots cp, cp + 8, .. + 24 of a tile (where the team has 128 threads per NB = 2; half
   // of that: eight slots), and their scales, which lie as [group][slot % 8][slot / 8]
@@ -305,7 +326,7 @@ __global__ void __launch_bounds__(kAttWarps * 32, 1) mem4_attend_kernel(const Me
   unsigned short sc_next[CPY];
   auto request = [&](int it) {
     if (it < my && copies) {
-      const int p0 = lo + (t0 + team + it * TEAMS) * kAttTile, n = hi - p0;
+      const int p0 = lo + (tile0 + it * STRIDE) * kAttTile, n = hi - p0;
       unsigned char* st = s_team + it % kAttStages * Sh::STAGE + cp * ROW + cq * 16;
       const uint8_t* from = codes + (size_t)p0 * row_codes;
       const unsigned short* sf = scales + (size_t)p0 * row_scales;
@@ -341,29 +362,48 @@ __global__ void __launch_bounds__(kAttWarps * 32, 1) mem4_attend_kernel(const Me
 
   // Q scaled by a power of two to at most 1; element e of a thread's word of 8 is half e / 4 of register 2 (e % 2) (+ 1: rows 8 .. 15) of k-step
   // (e % 4) / 2, so that a word of codes gives its fragments by masks alone
-  {
+  auto lay_out_row = [&](int r, const float (&x)[GP]) {
     unsigned m = 0;
 #pragma unroll
-    for (int k = 0; k < GP; ++k) m = max(m, __float_as_uint(qx[k]) & 0x7fffffffu);
+    for (int k = 0; k < GP; ++k) m = max(m, __float_as_uint(x[k]) & 0x7fffffffu);
     m = __reduce_max_sync(0xffffffffu, m);
     int e = 0;
     if (m != 0) frexpf(__uint_as_float(m), &e);
     const float down1 = ldexpf(1.f, -(e / 2)), down2 = ldexpf(1.f, -(e - e / 2));
     const int el = lane & 7, tt = lane >> 3;
     // (the fragments of odd k-steps have neighbouring rows exchanged: the two k-steps that a warp writes at once fall on different banks)
-    unsigned char* at = s_q + ((el & 3) / 2 * PARTS) * 512 + (((warp & 7) * 4 + tt) ^ ((el & 2) * 2)) * 16 + ((el & 1) * 2 + (warp >> 3)) * 4 + (el >> 2) * 2;
+    unsigned char* at = s_q + ((el & 3) / 2 * PARTS) * 512 + (((r & 7) * 4 + tt) ^ ((el & 2) * 2)) * 16 + ((el & 1) * 2 + (r >> 3)) * 4 + (el >> 2) * 2;
 #pragma unroll
     for (int k = 0; k < GP; ++k) {
       __half x0, x1;
-      split_half(qx[k] * down1 * down2, x0, x1);
+      split_half(x[k] * down1 * down2, x0, x1);
       *reinterpret_cast<__half*>(at + k * 2 * PARTS * 512) = x0;
       if (PARTS == 2) *reinterpret_cast<__half*>(at + k * 2 * PARTS * 512 + 512) = x1;
     }
-    if (lane == 0) s_fac[warp] = ldexpf(a.scale * 1.44269504f, e);  // (exponentials are powers of two)
+    const float fac = ldexpf(a.scale * 1.44269504f, e);  // (exponentials are powers of two)
+    if constexpr (SOLO) {
+      if (lane == 0) s_fac[r] = fac;
+    } else {  // every team has a copy
+      if (lane < TEAMS) s_fac[(lane - team) * (Sh::TEAM / 4) + r] = fac;
+    }
+  };
+  if constexpr (SOLO) {
+    for (int r0 = 0; r0 < 16; r0 += ROWS_AT_ONCE) {
+#pragma unroll
+      for (int r = 0; r < ROWS_AT_ONCE; ++r) lay_out_row(r0 + r, qx[r]);
+      if (r0 + ROWS_AT_ONCE < 16)
+#pragma unroll
+        for (int r = 0; r < ROWS_AT_ONCE; ++r) fetch_row(r0 + ROWS_AT_ONCE + r, qx[r]);
+    }
+  } else {
+    lay_out_row(warp, qx[0]);
   }
   keep_scales(0);
   request(1);
-  __syncthreads();
+  // rows without a column: weights 0, never rescaled
+  for (int i = tw; i < (Sh::W + 64) / 4; i += WT * 32) reinterpret_cast<unsigned*>(s_w)[i] = i < Sh::W / 4 ? 0u : 0x3f800000u;
+  if (SOLO) __syncwarp();
+  else __syncthreads();
 
   float acc[NB][8][4], l[4] = {0.f, 0.f, 0.f, 0.f};  // l: the weights' sums, as a product with ones (columns alike)
 #pragma unroll
@@ -381,7 +421,7 @@ __global__ void __launch_bounds__(kAttWarps * 32, 1) mem4_attend_kernel(const Me
     request(it + 2);
     const unsigned char* st = s_team + it % kAttStages * Sh::STAGE;
     const unsigned char* s_sc = st + kAttTile * ROW;
-    const int n = hi - (lo + (t0 + team + it * TEAMS) * kAttTile);
+    const int n = hi - (lo + (tile0 + it * STRIDE) * kAttTile);
     // scores of this warp's elements; n-tile j has slot 8 j + c in its column c
     {
       float z[PARTS][4][4];
@@ -427,6 +467,7 @@ __global__ void __launch_bounds__(kAttWarps * 32, 1) mem4_attend_kernel(const Me
 #pragma unroll
       for (int rr = 0; rr < ROWS; ++rr) {
         const int r = wt * ROWS + rr;
+        if (r >= n_cols) break;
         float z = 0.f;
 #pragma unroll
         for (int w = 0; w < WT; ++w) z += s_part[(w * 16 + r) * kAttPartLd + lane];
@@ -528,6 +569,35 @@ __global__ void __launch_bounds__(kAttWarps * 32, 1) mem4_attend_kernel(const Me
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
 
+  if constexpr (SOLO) {  // each lane has runs of 8 elements of two rows
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int r = g + 8 * half;
+      if (r >= n_cols) break;
+      const long long c = (long long)b * a.cols + c0 + r;
+      const float sum = l[2 * half], inv = sum != 0.f && (!a.mask || a.mask[c] != 0) ? 1.f / sum : 0.f;
+      const bool on = inv != 0.f;  // (a NaN is not 0)
+      T* o = static_cast<T*>(a.out) + c * a.ld_out + (long long)h * a.d;
+      const bool vec = ((uintptr_t)o & 15) == 0;
+#pragma unroll
+      for (int x = 0; x < NB; ++x)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int i = x * 64 + 8 * (2 * t + u);
+          float y[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) y[j] = on ? acc[x][j][2 * half + u] * inv : 0.f;
+          if (vec && i + 8 <= a.d) {
+            Mem4Vec<T>::store(o + i, y);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              if (i + j < a.d) o[i + j] = from_f32<T>(y[j]);
+          }
+        }
+    }
+    return;
+  }
   // the teams' maxima and sums, then their outputs side by side
   team_sync();
   if (wt == 0) {
@@ -693,20 +763,28 @@ AttPlan att_plan(int B, int cols, int S_cap, int heads, int d) {
   pl.q_tiles = (cols + 15) / 16;
   const long long units = (long long)B * pl.q_tiles * heads, most = S_cap / (kAttTile * 2 * (kAttWarps / pl.warps));
   pl.splits = (int)std::max<long long>(1, std::min<long long>(std::min<long long>(device_sms() / units, kMostSplits), most));
+  // a team on its own: as long as the tiles of all units take its multiprocessor no longer than the CTAs that a unit each would need (in tiles'
+  // times: two for the start and the end of a CTA)
+  const long long tiles = (S_cap + kAttTile - 1) / kAttTile, per_sm = pl.blocks == 1 ? 16 : 8, sms = device_sms();
+  const long long alone = (units + per_sm * sms - 1) / (per_sm * sms) * (2 + tiles), shared = (units + sms - 1) / sms * (2 + (tiles + 15) / 16);
+  pl.solo = pl.warps == 1 && pl.splits == 1 && alone <= shared;
   return pl;
 }
-template <class T, int WT, int NB>
+template <class T, int WT, int NB, bool SOLO>
 cudaError_t attend_launch(const Mem4Attend& a, const AttPlan& pl, cudaStream_t st) {
-  constexpr int smem = AttShape<std::is_same<T, float>::value ? 2 : 1, WT, NB>::SMEM;
+  using Sh = AttShape<std::is_same<T, float>::value ? 2 : 1, WT, NB, SOLO>;
+  constexpr int smem = Sh::SMEM;
   static bool configured[64] = {false};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
   if (!configured[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(mem4_attend_kernel<T, WT, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    const cudaError_t e = cudaFuncSetAttribute(mem4_attend_kernel<T, WT, NB, SOLO>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     configured[dev] = true;
   }
-  mem4_attend_kernel<T, WT, NB><<<dim3(pl.splits, (unsigned)(a.B * pl.q_tiles), (unsigned)a.heads), kAttWarps * 32, smem, st>>>(a, pl);
+  const long long units = (long long)a.B * pl.q_tiles * a.heads;
+  const dim3 grid = SOLO ? dim3((unsigned)((units + Sh::TEAMS - 1) / Sh::TEAMS)) : dim3(pl.splits, (unsigned)(a.B * pl.q_tiles), (unsigned)a.heads);
+  mem4_attend_kernel<T, WT, NB, SOLO><<<grid, Sh::WARPS * 32, smem, st>>>(a, pl);
   return cudaGetLastError();
 }
 template <class T>
@@ -727,9 +805,11 @@ cudaError_t attend_type(const Mem4Attend& all, cudaStream_t st) {
     a.q = static_cast<const T*>(a.q) + cols * a.ld_q;
     a.out = static_cast<T*>(a.out) + cols * a.ld_out;
     count_launch();
-    const cudaError_t e = pl.blocks == 1 ? attend_launch<T, 1, 1>(a, pl, st) : pl.warps == 1 ? attend_launch<T, 1, 2>(a, pl, st)
-                          : pl.warps == 2 ? attend_launch<T, 2, 2>(a, pl, st) : pl.warps == 4 ? attend_launch<T, 4, 2>(a, pl, st)
-                                                                                             : attend_launch<T, 8, 2>(a, pl, st);
+    const cudaError_t e = pl.blocks == 1   ? (pl.solo ? attend_launch<T, 1, 1, true>(a, pl, st) : attend_launch<T, 1, 1, false>(a, pl, st))
+                          : pl.warps == 1 ? (pl.solo ? attend_launch<T, 1, 2, true>(a, pl, st) : attend_launch<T, 1, 2, false>(a, pl, st))
+                          : pl.warps == 2 ? attend_launch<T, 2, 2, false>(a, pl, st)
+                          : pl.warps == 4 ? attend_launch<T, 4, 2, false>(a, pl, st)
+                                          : attend_launch<T, 8, 2, false>(a, pl, st);
     if (e != cudaSuccess) return e;
     if (pl.splits == 1) continue;
     cudaLaunchConfig_t cfg;
