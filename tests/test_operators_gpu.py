@@ -153,6 +153,17 @@ def test_attend(api, dtype, B, cols, S, heads, d):
     attend_case(api, dtype, B, cols, S, heads, d, lens, [S - n for n in lens], seed=d + S)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("B, cols, S, heads, d", [(130, 3, 40, 8, 64), (99, 1, 33, 16, 32), (60, 17, 5, 12, 100), (300, 12, 1, 4, 33), (41, 9, 70, 30, 128), (700, 2, 32, 1, 20)])
+def test_attend_with_many_short_heads(api, dtype, B, cols, S, heads, d):
+    """More column tiles and heads than multiprocessors: a warp each."""
+    rng = np.random.default_rng(d)
+    lens = rng.integers(0, S + 1, B).tolist()
+    offs = [int(rng.integers(0, S - n + 1)) for n in lens]
+    mask = (rng.random(B * cols) < 0.9).astype(np.int32).tolist()
+    attend_case(api, dtype, B, cols, S, heads, d, lens, offs, seed=d, mask=mask)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "f16"])
 @pytest.mark.parametrize("heads, d", [(1, 1000), (4, 64)])
 def test_attend_lengths_and_masks(api, dtype, heads, d):
@@ -264,7 +275,7 @@ def linear_case(api, dtype, n, K, N, act="none", bias=True, residual=False, pad=
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("n, K, N", [
     (1, 1, 1), (3, 5, 2), (64, 64, 1), (1000, 2000, 12), (1000, 2000, 5), (129, 257, 16), (200, 1000, 17), (500, 96, 33), (256, 512, 64), (300, 40, 65), (1000, 1000, 100),
-    (1000, 2000, 768), (333, 777, 200), (777, 1024, 129), (2048, 320, 300), (130, 4096, 257), (37, 1173, 1), (4100, 64, 513), (515, 8, 1000), (8, 515, 1000)])
+    (1000, 2000, 768), (333, 777, 200), (777, 1024, 129), (2048, 320, 300), (130, 4096, 257), (37, 1173, 1), (4100, 64, 513), (515, 8, 1000), (8, 515, 1000), (245, 7428, 3), (40, 16384, 16), (100, 9001, 30), (512, 8192, 512), (1000, 2000, 64)])
 def test_linear(api, dtype, n, K, N):
     linear_case(api, dtype, n, K, N, seed=n + K)
 

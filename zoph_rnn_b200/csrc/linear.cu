@@ -431,8 +431,9 @@ LinPlan lin_plan(const LinearArgs& a, int elem) {
   // tiles of 8, 16 and 32 columns).  Up to 8 columns it is ahead, up to 32 with few weights or rows that would have to be moved first.
   static const double lat[2][3] = {{300, 460, 550}, {270, 460, 840}}, thr[2][3] = {{232, 390, 520}, {154, 230, 380}};
   const int t = a.N <= 8 ? 0 : a.N <= 16 ? 1 : 2, cols = 8 << t;
-  const double ctas = (double)((a.n + 15) / 16) * ((a.N + cols - 1) / cols), chunks = (((long long)a.K * eb + 63) / 64 + 7) / 8;
-  pl.few = 4000 + chunks * std::max(lat[!f32][t], thr[!f32][t] * ctas / sms) <= best;
+  const int shared = few_cut(a.n, a.N, a.K, eb);
+  const double ctas = (double)((a.n + 15) / 16) * ((a.N + cols - 1) / cols) * shared, chunks = (((long long)a.K * eb + 63) / 64 + 8 * shared - 1) / (8 * shared);
+  pl.few = 4000 + (shared > 1 ? 1500 : 0) + chunks * std::max(lat[!f32][t], thr[!f32][t] * ctas / sms) <= best;
   if (pl.few) {
     pl.align_w = pl.align_x = false;
     return pl;

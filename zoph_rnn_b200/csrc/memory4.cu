@@ -131,29 +131,44 @@ template <class T> struct Mem4Vec {
 
 // A lane takes 8 elements, four lanes a group, a team of lanes one source column, whose slots it walks through: all indices are computed once
 // per thread (divided per vector, they were two thirds of the instructions).  ALIGNED: vectors lie on 16 bytes and a head is a
-// multiple of 8 elements.
+// multiple of 8 elements; else a warp's eight groups, all of one vector, go through shared memory, 32 consecutive elements at a time.
+constexpr int kMem4Stage = 8 * 36;  // floats of a warp's groups, four more per group: runs of 8 fall on different banks
 template <class T, bool ALIGNED>
 __global__ void __launch_bounds__(256) mem4_pack_kernel(const Mem4Pack a, int team) {
+  __shared__ __align__(16) float s_stage[ALIGNED ? 1 : 8 * kMem4Stage];
   const int G = mem4_groups(a.d), lane = threadIdx.x % team, sub = threadIdx.x / team, q = blockIdx.z * team + lane, quads = a.heads * G * 4;
   const long long b = (long long)blockIdx.x * (256 / team) + sub;
-  if (sub >= 256 / team || b >= a.B || q >= quads) return;  // (whole groups of four leave)
+  const bool mine = q < quads;
+  if (sub >= 256 / team || b >= a.B || (ALIGNED && !mine)) return;  // (whole groups of four leave; unaligned: whole warps)
   const int g = q >> 2, h = g / G, i = (q - h * G * 4) * 8;
-  const T* x = static_cast<const T*>(a.x) + b * a.ld_col + (long long)h * a.d + i + blockIdx.y * a.ld_slot;
+  const T* row_x = static_cast<const T*>(a.x) + b * a.ld_col + blockIdx.y * a.ld_slot;
   const long long row = (long long)a.heads * G, to = (b * a.S_cap + a.slot0 + blockIdx.y) * row + g;
   unsigned* codes = reinterpret_cast<unsigned*>(a.codes) + to * 4 + (q & 3);
   __half* scales = a.scales + to;
   const unsigned four = 0xfu << (threadIdx.x & 28);
   const long long x_step = gridDim.y * a.ld_slot, step = gridDim.y * row;
+  float* stage = s_stage + (ALIGNED ? 0 : (threadIdx.x >> 5) * kMem4Stage);
+  const int l32 = threadIdx.x & 31, g0 = (blockIdx.z * team + (lane & ~31)) >> 2;  // the warp's first group
 #pragma unroll 2
-  for (int s = blockIdx.y; s < a.S; s += gridDim.y, x += x_step, codes += step * 4, scales += step) {
+  for (int s = blockIdx.y; s < a.S; s += gridDim.y, row_x += x_step, codes += step * 4, scales += step) {
     float v[8];
     if (ALIGNED) {
 #pragma unroll
       for (int u = 0; u < 8; ++u) v[u] = 0.f;
-      if (i < a.d) Mem4Vec<T>::load(x, v);
+      if (i < a.d) Mem4Vec<T>::load(row_x + (long long)h * a.d + i, v);
     } else {
+      float x[8];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) v[u] = i + u < a.d ? to_f32(__ldg(x + u)) : 0.f;
+      for (int u = 0; u < 8; ++u) {
+        const int gu = g0 + u, hu = a.heads == 1 ? 0 : gu / G, e = (gu - hu * G) * 32 + l32;
+        x[u] = hu < a.heads && e < a.d ? to_f32(__ldg(row_x + (long long)hu * a.d + e)) : 0.f;
+      }
+      __syncwarp();
+#pragma unroll
+      for (int u = 0; u < 8; ++u) stage[u * 36 + l32] = x[u];
+      __syncwarp();
+      const float4 lo = *reinterpret_cast<const float4*>(stage + (l32 >> 2) * 36 + (l32 & 3) * 8), hi = *reinterpret_cast<const float4*>(stage + (l32 >> 2) * 36 + (l32 & 3) * 8 + 4);
+      v[0] = lo.x; v[1] = lo.y; v[2] = lo.z; v[3] = lo.w; v[4] = hi.x; v[5] = hi.y; v[6] = hi.z; v[7] = hi.w;
     }
     float m = fabsf(v[0]);
 #pragma unroll
@@ -162,25 +177,32 @@ __global__ void __launch_bounds__(256) mem4_pack_kernel(const Mem4Pack a, int te
     m = max_nan(m, __shfl_xor_sync(four, m, 2));
     const __half sh = mem4_scale(m);
     const float sc = __half2float(sh);
-    *codes = sc > 0.f ? mem4_codes(v, sc) : 0x88888888u;
-    if ((q & 3) == 0) *scales = sh;
+    const unsigned w = sc > 0.f ? mem4_codes(v, sc) : 0x88888888u;
+    if (ALIGNED || mine) {
+      *codes = w;
+      if ((q & 3) == 0) *scales = sh;
+    }
   }
 }
 template <class T, bool ALIGNED>
 __global__ void __launch_bounds__(256) mem4_unpack_kernel(const Mem4Unpack a, int team) {
+  __shared__ __align__(16) float s_stage[ALIGNED ? 1 : 8 * kMem4Stage];
   const int G = mem4_groups(a.d), lane = threadIdx.x % team, sub = threadIdx.x / team, q = blockIdx.z * team + lane, quads = a.heads * G * 4;
   const long long b = (long long)blockIdx.x * (256 / team) + sub;
+  const bool mine = q < quads;
   const int g = q >> 2, h = g / G, i = (q - h * G * 4) * 8;
-  if (sub >= 256 / team || b >= a.B || q >= quads || i >= a.d) return;
+  if (sub >= 256 / team || b >= a.B || (ALIGNED && (!mine || i >= a.d))) return;
   const long long row = (long long)a.heads * G, from = (b * a.S_cap + a.slot0 + blockIdx.y) * row + g, width = (long long)a.heads * a.d;
   const unsigned* codes = reinterpret_cast<const unsigned*>(a.codes) + from * 4 + (q & 3);
   const __half* scales = a.scales + from;
-  T* out = static_cast<T*>(a.out) + (b * a.S + blockIdx.y) * width + (long long)h * a.d + i;
+  T* row_out = static_cast<T*>(a.out) + (b * a.S + blockIdx.y) * width;
   const long long step = gridDim.y * row;
+  float* stage = s_stage + (ALIGNED ? 0 : (threadIdx.x >> 5) * kMem4Stage);
+  const int l32 = threadIdx.x & 31, g0 = (blockIdx.z * team + (lane & ~31)) >> 2;
 #pragma unroll 4
-  for (int s = blockIdx.y; s < a.S; s += gridDim.y, codes += step * 4, scales += step, out += gridDim.y * width) {
-    uint32_t p[4];  // (elements 0, 4), (1, 5), (2, 6), (3, 7)
-    dequant4(__ldg(codes), __half2half2(__ldg(scales)), p);
+  for (int s = blockIdx.y; s < a.S; s += gridDim.y, codes += step * 4, scales += step, row_out += gridDim.y * width) {
+    uint32_t p[4] = {0u, 0u, 0u, 0u};  // (elements 0, 4), (1, 5), (2, 6), (3, 7)
+    if (ALIGNED || mine) dequant4(__ldg(codes), __half2half2(__ldg(scales)), p);
     float v[8];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
@@ -189,11 +211,18 @@ __global__ void __launch_bounds__(256) mem4_unpack_kernel(const Mem4Unpack a, in
       v[u + 4] = f.y;
     }
     if (ALIGNED) {
-      Mem4Vec<T>::store(out, v);
+      Mem4Vec<T>::store(row_out + (long long)h * a.d + i, v);
     } else {
+      __syncwarp();
+      float4* at = reinterpret_cast<float4*>(stage + (l32 >> 2) * 36 + (l32 & 3) * 8);
+      at[0] = make_float4(v[0], v[1], v[2], v[3]);
+      at[1] = make_float4(v[4], v[5], v[6], v[7]);
+      __syncwarp();
 #pragma unroll
-      for (int u = 0; u < 8; ++u)
-        if (i + u < a.d) out[u] = from_f32<T>(v[u]);
+      for (int u = 0; u < 8; ++u) {
+        const int gu = g0 + u, hu = a.heads == 1 ? 0 : gu / G, e = (gu - hu * G) * 32 + l32;
+        if (hu < a.heads && e < a.d) row_out[(long long)hu * a.d + e] = from_f32<T>(stage[u * 36 + l32]);
+      }
     }
   }
 }
@@ -715,9 +744,9 @@ __global__ void __launch_bounds__(256) mem4_combine_kernel(const Mem4Attend a, c
 namespace {
 
 // Teams of as many lanes as a vector has (256 at most, then several CTAs share it); CTAs along the slots: eight per multiprocessor in all
-dim3 mem4_grid(int B, int S, int heads, int d, int* team) {
+dim3 mem4_grid(int B, int S, int heads, int d, bool aligned, int* team) {
   const int quads = heads * mem4_groups(d) * 4;
-  *team = std::min(quads, 256);
+  *team = std::min(aligned ? quads : (quads + 31) / 32 * 32, 256);  // (unaligned: whole warps)
   const long long x = (B + 256 / *team - 1) / (256 / *team), z = (quads + *team - 1) / *team;
   const long long y = std::max<long long>(1, std::min<long long>(S, (16ll * device_sms() + x * z - 1) / (x * z)));
   return dim3((unsigned)x, (unsigned)std::min<long long>(y, 65535), (unsigned)z);
@@ -725,8 +754,8 @@ dim3 mem4_grid(int B, int S, int heads, int d, int* team) {
 template <class T>
 cudaError_t pack_type(const Mem4Pack& a, cudaStream_t st) {
   int team;
-  const dim3 grid = mem4_grid(a.B, a.S, a.heads, a.d, &team);
   const bool aligned = ((uintptr_t)a.x & 15) == 0 && a.ld_slot * sizeof(T) % 16 == 0 && a.ld_col * sizeof(T) % 16 == 0 && a.d % 8 == 0;
+  const dim3 grid = mem4_grid(a.B, a.S, a.heads, a.d, aligned, &team);
   if (aligned) mem4_pack_kernel<T, true><<<grid, 256, 0, st>>>(a, team);
   else mem4_pack_kernel<T, false><<<grid, 256, 0, st>>>(a, team);
   return cudaGetLastError();
@@ -734,8 +763,9 @@ cudaError_t pack_type(const Mem4Pack& a, cudaStream_t st) {
 template <class T>
 cudaError_t unpack_type(const Mem4Unpack& a, cudaStream_t st) {
   int team;
-  const dim3 grid = mem4_grid(a.B, a.S, a.heads, a.d, &team);
-  if (((uintptr_t)a.out & 15) == 0 && a.d % 8 == 0) mem4_unpack_kernel<T, true><<<grid, 256, 0, st>>>(a, team);
+  const bool aligned = ((uintptr_t)a.out & 15) == 0 && a.d % 8 == 0;
+  const dim3 grid = mem4_grid(a.B, a.S, a.heads, a.d, aligned, &team);
+  if (aligned) mem4_unpack_kernel<T, true><<<grid, 256, 0, st>>>(a, team);
   else mem4_unpack_kernel<T, false><<<grid, 256, 0, st>>>(a, team);
   return cudaGetLastError();
 }

@@ -80,6 +80,7 @@ struct LinearArgs {
 size_t linear_work(const LinearArgs& a, int elem);
 cudaError_t launch_linear(const LinearArgs& a, int elem, cudaStream_t st);
 cudaError_t launch_linear_few(const LinearArgs& a, int elem, cudaStream_t st);  // few columns (linear_few.cu)
+int few_cut(int n, int N, int K, int eb);  // ... and how many CTAs share the K axis there
 
 // ---- selection over beams and vocabulary
 constexpr int kSelectMax = 64;  // survivors of a sentence
