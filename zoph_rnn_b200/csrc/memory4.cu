@@ -493,26 +493,33 @@ __global__ void __launch_bounds__((SOLO ? 8 : kAttWarps) * 32, SOLO && NB == 1 ?
     // c / 2 (of a row's four), k-step c % 2, so that a thread's four scales lie side by side
     {
       unsigned char* at0 = s_w + (lane & 1) * PARTS * 512 + (lane & 7) / 2 * 16 + (lane >> 4) * 8 + (lane >> 3 & 1) * 2;
+      constexpr int RC = ROWS < 4 ? ROWS : 4;  // rows side by side: one's latency is another's work
+      for (int r0 = wt * ROWS; r0 < (wt + 1) * ROWS && r0 < n_cols; r0 += RC) {
+        float z[RC], m_old[RC];
 #pragma unroll
-      for (int rr = 0; rr < ROWS; ++rr) {
-        const int r = wt * ROWS + rr;
-        if (r >= n_cols) break;
-        float z = 0.f;
+        for (int rr = 0; rr < RC; ++rr) {
+          z[rr] = 0.f;
 #pragma unroll
-        for (int w = 0; w < WT; ++w) z += s_part[(w * 16 + r) * kAttPartLd + lane];
-        z = lane < n ? z * s_fac[r] : -INFINITY;
-        const float m_old = s_m[r], m_new = fmaxf(m_old, warp_max(z)), ref = m_new == -INFINITY ? 0.f : m_new;
-        const float alpha = exp2_approx(m_old - ref), p = exp2_approx(z - ref);
-        __syncwarp();
-        if (lane == 0) {
-          s_alpha[r] = alpha;
-          s_m[r] = m_new;
+          for (int w = 0; w < WT; ++w) z[rr] += s_part[(w * 16 + r0 + rr) * kAttPartLd + lane];
+          z[rr] = lane < n ? z[rr] * s_fac[r0 + rr] : -INFINITY;
+          m_old[rr] = s_m[r0 + rr];
         }
-        __half p0h, p1h;
-        split_half(p, p0h, p1h);
-        unsigned char* at = at0 + (r & 7) * 64 + (r >> 3) * 4;
-        *reinterpret_cast<__half*>(at) = p0h;
-        if (PARTS == 2) *reinterpret_cast<__half*>(at + 512) = p1h;
+        __syncwarp();
+#pragma unroll
+        for (int rr = 0; rr < RC; ++rr) {
+          const int r = r0 + rr;
+          const float m_new = fmaxf(m_old[rr], warp_max(z[rr])), ref = m_new == -INFINITY ? 0.f : m_new;
+          const float alpha = exp2_approx(m_old[rr] - ref), p = exp2_approx(z[rr] - ref);
+          if (lane == 0) {
+            s_alpha[r] = alpha;
+            s_m[r] = m_new;
+          }
+          __half p0h, p1h;
+          split_half(p, p0h, p1h);
+          unsigned char* at = at0 + (r & 7) * 64 + (r >> 3) * 4;
+          *reinterpret_cast<__half*>(at) = p0h;
+          if (PARTS == 2) *reinterpret_cast<__half*>(at + 512) = p1h;
+        }
       }
     }
     team_sync();
@@ -695,7 +702,8 @@ __global__ void __launch_bounds__(256) mem4_combine_kernel(const Mem4Attend a, c
   __shared__ float s_f[kMostSplits], s_red[8];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int tid = threadIdx.x, h = blockIdx.y, dp = pl.G * 32;
-  const long long c = blockIdx.x, b = c / a.cols;
+  const int pieces = (a.d + 255) / 256;  // of 256 elements, a CTA each
+  const long long c = blockIdx.x / pieces, b = c / a.cols;
   const int at = (int)(c - b * a.cols);
   const float* w = a.work + ((b * pl.q_tiles + at / 16) * a.heads + h) * pl.splits * 16 * (dp + 2) + (at % 16) * (dp + 2);
   const long long step = 16ll * (dp + 2);
@@ -728,9 +736,10 @@ __global__ void __launch_bounds__(256) mem4_combine_kernel(const Mem4Attend a, c
   // (l is 0 only where no part had a slot: a NaN among the weights is one here, too)
   const bool on = l != 0.f && (!a.mask || a.mask[c] != 0);
   T* out = static_cast<T*>(a.out) + c * a.ld_out + (long long)h * a.d;
-  for (int i = tid; i < a.d; i += 256) {
+  const int i = (int)(blockIdx.x - c * pieces) * 256 + tid;
+  if (i < a.d) {
     float y = 0.f;
-#pragma unroll 4
+#pragma unroll 8
     for (int s = 0; s < pl.splits; ++s) {
       const float x = __ldcg(w + s * step + 2 + i), f = s_f[s];
       y = f != 0.f ? fmaf(x, f, y) : y;
@@ -844,7 +853,7 @@ cudaError_t attend_type(const Mem4Attend& all, cudaStream_t st) {
     if (pl.splits == 1) continue;
     cudaLaunchConfig_t cfg;
     std::memset(&cfg, 0, sizeof(cfg));
-    cfg.gridDim = dim3((unsigned)(a.B * a.cols), a.heads);
+    cfg.gridDim = dim3((unsigned)((long long)a.B * a.cols * ((a.d + 255) / 256)), a.heads);
     cfg.blockDim = dim3(256);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
