@@ -140,6 +140,11 @@ int zrnn_att_load(zrnn_attention* att, const float* const* h_tensors, int n_tens
  * replaces the per-beam replication of src/model.hpp:2434-2445). */
 int zrnn_att_set_source(zrnn_attention* att, const float* d_hs, int S_max, int B_src, const int* d_len,
                         const int* d_offset, int cols_per_sentence);
+/* The same with the source states held in 4 bits (zrnn_memory4_pack with heads = 1, d = H <= 1024, below): S_max slots per source column, lengths
+ * and offsets as above.  Global dot attention only; zrnn_att_forward then takes whole sentences (B a multiple of
+ * cols_per_sentence) and keeps no alignments. */
+int zrnn_att_set_source_memory4(zrnn_attention* att, const void* d_codes, const void* d_scales, int S_max, int B_src,
+                                const int* d_len, const int* d_offset, int cols_per_sentence);
 /* attention_node::forward_prop (src/attention_node.hpp:73-394).  d_align_out (optional): local-p
  * (2D+1) x B weights stored [j*B+b]; global S_max x B stored [s*B+b] in source-position order. */
 int zrnn_att_forward(zrnn_attention* att, const float* d_h_t, const int* d_mask01, int B, float* d_htild_out,

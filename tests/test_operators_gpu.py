@@ -592,3 +592,129 @@ def test_the_calls_allocate_nothing(api):
         s.run(mem)
     torch.cuda.synchronize()
     assert torch.cuda.mem_get_info()[0] >= before
+
+
+@pytest.mark.parametrize("dtype", [3, 0, 1, 4])  # exact fp32, fp16 split, bf16, 3xTF32
+@pytest.mark.parametrize("H, S, B, cols", [(64, 20, 3, 1), (320, 50, 5, 12), (1000, 33, 2, 4)])
+def test_attention_layer_over_a_source_in_4_bits(api, dtype, H, S, B, cols):
+    """The layer gives what it gives over the same numbers in 32 bits: the two contexts differ by roundings of 32 bits (sums over S and H
+    products), which the combiner's sum of 2 H products and tanh pass on; with bf16 operands a rounding may fall to the other side."""
+    g = gen(H)
+    rng = np.random.default_rng(H)
+    att = api.attention_layer(H, 10, att_type=api.ATT_GLOBAL_DOT, dtype=dtype)
+    w = [rng.uniform(-0.1, 0.1, n).astype(np.float32) for n in (H * H, H * H, H, H, H * H, H * H)]
+    att.load_weights(w)
+    hs = torch.tanh(0.5 * torch.randn(S, B, H, generator=g, device="cuda"))
+    lens = torch.tensor([S, S // 2, 3, 1, S - 1][:B], dtype=torch.int32, device="cuda")
+    offs = S - lens
+    m = api.memory4(B, S, H).pack(hs)
+    values = m.unpack().view(B, S, H).permute(1, 0, 2).contiguous()
+    h = torch.tanh(0.3 * torch.randn(B * cols, H, generator=g, device="cuda")).view(-1)
+    mask = torch.ones(B * cols, dtype=torch.int32, device="cuda")
+    mask[-1] = 0
+    att.prep_minibatch_info(values.view(-1), S, B, lens, offs, cols_per_sentence=cols)
+    want = att.forward_prop(h, mask)
+    att.prep_minibatch_memory4(m, lens, offs, cols_per_sentence=cols)
+    got = att.forward_prop(h, mask)
+    # the context's error times the row sums of |W_c1| (0.05 H), and for bf16 a step of 2^-8 of a context of up to 1 with random signs
+    tol = 0.05 * H * 2 * sum_tol(H) if dtype != 1 else 0.06 * H ** 0.5 * 2.0 ** -8 + 2.0 ** -10
+    assert float((got - want).abs().max()) <= tol
+    assert got.view(B * cols, H)[-1].eq(0).all()
+    with pytest.raises(api.ZrnnError):
+        att.forward_prop(h, mask, want_alignments=True)
+    with pytest.raises(api.ZrnnError):
+        att.forward_prop_viterbi(h, mask)
+    if cols > 1:
+        with pytest.raises(api.ZrnnError):
+            att.forward_prop(h[: (cols + 1) * H].contiguous(), mask[: cols + 1].contiguous())
+    att.prep_minibatch_info(values.view(-1), S, B, lens, offs, cols_per_sentence=cols)
+    assert torch.equal(att.forward_prop(h, mask), want)
+    local = api.attention_layer(H, 10, att_type=api.ATT_LOCAL_P, dtype=dtype)
+    with pytest.raises(api.ZrnnError):
+        local.prep_minibatch_memory4(m, lens, offs)
+
+
+def test_the_first_calls_of_a_process_may_be_captured():
+    """Nothing is set up by a call that a capture would not allow."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import torch
+from zoph_rnn_b200 import api
+torch.manual_seed(0)
+r = lambda *s: torch.randn(*s, device="cuda")
+hs, q, lens = torch.tanh(r(700, 2, 64)), r(6, 64), torch.tensor([700, 20], dtype=torch.int32, device="cuda")
+W, X, X2, z, sc = r(300, 700), r(200, 700), r(3, 700), r(8, 40000), r(8)
+m = api.memory4(2, 700, 64)
+torch.cuda.synchronize()
+def step():
+    m.pack(hs)
+    a = m.attend(q, lens)
+    v, w, p = api.beam_select(z, sc, 4, 4)
+    s, = api.beam_reorder([z], p)
+    return a, api.linear(W, X, act="gelu"), api.linear(W, X2), api.linear(W.half(), X.half()), v, w, p, s
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    out = step()
+g.replay()
+torch.cuda.synchronize()
+for a, b in zip(out, step()):
+    assert torch.equal(a, b)
+assert api.lib().zrnn_tc_error() == 0
+print("captured")
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    p = subprocess.run([sys.executable, "-c", code], cwd=root, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, timeout=300)
+    assert p.returncode == 0 and "captured" in p.stdout, p.stdout
+
+
+def test_several_threads_at_once(api):
+    """The calls have no handle: threads call them side by side, each on its stream."""
+    import threading
+    s = [Step(api, n=2, beam=4 + i, H=64 * (i + 1), V=700 + i, dtype=d) for i, d in enumerate(("f32", "bf16", "f16", "f32"))]
+    mem = [api.memory4(x.n, 37, x.H).pack(x.hs) for x in s]
+    want = [x.run(m) for x, m in zip(s, mem)]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        st = torch.cuda.Stream()
+        with torch.cuda.stream(st):
+            for _ in range(20):
+                got = s[i].run(mem[i])
+                st.synchronize()
+                if not all(torch.equal(a, b) for a, b in zip(got, want[i])):
+                    bad.append(i)
+    ts = [threading.Thread(target=work, args=(i,)) for i in range(len(s))]
+    [t.start() for t in ts]
+    [t.join() for t in ts]
+    assert not bad
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("n, K, N", [(520, 1024, 300), (1000, 520, 2000), (4100, 640, 5000)])
+def test_linear_long_products_with_a_residual(api, dtype, n, K, N):
+    """Several tiles per CTA, tiles that end in the middle, outputs as whole tiles and (odd rows) by stores; in place, too."""
+    linear_case(api, dtype, n, K, N, "gelu", residual=True, seed=5)
+    linear_case(api, dtype, n, K, N, "none", residual=True, inplace=True, seed=6)
+    linear_case(api, dtype, n, K, N, "silu", residual=True, pad=(8, 16, 24, 8), seed=7)
+    linear_case(api, dtype, n, K, N, "relu", residual=True, pad=(0, 0, 1, 3), seed=8)
+
+
+def test_many_sentences(api):
+    """More sentences than a grid's dimension holds."""
+    g = gen(40)
+    z = randn(g, 70000, 9)
+    select_case(api, z, randn(g, 70000), 1, 3)
+    x = randn(g, 140000, 3)
+    p = torch.arange(140000, device="cuda", dtype=torch.int32).flip(0).contiguous()
+    out, = api.beam_reorder([x], p)
+    assert torch.equal(out, x.flip(0))
+    hs, q = torch.tanh(randn(g, 2, 70000, 32)), randn(g, 70000, 32)
+    m = api.memory4(70000, 2, 32).pack(hs)
+    lens = torch.randint(0, 3, (70000,), generator=g, device="cuda", dtype=torch.int32)
+    out = m.attend(q, lens)
+    at = [0, 1, 65534, 65535, 65536, 69999]
+    v = f64(m.unpack())[at]
+    check_attend(out[at], v, f64(q)[at], lens.cpu().numpy()[at], [0] * 6, 1.0, "f32")

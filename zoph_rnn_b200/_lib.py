@@ -66,6 +66,8 @@ SIGNATURES = {
     "zrnn_att_load": (ctypes.c_int, [c_void_p, ctypes.POINTER(c_float_p), ctypes.c_int]),
     "zrnn_att_set_source": (ctypes.c_int, [c_void_p, c_void_p, ctypes.c_int, ctypes.c_int, c_void_p, c_void_p,
                                            ctypes.c_int]),
+    "zrnn_att_set_source_memory4": (ctypes.c_int, [c_void_p, c_void_p, c_void_p, ctypes.c_int, ctypes.c_int, c_void_p, c_void_p,
+                                                   ctypes.c_int]),
     "zrnn_att_forward": (ctypes.c_int, [c_void_p, c_void_p, c_void_p, ctypes.c_int, c_void_p, c_void_p, c_void_p]),
     "zrnn_att_forward_viterbi": (ctypes.c_int, [c_void_p, c_void_p, c_void_p, ctypes.c_int, c_void_p, c_void_p,
                                                 c_void_p]),

@@ -132,6 +132,17 @@ class attention_layer:
         self.S_max = S_max
         check(lib().zrnn_att_set_source(self._h, _ptr(hs), S_max, B_src, _ptr(lens), _ptr(offsets), cols_per_sentence))
 
+    def prep_minibatch_memory4(self, memory, lens, offsets, cols_per_sentence=1):
+        """prep_minibatch_info with the source states in 4 bits: memory is a memory4 of heads = 1, d = H (global dot attention only)."""
+        if memory.heads != 1 or memory.d != self.H:
+            raise ValueError("prep_minibatch_memory4: a memory4 of one head of H elements")
+        _dense(lens, "prep_minibatch_memory4: lens", torch.int32, (memory.B,))
+        _dense(offsets, "prep_minibatch_memory4: offsets", torch.int32, (memory.B,))
+        self._keep = (memory, lens, offsets)
+        self.S_max = memory.S_max
+        check(lib().zrnn_att_set_source_memory4(self._h, _ptr(memory.codes), _ptr(memory.scales), memory.S_max, memory.B, _ptr(lens),
+                                                _ptr(offsets), cols_per_sentence))
+
     def forward_prop(self, h_t, mask01, want_alignments=False):
         """attention_node::forward_prop (src/attention_node.hpp:73-394)."""
         B = h_t.numel() // self.H

@@ -6,11 +6,13 @@
 #include <nccl.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
 #include <functional>
+#include <mutex>
 #include <set>
 #include <string>
 #include <vector>
@@ -301,6 +303,9 @@ struct zrnn_attention {
   int S_max = 0, B_src = 0, cols_per_sent = 1;
   const int* len = nullptr;
   const int* off = nullptr;
+  const void* m4_codes = nullptr;  // the source states in 4 bits instead of hs
+  const void* m4_scales = nullptr;
+  DevBuf m4_work;
   DevBuf tq, ctx;
   int Kpad = 0, BN = 128;
   OpMem WpWaT_op, Wc_op;  // [2H rows x Kpad], [H rows x 2*Kpad]
@@ -309,7 +314,7 @@ struct zrnn_attention {
   ~zrnn_attention() {
     cudaFree(WpWaT); cudaFree(v_p); cudaFree(bias); cudaFree(Wc1); cudaFree(Wc2);
     tq.release(); ctx.release(); WpWaT_op.release(); Wc_op.release();
-    ctx_op.release(); sc_h.release();
+    ctx_op.release(); sc_h.release(); m4_work.release();
   }
 };
 
@@ -349,15 +354,25 @@ void prof_attach(P& tp) {
 
 // One word per device, in page-locked host memory that the device can write: after a synchronised pass the host reads it
 // without a copy (a blocking 4-byte copy took 8 of the 127 us of the smallest scoring call).
+// The first call on a device may come from several threads at once, or from within a stream capture, which an allocation would end.
 int* tc_error_word() {
-  static int* p[64] = {nullptr};
+  static std::atomic<int*> p[64];
+  static std::mutex m;
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
-  if (!p[dev]) {
-    if (cudaHostAlloc((void**)&p[dev], sizeof(int), cudaHostAllocMapped) != cudaSuccess) return nullptr;
-    *p[dev] = 0;
-  }
-  return p[dev];
+  int* w = p[dev].load(std::memory_order_acquire);
+  if (w) return w;
+  std::lock_guard<std::mutex> hold(m);
+  w = p[dev].load(std::memory_order_acquire);
+  if (w) return w;
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  const cudaError_t e = cudaHostAlloc((void**)&w, sizeof(int), cudaHostAllocMapped);
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  if (e != cudaSuccess) return nullptr;
+  *w = 0;
+  p[dev].store(w, std::memory_order_release);
+  return w;
 }
 
 // tensor maps of an activation operand: `rows` rows of H valid elements, stride Kpad
@@ -588,6 +603,28 @@ int link_store(int eng, const OpMem& w, int N, int H, int Kpad, const Act* a0, c
   return ZRNN_OK;
 }
 
+int mem4_check(const char* what, int elem, int B, int S_cap, int heads, int d) {
+  ZR_CHECK(elem >= ZRNN_ELEM_F32 && elem <= ZRNN_ELEM_F16, std::string(what) + ": unknown element type");
+  ZR_CHECK(B >= 1 && S_cap >= 1 && heads >= 1 && d >= 1, std::string(what) + ": sizes must be positive");
+  ZR_CHECK(heads <= 65535 && (long long)heads * zrnn::mem4_groups(d) <= (1 << 20), std::string(what) + ": heads * d is too large");
+  ZR_CHECK((long long)B * S_cap <= (1ll << 40) / ((long long)heads * zrnn::mem4_groups(d)), std::string(what) + ": the memory is too large");
+  return ZRNN_OK;
+}
+// global dot attention over a source held in 4 bits: the context, also in operand form
+int att_memory4(zrnn_attention* A, const float* h_t, const int* mask, int B, const Act& ctx, cudaStream_t st) {
+  zrnn::Mem4Attend m;
+  std::memset(&m, 0, sizeof(m));
+  m.codes = (const uint8_t*)A->m4_codes; m.scales = (const __half*)A->m4_scales;
+  m.B = B / A->cols_per_sent; m.S_cap = A->S_max; m.heads = 1; m.d = A->H;
+  m.len = A->len; m.offset = A->off; m.q = h_t; m.ld_q = A->H; m.cols = A->cols_per_sent; m.mask = mask; m.scale = 1.f;
+  m.out = ctx.f32; m.ld_out = A->H;
+  const size_t need = zrnn::mem4_attend_work(m.B, m.cols, m.S_cap, 1, m.d) * sizeof(float);
+  ZR_CUDA(A->m4_work.reserve(need));
+  m.work = A->m4_work.as<float>();
+  ZR_CUDA(zrnn::launch_mem4_attend(m, zrnn::ELEM_F32, st));
+  if (A->eng != ENG_SIMT) ZR_CUDA(zrnn::launch_convert_rows(ctx.f32, B, A->H, A->H, eng_opmode(A->eng), ctx.hi, ctx.lo, A->Kpad, st));
+  return ZRNN_OK;
+}
 // src_ready: a launch of this library lies between the ones that wrote the source states and lengths and the one ahead of this call
 int att_forward(zrnn_attention* A, const Act& h_t, const int* mask, int B, const Act& out, float* align, cudaStream_t st,
                 int* viterbi = nullptr, float viterbi_init = -1.f, bool align_by_pos = false, bool src_ready = true, bool beside = false) {
@@ -627,6 +664,8 @@ int att_forward(zrnn_attention* A, const Act& h_t, const int* mask, int B, const
     }
     a.tanh1 = A->tq.as<float>(); a.q = A->tq.as<float>() + H; a.ld_tq = 2 * H; a.v_p = A->v_p;
     ZR_CUDA(zrnn::launch_att_local(a, st));
+  } else if (A->m4_codes) {
+    ZR_TRY(att_memory4(A, h_t.f32, mask, B, ctx, st));
   } else {
     ZR_CUDA(zrnn::launch_att_global(a, st));
   }
@@ -1267,6 +1306,21 @@ int zrnn_att_set_source(zrnn_attention* A, const float* d_hs, int S_max, int B_s
   ZR_CHECK(S_max <= 10000, "att_set_source: S_max too large");
   A->hs = d_hs; A->S_max = S_max; A->B_src = B_src; A->len = d_len; A->off = d_offset;
   A->cols_per_sent = cols_per_sentence;
+  A->m4_codes = A->m4_scales = nullptr;
+  return ZRNN_OK;
+}
+int zrnn_att_set_source_memory4(zrnn_attention* A, const void* d_codes, const void* d_scales, int S_max, int B_src, const int* d_len,
+                                const int* d_offset, int cols_per_sentence) {
+  ZR_CHECK(A && d_codes && d_scales && d_len && d_offset, "att_set_source_memory4: null argument");
+  ZR_CHECK(A->type == ZRNN_ATT_GLOBAL_DOT, "att_set_source_memory4: global dot attention only");
+  ZR_CHECK(A->H <= zrnn::kMem4MaxHead, "att_set_source_memory4: H of more than 1024");
+  ZR_CHECK(S_max > 0 && B_src > 0 && cols_per_sentence > 0, "att_set_source_memory4: sizes must be positive");
+  ZR_CHECK(cols_per_sentence <= 1000000 && (long long)B_src * cols_per_sentence <= 0x7fffffff, "att_set_source_memory4: too many columns");
+  ZR_CHECK(((uintptr_t)d_codes & 15) == 0 && ((uintptr_t)d_scales & 1) == 0, "att_set_source_memory4: misaligned pointer (codes: 16 bytes)");
+  ZR_TRY(mem4_check("att_set_source_memory4", ZRNN_ELEM_F32, B_src, S_max, 1, A->H));
+  A->hs = nullptr; A->S_max = S_max; A->B_src = B_src; A->len = d_len; A->off = d_offset;
+  A->cols_per_sent = cols_per_sentence;
+  A->m4_codes = d_codes; A->m4_scales = d_scales;
   return ZRNN_OK;
 }
 static thread_local int* g_att_viterbi_out = nullptr;  // set only inside zrnn_att_forward_viterbi
@@ -1274,8 +1328,10 @@ int zrnn_att_forward(zrnn_attention* A, const float* d_h_t, const int* d_mask, i
                      float* d_align_out, void* stream) {
   ZR_CHECK(A && d_h_t && d_htild_out && B >= 0, "att_forward: bad arguments");
   if (!A->loaded) return fail(ZRNN_E_STATE, "att_forward: weights not loaded");
-  if (!A->hs) return fail(ZRNN_E_STATE, "att_forward: zrnn_att_set_source has not been called");
-  ZR_CHECK(B <= A->B_src * A->cols_per_sent, "att_forward: more target columns than source columns provide");
+  if (!A->hs && !A->m4_codes) return fail(ZRNN_E_STATE, "att_forward: zrnn_att_set_source has not been called");
+  ZR_CHECK(B <= (long long)A->B_src * A->cols_per_sent, "att_forward: more target columns than source columns provide");
+  ZR_CHECK(!A->m4_codes || (!d_align_out && !g_att_viterbi_out), "att_forward: alignments are not kept over a source in 4 bits");
+  ZR_CHECK(!A->m4_codes || B % A->cols_per_sent == 0, "att_forward: over a source in 4 bits all columns of a sentence take part");
   if (B == 0) return ZRNN_OK;
   cudaStream_t st = (cudaStream_t)stream;
   Act h, out;
@@ -3059,13 +3115,6 @@ struct Span {
 long long extent(long long cols, long long ld, long long width) { return cols > 0 ? (cols - 1) * ld + width : 0; }
 bool elem_aligned(const void* p, int elem) { return ((uintptr_t)p & (zrnn::elem_bytes(elem) - 1)) == 0; }
 
-int mem4_check(const char* what, int elem, int B, int S_cap, int heads, int d) {
-  ZR_CHECK(elem >= ZRNN_ELEM_F32 && elem <= ZRNN_ELEM_F16, std::string(what) + ": unknown element type");
-  ZR_CHECK(B >= 1 && S_cap >= 1 && heads >= 1 && d >= 1, std::string(what) + ": sizes must be positive");
-  ZR_CHECK(heads <= 65535 && (long long)heads * zrnn::mem4_groups(d) <= (1 << 20), std::string(what) + ": heads * d is too large");
-  ZR_CHECK((long long)B * S_cap <= (1ll << 40) / ((long long)heads * zrnn::mem4_groups(d)), std::string(what) + ": the memory is too large");
-  return ZRNN_OK;
-}
 }  // namespace
 
 extern "C" {
@@ -3143,6 +3192,7 @@ static int linear_args(const char* what, int elem, int act, int n_rows, int n_co
   ZR_CHECK(act >= ZRNN_ACT_NONE && act <= ZRNN_ACT_SILU, std::string(what) + ": unknown activation");
   ZR_CHECK(n_rows >= 1 && n_cols >= 0 && K >= 1, std::string(what) + ": sizes must be positive");
   ZR_CHECK(n_rows <= (1 << 24) && n_cols <= (1 << 24) && K <= (1 << 24), std::string(what) + ": a size of more than 2^24");
+  ZR_CHECK((long long)n_rows * n_cols <= (1ll << 40), std::string(what) + ": more than 2^40 outputs");
   ZR_CHECK(ldw >= K && ldx >= K && ldw <= (1ll << 30) && ldx <= (1ll << 30), std::string(what) + ": bad leading dimension");
   ZR_CHECK(elem_aligned(d_W, elem) && elem_aligned(d_X, elem), std::string(what) + ": misaligned pointer");
   return ZRNN_OK;
@@ -3187,7 +3237,7 @@ int zrnn_linear(int elem, int act, int n_rows, int n_cols, int K, const void* d_
 static int select_args(const char* what, int elem, int n_sent, int beam, int V, int k) {
   ZR_CHECK(elem >= ZRNN_ELEM_F32 && elem <= ZRNN_ELEM_F16, std::string(what) + ": unknown element type");
   ZR_CHECK(n_sent >= 0 && beam >= 1 && V >= 1, std::string(what) + ": sizes must be positive");
-  ZR_CHECK((long long)beam * V <= 0x7fffffff && (long long)n_sent * beam <= 0x7fffffff, std::string(what) + ": too many candidates");
+  ZR_CHECK((long long)beam * V <= 0x7fff0000 && (long long)n_sent * beam <= 0x7fffffff, std::string(what) + ": too many candidates");
   ZR_CHECK(k >= 1 && k <= zrnn::kSelectMax && k <= (long long)beam * V, std::string(what) + ": k must be in [1,64] and at most beam * V");
   return ZRNN_OK;
 }
