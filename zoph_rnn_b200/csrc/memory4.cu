@@ -239,6 +239,7 @@ __global__ void __launch_bounds__(256) mem4_unpack_kernel(const Mem4Unpack a, in
 // asynchronous copies.  Many short heads (SOLO, one warp per team): each team has a column tile and head of its own, all of its slots, and
 // nothing to put together at the end; 481 x 16 heads of 32, one slot: 200 us with a CTA each.  What bounds it is the issue of instructions: turning 8 codes into 4 pairs of halves takes 13, twice per code.
 constexpr int kAttWarps = 16, kAttTile = 32, kAttStages = 3, kAttPartLd = 40;
+enum { ALONE, WHOLE, DEALT };  // a warp per column tile and head; a CTA; several CTAs
 template <int PARTS, int WT, int NB, bool SOLO>
 struct AttShape {
   static constexpr int WARPS = SOLO ? 8 : kAttWarps, TEAMS = WARPS / WT, GP = 2 * NB * WT;  // groups that the team's warps have room for
@@ -254,7 +255,8 @@ struct AttShape {
 };
 struct AttPlan {
   int G, warps, blocks;       // groups of a head; WT and NB
-  int q_tiles, splits;
+  int q_tiles;
+  int parts;                  // > 0: CTAs (per column tile and head) that share the source columns; their sums are combined by a second launch
   bool solo;
 };
 
@@ -288,30 +290,15 @@ __device__ __forceinline__ void copy16(void* dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(shared_at(dst)), "l"(src) : "memory");
 }
 
+// Tiles t0 .. t1 - 1 of source column b (t1 < 0: all of them) for the columns from c0 on and head h.  w: where the sums go, if the column has others
 template <class T, int WT, int NB, bool SOLO>
-__global__ void __launch_bounds__((SOLO ? 8 : kAttWarps) * 32, SOLO && NB == 1 ? 2 : 1) mem4_attend_kernel(const Mem4Attend a, const AttPlan pl) {
+__device__ __forceinline__ void attend_part(const Mem4Attend& a, const AttPlan& pl, unsigned char* smem, int b, int c0, int h, int t0, int t1, float* w) {
   constexpr int PARTS = std::is_same<T, float>::value ? 2 : 1, ROWS = 16 / WT;
   using Sh = AttShape<PARTS, WT, NB, SOLO>;
   static_assert(!SOLO || WT == 1, "");
   constexpr int TEAMS = Sh::TEAMS, GP = Sh::GP, ROW = Sh::ROW;
-  extern __shared__ __align__(16) unsigned char smem[];
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // (the combination waits for this launch's end before it reads anything)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, team = warp / WT, wt = warp % WT;
   const int g = lane >> 2, t = lane & 3, G = pl.G;
-  int b, c0, h, split = 0;
-  if constexpr (SOLO) {
-    const long long unit = (long long)blockIdx.x * TEAMS + team;
-    if (unit >= (long long)a.B * pl.q_tiles * a.heads) return;  // (teams of one warp: no barrier is missed)
-    h = (int)(unit % a.heads);
-    const int bq = (int)(unit / a.heads);
-    b = bq / pl.q_tiles;
-    c0 = (bq - b * pl.q_tiles) * 16;
-  } else {
-    b = blockIdx.y / pl.q_tiles;
-    c0 = (blockIdx.y - b * pl.q_tiles) * 16;
-    h = blockIdx.z;
-    split = blockIdx.x;
-  }
   const int n_cols = min(16, a.cols - c0);
   unsigned char* s_team = smem + (SOLO ? 0 : Sh::Q) + team * Sh::TEAM;
   unsigned char* s_q = SOLO ? s_team + Sh::TEAM - Sh::Q : smem;
@@ -338,8 +325,7 @@ __global__ void __launch_bounds__((SOLO ? 8 : kAttWarps) * 32, SOLO && NB == 1 ?
   const long long off = a.offset ? a.offset[b] : 0;
   const int lo = (int)max(off, 0ll), hi = (int)min(max(off + a.len[b], 0ll), (long long)a.S_cap);
   const int tiles = hi > lo ? (hi - lo + kAttTile - 1) / kAttTile : 0;
-  const int share = pl.splits == 1 ? tiles : tiles / pl.splits, more = tiles - share * pl.splits;
-  const int t0 = split * share + min(split, more), t1 = t0 + share + (split < more);
+  if (t1 < 0) t1 = tiles;
   constexpr int STRIDE = SOLO ? 1 : TEAMS;
   const int tile0 = t0 + (SOLO ? 0 : team), my = t1 > tile0 ? (t1 - tile0 + STRIDE - 1) / STRIDE : 0;  // tiles tile0, + STRIDE, ...
 
@@ -667,9 +653,9 @@ __global__ void __launch_bounds__((SOLO ? 8 : kAttWarps) * 32, SOLO && NB == 1 ?
     if (k < busy) sum += s_ml[256 + k * 16 + warp] * f[k];
   }
   const long long c = (long long)b * a.cols + c0 + warp;
-  const bool part = pl.splits > 1, on = sum != 0.f && (!a.mask || a.mask[c] != 0);
+  const bool part = w != nullptr, on = sum != 0.f && (!a.mask || a.mask[c] != 0);
   const int dp = G * 32;
-  float* w = part ? a.work + (((long long)blockIdx.y * a.heads + h) * pl.splits + split) * 16 * (dp + 2) + warp * (dp + 2) : nullptr;
+  w += part ? warp * (dp + 2) : 0;
   T* out = static_cast<T*>(a.out) + c * a.ld_out + (long long)h * a.d;
   if (part && lane == 0) { w[0] = m; w[1] = sum; }
   const float inv = on ? 1.f / sum : 0.f;
@@ -695,20 +681,80 @@ __global__ void __launch_bounds__((SOLO ? 8 : kAttWarps) * 32, SOLO && NB == 1 ?
     }
   }
 }
+// `parts` CTAs are dealt out to the source columns, one to each and the others by their tiles (16 columns of 4000 .. 8192 slots, 9 CTAs each: the
+// multiprocessors were at work 70 % of the time): the first CTA of column b, for b = 0 .. B (B <= kMostColumns), and its tiles.  By one warp.
+constexpr int kMostColumns = 256;
+__device__ __forceinline__ void deal_out(const Mem4Attend& a, int parts, int* first, int* tiles) {
+  const int lane = threadIdx.x & 31;
+  int total = 0, before = 0;
+  for (int b = lane; b < a.B; b += 32) {
+    const long long off = a.offset ? a.offset[b] : 0;
+    const int lo = (int)max(off, 0ll), hi = (int)min(max(off + a.len[b], 0ll), (long long)a.S_cap);
+    const int n = hi > lo ? (hi - lo + kAttTile - 1) / kAttTile : 0;
+    tiles[b] = n;
+    total += n;
+  }
+  total = __reduce_add_sync(0xffffffffu, total);
+  for (int b0 = 0; b0 < a.B; b0 += 32) {
+    const int b = b0 + lane, n = b < a.B ? 1 + (int)((long long)tiles[b] * (parts - a.B) / max(total, 1)) : 0;
+    int up = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, up, o);
+      if (lane >= o) up += x;
+    }
+    if (b < a.B) first[b] = before + up - n;
+    before += __shfl_sync(0xffffffffu, up, 31);
+  }
+  if (lane == 0) first[a.B] = before;
+  __syncwarp();
+}
+template <class T, int WT, int NB, int HOW>  // HOW: ALONE, WHOLE, DEALT
+__global__ void __launch_bounds__((HOW == ALONE ? 8 : kAttWarps) * 32, HOW == ALONE && NB == 1 ? 2 : 1) mem4_attend_kernel(const Mem4Attend a, const AttPlan pl) {
+  constexpr bool SOLO = HOW == ALONE;
+  extern __shared__ __align__(16) unsigned char smem[];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // (the combination waits for this launch's end before it reads anything)
+  if constexpr (SOLO) {
+    const long long unit = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (unit >= (long long)a.B * pl.q_tiles * a.heads) return;  // (teams of one warp: no barrier is missed)
+    const int bq = (int)(unit / a.heads), b = bq / pl.q_tiles;
+    attend_part<T, WT, NB, SOLO>(a, pl, smem, b, (bq - b * pl.q_tiles) * 16, (int)(unit - (long long)bq * a.heads), 0, -1, nullptr);
+  } else if constexpr (HOW == DEALT) {
+    __shared__ int s_first[kMostColumns + 1], s_tiles[kMostColumns];
+    if (threadIdx.x < 32) deal_out(a, pl.parts, s_first, s_tiles);
+    __syncthreads();
+    const int p = blockIdx.x;
+    if (p >= s_first[a.B]) return;  // (the whole CTA)
+    int b = 0, hi = a.B;
+    while (hi - b > 1) {
+      const int mid = (b + hi) / 2;
+      if (s_first[mid] <= p) b = mid;
+      else hi = mid;
+    }
+    const int n = s_first[b + 1] - s_first[b], k = p - s_first[b], share = s_tiles[b] / n, more = s_tiles[b] - share * n, t0 = k * share + min(k, more);
+    attend_part<T, WT, NB, SOLO>(a, pl, smem, b, blockIdx.y * 16, blockIdx.z, t0, t0 + share + (k < more),
+                                 a.work + (((long long)blockIdx.z * pl.q_tiles + blockIdx.y) * pl.parts + p) * 16 * (pl.G * 32 + 2));
+  } else {
+    const int b = blockIdx.y / pl.q_tiles;
+    attend_part<T, WT, NB, SOLO>(a, pl, smem, b, (blockIdx.y - b * pl.q_tiles) * 16, blockIdx.z, 0, -1, nullptr);
+  }
+}
 // The parts of a column and head: their weights first, then a thread per element
-constexpr int kMostSplits = 1024;
 template <class T>
-__global__ void __launch_bounds__(256) mem4_combine_kernel(const Mem4Attend a, const AttPlan pl) {
-  __shared__ float s_f[kMostSplits], s_red[8];
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int tid = threadIdx.x, h = blockIdx.y, dp = pl.G * 32;
+__global__ void __launch_bounds__(256) mem4_combine_kernel(const __grid_constant__ Mem4Attend a, const AttPlan pl) {
+  __shared__ int s_first[kMostColumns + 1], s_tiles[kMostColumns];
+  __shared__ float s_f[kMostColumns], s_red[8];
   const int pieces = (a.d + 255) / 256;  // of 256 elements, a CTA each
   const long long c = blockIdx.x / pieces, b = c / a.cols;
-  const int at = (int)(c - b * a.cols);
-  const float* w = a.work + ((b * pl.q_tiles + at / 16) * a.heads + h) * pl.splits * 16 * (dp + 2) + (at % 16) * (dp + 2);
+  const int tid = threadIdx.x, h = blockIdx.y, dp = pl.G * 32, at = (int)(c - b * a.cols);
+  if (tid < 32) deal_out(a, pl.parts, s_first, s_tiles);  // (the lengths are not the launch's ahead)
+  __syncthreads();
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const long long step = 16ll * (dp + 2);
+  const int n = s_first[b + 1] - s_first[b];
+  const float* w = a.work + (((long long)h * pl.q_tiles + at / 16) * pl.parts + s_first[b]) * step + (at % 16) * (dp + 2);
   float m = -INFINITY;
-  for (int s = tid; s < pl.splits; s += 256) {
+  for (int s = tid; s < n; s += 256) {
     const float x = __ldcg(w + s * step);
     s_f[s] = x;
     m = fmaxf(m, x);
@@ -721,7 +767,7 @@ __global__ void __launch_bounds__(256) mem4_combine_kernel(const Mem4Attend a, c
   for (int k = 0; k < 8; ++k) m = fmaxf(m, s_red[k]);
   __syncthreads();
   float l = 0.f;
-  for (int s = tid; s < pl.splits; s += 256) {
+  for (int s = tid; s < n; s += 256) {
     const float f = exp2f(s_f[s] - (m == -INFINITY ? 0.f : m));
     s_f[s] = f;
     if (f != 0.f) l += __ldcg(w + s * step + 1) * f;
@@ -740,7 +786,7 @@ __global__ void __launch_bounds__(256) mem4_combine_kernel(const Mem4Attend a, c
   if (i < a.d) {
     float y = 0.f;
 #pragma unroll 8
-    for (int s = 0; s < pl.splits; ++s) {
+    for (int s = 0; s < n; ++s) {
       const float x = __ldcg(w + s * step + 2 + i), f = s_f[s];
       y = f != 0.f ? fmaf(x, f, y) : y;
     }
@@ -793,38 +839,47 @@ cudaError_t launch_mem4_unpack(const Mem4Unpack& a, int elem, cudaStream_t st) {
 }
 namespace {
 
-// Splits: CTAs for every multiprocessor, but at least two tiles for each team of a part.
 AttPlan att_plan(int B, int cols, int S_cap, int heads, int d) {
   AttPlan pl;
   pl.G = mem4_groups(d);
   pl.warps = pl.G <= 4 ? 1 : pl.G <= 8 ? 2 : pl.G <= 16 ? 4 : 8;
   pl.blocks = pl.G <= 2 ? 1 : 2;
   pl.q_tiles = (cols + 15) / 16;
-  const long long units = (long long)B * pl.q_tiles * heads, most = S_cap / (kAttTile * 2 * (kAttWarps / pl.warps));
-  pl.splits = (int)std::max<long long>(1, std::min<long long>(std::min<long long>(device_sms() / units, kMostSplits), most));
+  const long long units = (long long)B * pl.q_tiles * heads, sms = device_sms(), tiles = (S_cap + kAttTile - 1) / kAttTile;
+  // Parts: no more than the multiprocessors, nor than leave each team of a part two tiles; only where there are twice as many of them as source
+  // columns (100 columns of up to 1000 slots on 148 CTAs: 65 us, on 100 53)
+  const long long parts = std::min<long long>(sms / ((long long)pl.q_tiles * heads), B * tiles / (2 * (kAttWarps / pl.warps)));
+  pl.parts = parts >= 2ll * B && parts > 1 && parts <= kMostColumns ? (int)parts : 0;
   // a team on its own: as long as the tiles of all units take its multiprocessor no longer than the CTAs that a unit each would need (in tiles'
   // times: two for the start and the end of a CTA)
-  const long long tiles = (S_cap + kAttTile - 1) / kAttTile, per_sm = pl.blocks == 1 ? 16 : 8, sms = device_sms();
+  const long long per_sm = pl.blocks == 1 ? 16 : 8;
   const long long alone = (units + per_sm * sms - 1) / (per_sm * sms) * (2 + tiles), shared = (units + sms - 1) / sms * (2 + (tiles + 15) / 16);
-  pl.solo = pl.warps == 1 && pl.splits == 1 && alone <= shared;
+  pl.solo = pl.warps == 1 && pl.parts == 0 && alone <= shared;
   return pl;
 }
-template <class T, int WT, int NB, bool SOLO>
+template <class T, int WT, int NB, int HOW>
 cudaError_t attend_launch(const Mem4Attend& a, const AttPlan& pl, cudaStream_t st) {
+  constexpr bool SOLO = HOW == ALONE;
   using Sh = AttShape<std::is_same<T, float>::value ? 2 : 1, WT, NB, SOLO>;
   constexpr int smem = Sh::SMEM;
   static bool configured[64] = {false};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
   if (!configured[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(mem4_attend_kernel<T, WT, NB, SOLO>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    const cudaError_t e = cudaFuncSetAttribute(mem4_attend_kernel<T, WT, NB, HOW>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     configured[dev] = true;
   }
   const long long units = (long long)a.B * pl.q_tiles * a.heads;
-  const dim3 grid = SOLO ? dim3((unsigned)((units + Sh::TEAMS - 1) / Sh::TEAMS)) : dim3(pl.splits, (unsigned)(a.B * pl.q_tiles), (unsigned)a.heads);
-  mem4_attend_kernel<T, WT, NB, SOLO><<<grid, Sh::WARPS * 32, smem, st>>>(a, pl);
+  const dim3 grid = SOLO ? dim3((unsigned)((units + Sh::TEAMS - 1) / Sh::TEAMS)) : pl.parts ? dim3(pl.parts, pl.q_tiles, (unsigned)a.heads) : dim3(1, (unsigned)(a.B * pl.q_tiles), (unsigned)a.heads);
+  mem4_attend_kernel<T, WT, NB, HOW><<<grid, Sh::WARPS * 32, smem, st>>>(a, pl);
   return cudaGetLastError();
+}
+template <class T, int WT, int NB>
+cudaError_t attend_how(const Mem4Attend& a, const AttPlan& pl, cudaStream_t st) {
+  if constexpr (WT == 1)
+    if (pl.solo) return attend_launch<T, WT, NB, ALONE>(a, pl, st);
+  return pl.parts ? attend_launch<T, WT, NB, DEALT>(a, pl, st) : attend_launch<T, WT, NB, WHOLE>(a, pl, st);
 }
 template <class T>
 cudaError_t attend_type(const Mem4Attend& all, cudaStream_t st) {
@@ -844,13 +899,13 @@ cudaError_t attend_type(const Mem4Attend& all, cudaStream_t st) {
     a.q = static_cast<const T*>(a.q) + cols * a.ld_q;
     a.out = static_cast<T*>(a.out) + cols * a.ld_out;
     count_launch();
-    const cudaError_t e = pl.blocks == 1   ? (pl.solo ? attend_launch<T, 1, 1, true>(a, pl, st) : attend_launch<T, 1, 1, false>(a, pl, st))
-                          : pl.warps == 1 ? (pl.solo ? attend_launch<T, 1, 2, true>(a, pl, st) : attend_launch<T, 1, 2, false>(a, pl, st))
-                          : pl.warps == 2 ? attend_launch<T, 2, 2, false>(a, pl, st)
-                          : pl.warps == 4 ? attend_launch<T, 4, 2, false>(a, pl, st)
-                                          : attend_launch<T, 8, 2, false>(a, pl, st);
+    const cudaError_t e = pl.blocks == 1   ? attend_how<T, 1, 1>(a, pl, st)
+                          : pl.warps == 1 ? attend_how<T, 1, 2>(a, pl, st)
+                          : pl.warps == 2 ? attend_how<T, 2, 2>(a, pl, st)
+                          : pl.warps == 4 ? attend_how<T, 4, 2>(a, pl, st)
+                                          : attend_how<T, 8, 2>(a, pl, st);
     if (e != cudaSuccess) return e;
-    if (pl.splits == 1) continue;
+    if (pl.parts == 0) continue;
     cudaLaunchConfig_t cfg;
     std::memset(&cfg, 0, sizeof(cfg));
     cfg.gridDim = dim3((unsigned)((long long)a.B * a.cols * ((a.d + 255) / 256)), a.heads);
@@ -872,7 +927,7 @@ cudaError_t attend_type(const Mem4Attend& all, cudaStream_t st) {
 
 size_t mem4_attend_work(int B, int cols, int S_cap, int heads, int d) {
   const AttPlan pl = att_plan(B, cols, S_cap, heads, d);
-  return pl.splits > 1 ? (size_t)B * pl.q_tiles * heads * pl.splits * 16 * (pl.G * 32 + 2) : 0;
+  return pl.parts ? (size_t)heads * pl.q_tiles * pl.parts * 16 * (pl.G * 32 + 2) : 0;
 }
 cudaError_t launch_mem4_attend(const Mem4Attend& a, int elem, cudaStream_t st) {
   if (a.B == 0 || a.cols == 0) return cudaSuccess;
