@@ -246,7 +246,7 @@ struct AttShape {
   static constexpr int ROW = (GP | 1) * 16;                       // bytes of a slot's codes in shared memory: an odd number of 16 spreads them over the banks
   static constexpr int Q = GP * 2 * PARTS * 512;                  // Q as fragments
   static constexpr int STAGE = kAttTile * ROW + GP * kAttTile * 2;
-  static constexpr int PART = WT * 16 * kAttPartLd * 4, W = 2 * PARTS * 512;
+  static constexpr int PART = WT == 1 ? 0 : WT * 16 * kAttPartLd * 4, W = WT == 1 ? 0 : 2 * PARTS * 512;  // partial scores, weights: a warp alone keeps them
   static constexpr int TEAM = kAttStages * STAGE + PART + W + 192 + (SOLO ? Q : 0);
   static constexpr int OUT_LD = GP * 32 + 2;                      // floats; the teams' outputs take the place of all that
   static constexpr int RUN = (SOLO ? 0 : Q) + TEAMS * TEAM, OUT = SOLO ? 0 : TEAMS * 16 * OUT_LD * 4;
@@ -428,6 +428,12 @@ __device__ __forceinline__ void attend_part(const Mem4Attend& a, const AttPlan& 
 #pragma unroll
       for (int u = 0; u < 4; ++u) acc[x][j][u] = 0.f;
   if (wt == 0 && lane < 16) s_m[lane] = -INFINITY;
+  constexpr bool REG = WT == 1;  // the scores are complete in a warp's registers, and so are the maxima of its rows g and g + 8
+  float m_run[2] = {-INFINITY, -INFINITY}, fac[2] = {0.f, 0.f};
+  if (REG) {
+    fac[0] = s_fac[g];
+    fac[1] = s_fac[g + 8];
+  }
   keep_scales(1);
 
   for (int it = 0; it < my; ++it) {
@@ -438,8 +444,8 @@ __device__ __forceinline__ void attend_part(const Mem4Attend& a, const AttPlan& 
     const unsigned char* s_sc = st + kAttTile * ROW;
     const int n = hi - (lo + (tile0 + it * STRIDE) * kAttTile);
     // scores of this warp's elements; n-tile j has slot 8 j + c in its column c
+    float z[PARTS][4][4];
     {
-      float z[PARTS][4][4];
       const unsigned char* cw = st + g * ROW + wt * (2 * NB * 16) + t * 4;
 #pragma unroll
       for (int k = 0; k < 2 * NB; ++k) {
@@ -464,6 +470,49 @@ __device__ __forceinline__ void attend_part(const Mem4Attend& a, const AttPlan& 
             }
         }
       }
+    }
+    uint4 w[2][PARTS];  // the weights as fragments of the second product
+    float al0, al1;     // what the rows' earlier sums are worth now
+    if constexpr (REG) {
+      // The scores lie as the weights have to: half u % 2 of register 2 (j % 2) (+ 1: rows 8 .. 15) of k-step j / 2 is slot 8 j + 2 t + u % 2
+      float m[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const float y = PARTS == 2 ? fmaf(z[PARTS - 1][j][u], 1.f / 2048.f, z[0][j][u]) : z[0][j][u];
+          z[0][j][u] = 8 * j + 2 * t + (u & 1) < n ? y * fac[u >> 1] : -INFINITY;
+          m[u >> 1] = fmaxf(m[u >> 1], z[0][j][u]);
+        }
+      float ref[2], al[2];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        m[r] = fmaxf(m[r], __shfl_xor_sync(0xffffffffu, m[r], 1));
+        m[r] = fmaxf(fmaxf(m[r], __shfl_xor_sync(0xffffffffu, m[r], 2)), m_run[r]);
+        ref[r] = m[r] == -INFINITY ? 0.f : m[r];
+        al[r] = exp2_approx(m_run[r] - ref[r]);
+        m_run[r] = m[r];
+      }
+      al0 = al[0];
+      al1 = al[1];
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {  // register k: n-tile 2 s + k / 2, rows of half k % 2
+          const int j = 2 * s + (k >> 1), r = k & 1;
+          const float p0 = exp2_approx(z[0][j][2 * r] - ref[r]), p1 = exp2_approx(z[0][j][2 * r + 1] - ref[r]);
+          const __half2 h = __floats2half2_rn(p0, p1);
+          hi[k] = h2_bits(h);
+          if (PARTS == 2) {
+            const float2 f = __half22float2(h);
+            lo[k] = h2_bits(__floats2half2_rn((p0 - f.x) * 2048.f, (p1 - f.y) * 2048.f));
+          }
+        }
+        w[s][0] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        if (PARTS == 2) w[s][PARTS - 1] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      }
+    } else {
       float* at = s_part + (wt * 16 + g) * kAttPartLd + 2 * t;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -473,7 +522,6 @@ __device__ __forceinline__ void attend_part(const Mem4Attend& a, const AttPlan& 
         *reinterpret_cast<float2*>(at + 8 * j) = make_float2(y[0], y[1]);
         *reinterpret_cast<float2*>(at + 8 * j + 8 * kAttPartLd) = make_float2(y[2], y[3]);
       }
-    }
     team_sync();
     // softmax: row r of this warp, slot `lane`; as the second product's k, slot 8 j + c is half j % 2 of register 2 (j / 2) (+ 1: rows 8 .. 15) of lane
     // c / 2 (of a row's four), k-step c % 2, so that a thread's four scales lie side by side
@@ -509,14 +557,15 @@ __device__ __forceinline__ void attend_part(const Mem4Attend& a, const AttPlan& 
       }
     }
     team_sync();
-    // weights x values: n-tile j of a block has element 8 c + j of the block in its column c
-    {
-      uint4 w[2][PARTS];
 #pragma unroll
       for (int s = 0; s < 2; ++s)
 #pragma unroll
         for (int x = 0; x < PARTS; ++x) w[s][x] = *reinterpret_cast<const uint4*>(s_w + (s * PARTS + x) * 512 + lane * 16);
-      const float al0 = s_alpha[g], al1 = s_alpha[g + 8];
+      al0 = s_alpha[g];
+      al1 = s_alpha[g + 8];
+    }
+    // weights x values: n-tile j of a block has element 8 c + j of the block in its column c
+    {
       // With 16-bit operands the products go straight onto the accumulators, which are rescaled where a maximum rose.  The tensor core cuts its
       // sums off: 2^-23 per tile, which 32 bits of result would show, so those add the tile's sums in the ordinary way.
       if (PARTS == 1 && __any_sync(0xffffffffu, al0 != 1.f || al1 != 1.f)) {
@@ -555,8 +604,14 @@ __device__ __forceinline__ void attend_part(const Mem4Attend& a, const AttPlan& 
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
 #pragma unroll
-          for (int u = 0; u < 4; ++u) cw[s][u] = *reinterpret_cast<const uint32_t*>(at + (s + 8 * u) * ROW);
-          sc[s] = *reinterpret_cast<const uint2*>(s_sc + (2 * blk + (g >> 2)) * (kAttTile * 2) + (2 * t + s) * 8);
+          for (int u = 0; u < 4; ++u) cw[s][u] = *reinterpret_cast<const uint32_t*>(at + (REG ? 16 * s + 8 * (u >> 1) + (u & 1) : s + 8 * u) * ROW);
+          const unsigned char* sc_at = s_sc + (2 * blk + (g >> 2)) * (kAttTile * 2) + (2 * t + (REG ? 0 : s)) * 8;
+          if (REG) {  // slots 16 s + 2 t, + 1 and + 8, + 9
+            const uint32_t even = *reinterpret_cast<const uint32_t*>(sc_at + 4 * s), odd = *reinterpret_cast<const uint32_t*>(sc_at + 8 + 4 * s);
+            sc[s] = make_uint2(__byte_perm(even, odd, 0x5410), __byte_perm(even, odd, 0x7632));
+          } else {
+            sc[s] = *reinterpret_cast<const uint2*>(sc_at);
+          }
         }
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
@@ -623,7 +678,14 @@ __device__ __forceinline__ void attend_part(const Mem4Attend& a, const AttPlan& 
   // the teams' maxima and sums, then their outputs side by side
   team_sync();
   if (wt == 0) {
-    if (lane < 16) s_ml[team * 16 + lane] = s_m[lane];
+    if (REG) {
+      if (t == 0) {
+        s_ml[team * 16 + g] = m_run[0];
+        s_ml[team * 16 + g + 8] = m_run[1];
+      }
+    } else if (lane < 16) {
+      s_ml[team * 16 + lane] = s_m[lane];
+    }
     if (t == 0) {
       s_ml[256 + team * 16 + g] = l[0];
       s_ml[256 + team * 16 + g + 8] = l[2];
