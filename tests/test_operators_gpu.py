@@ -718,3 +718,15 @@ def test_many_sentences(api):
     at = [0, 1, 65534, 65535, 65536, 69999]
     v = f64(m.unpack())[at]
     check_attend(out[at], v, f64(q)[at], lens.cpu().numpy()[at], [0] * 6, 1.0, "f32")
+
+
+def test_rows_that_overlap_are_refused(api):
+    one = torch.zeros(1, 64, device="cuda")
+    W = torch.zeros(8, 64, device="cuda")
+    lens = torch.ones(2, dtype=torch.int32, device="cuda")
+    m = api.memory4(2, 3, 64).pack(torch.zeros(3, 1, 64, device="cuda").expand(3, 2, 64))  # (read only: a column for all is fine)
+    for call in (lambda: api.linear(W, one.expand(5, 64)), lambda: api.linear(one.expand(5, 64), W), lambda: api.linear(W, W, out=torch.zeros(1, 8, device="cuda").expand(8, 8)),
+                 lambda: api.beam_select(one.expand(4, 64), torch.zeros(4, device="cuda"), 2, 2), lambda: m.attend(one.expand(4, 64), lens),
+                 lambda: api.linear(W, W.as_strided((4, 64), (32, 1)))):
+        with pytest.raises((api.ZrnnError, ValueError)):
+            call()

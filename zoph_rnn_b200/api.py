@@ -553,7 +553,7 @@ def _rows(t, what, width=None):
         n, w = t.shape
         ld, one = t.stride()
         if (w == width or width is None) and (one == 1 or w <= 1):
-            return n, (ld if n > 1 and ld > 0 else w)
+            return n, (ld if n > 1 else w)  # (rows that overlap: the library refuses them)
     raise ValueError(f"{what}: expected [columns, {'n' if width is None else width}] with contiguous rows, got {tuple(t.shape)} with "
                      f"strides {t.stride()}")
 

@@ -236,8 +236,18 @@ __global__ void __launch_bounds__(256) mem4_unpack_kernel(const Mem4Unpack a, in
 // covers the head and takes tiles of 32 slots, and a CTA has 16 / WT teams, each with slots of its own.  Per tile: the warps'
 // partial scores meet in shared memory, each warp finishes 16 / WT rows (a lane per slot: maximum, exponential, weights written as the
 // fragments of the second product), and all warps add weights x values to their registers.  Codes come three tiles ahead by
-// asynchronous copies.  Many short heads (SOLO, one warp per team): each team has a column tile and head of its own, all of its slots, and
-// nothing to put together at the end; 481 x 16 heads of 32, one slot: 200 us with a CTA each.  What bounds it is the issue of instructions: turning 8 codes into 4 pairs of halves takes 13, twice per code.
+// asynchronous copies.  A warp that has a head to itself (up to 128 elements) keeps scores and weights in registers: they lie there as
+// the second product wants them.
+//
+// Who takes what: ALONE, many short heads: every warp has a column tile and head of its own and all of its slots (481 x 16 heads of 32, one slot: 29 us,
+// with a CTA each 200).  WHOLE: a CTA has a source column.  DEALT: where there are fewer of those than multiprocessors, several CTAs, more for
+// longer ones, and a second launch that combines them.
+//
+// What bounds it is neither memory (16 x 12 columns, 4000 .. 8192 slots of 1024 in bf16: 54 us, 1.0 TB/s) nor one pipe: per 64 slots x 1024 elements a
+// quarter of a multiprocessor has 264 tensor instructions of 8 cycles, 1024 half-precision and some 800 integer ones of 2 each (a word of
+// 8 codes takes 13 instructions to become 4 pairs of halves, twice: the scores need pairs of elements, the output pairs of slots), 2100
+// cycles at the least in each of three pipes, and takes 5300: four warps and their barriers do not fill each other's latencies, and 64
+// registers of output per thread leave no room for more of them.
 constexpr int kAttWarps = 16, kAttTile = 32, kAttStages = 3, kAttPartLd = 40;
 enum { ALONE, WHOLE, DEALT };  // a warp per column tile and head; a CTA; several CTAs
 template <int PARTS, int WT, int NB, bool SOLO>
