@@ -275,7 +275,7 @@ def linear_case(api, dtype, n, K, N, act="none", bias=True, residual=False, pad=
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("n, K, N", [
     (1, 1, 1), (3, 5, 2), (64, 64, 1), (1000, 2000, 12), (1000, 2000, 5), (129, 257, 16), (200, 1000, 17), (500, 96, 33), (256, 512, 64), (300, 40, 65), (1000, 1000, 100),
-    (1000, 2000, 768), (333, 777, 200), (777, 1024, 129), (2048, 320, 300), (130, 4096, 257), (37, 1173, 1), (4100, 64, 513), (515, 8, 1000), (8, 515, 1000), (245, 7428, 3), (40, 16384, 16), (100, 9001, 30), (512, 8192, 512), (1000, 2000, 64)])
+    (1000, 2000, 768), (333, 777, 200), (777, 1024, 129), (2048, 320, 300), (130, 4096, 257), (37, 1173, 1), (4100, 64, 513), (515, 8, 1000), (8, 515, 1000), (300, 1, 300), (300, 3, 200), (245, 7428, 3), (40, 16384, 16), (100, 9001, 30), (512, 8192, 512), (1000, 2000, 64)])
 def test_linear(api, dtype, n, K, N):
     linear_case(api, dtype, n, K, N, seed=n + K)
 
@@ -376,6 +376,22 @@ def test_beam_select(api, dtype, n, beam, V, k):
     lse = torch.logsumexp(z.float(), 1)
     select_case(api, z, scores, beam, k, lse=lse)
     select_case(api, z, scores, beam, k)
+
+
+@pytest.mark.parametrize("dtype, n, beam, V", [("f32", 1, 32, 200001), ("f32", 2, 25, 190003), ("bf16", 1, 50, 200000), ("f16", 1, 3, 3000001)])
+def test_beam_select_of_sentences_too_long_for_a_cluster(api, dtype, n, beam, V):
+    """Lists of many CTAs, merged by a second launch: in shared memory, out of it, and with more ties than it ranks."""
+    g = gen(V)
+    z = 2 * randn(g, n * beam, V, dtype=dtype)
+    scores = -20 + 3 * randn(g, n * beam)
+    done = (torch.rand(n * beam, generator=g, device="cuda") < 0.3).int()
+    for k in (1, 8, 64):
+        select_case(api, z, scores, beam, k)
+    select_case(api, z, scores, beam, 12, done=done, eos=V - 1)
+    z.zero_()
+    for k in (8, 64):
+        _, word, parent = select_case(api, z, torch.zeros_like(scores), beam, k)
+        assert word[0].tolist() == list(range(k)) and parent[0].eq(0).all()
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])

@@ -248,6 +248,7 @@ __global__ void __launch_bounds__(lin_threads(MODE), 1) linear_tc_kernel(const _
       if (CUT) {
         // The CTAs of the cluster each finish every cut-th group of 8 columns: the other ones' sums of it go into that CTA's shared memory, where
         // the operands were (one tile per cluster), and are added to its own in the order of the CTAs.
+        __syncwarp();
         cluster_sync_all();  // all MMAs of all of them are over
         const int per = (nb / 8 + cut - 1) >> p.cut_log2;
         auto slot = [&](int from, int group) { return (uint32_t)((((from * 4 + quad) * per + (group >> p.cut_log2)) * 64 + lane) * 16); };
@@ -261,6 +262,7 @@ __global__ void __launch_bounds__(lin_threads(MODE), 1) linear_tc_kernel(const _
             st_cluster_v4(at + 512, z[j][4], z[j][5], z[j][6], z[j][7]);
           }
         }
+        __syncwarp();
         cluster_sync_all();
         if (ready) {
 #pragma unroll
