@@ -392,7 +392,7 @@ typedef enum { ZRNN_ELEM_F32 = 0, ZRNN_ELEM_BF16 = 1, ZRNN_ELEM_F16 = 2 } zrnn_e
  *   s = fp16(min(a * (1/7), 9352)), a the largest magnitude of the group;  q = x / s rounded to the nearest integer, ties to
  *   even, within -7 .. 7;  the element's value is then q * s rounded to fp16.
  * d_codes [B][S_cap][heads][groups * 16] bytes: q + 8 in 4 bits, the even element of a pair in the low ones; d_scales
- * [B][S_cap][heads][groups] fp16; groups = ceil(d / 32).  4.5 bits per element.  A group of zeros has s = 0; one that holds an
+ * [B][S_cap][heads][groups] fp16; groups = ceil(d / 32), S_cap <= 2^30.  4.5 bits per element.  A group of zeros has s = 0; one that holds an
  * infinity or a NaN has s = NaN, and a column that attends to it gets NaN; magnitudes beyond 65472 saturate.
  * zrnn_memory4_sizes gives the bytes of d_codes (16-byte aligned) and the number of scales. */
 int zrnn_memory4_sizes(int B, int S_cap, int heads, int d, size_t* code_bytes, size_t* n_scales);
@@ -415,8 +415,8 @@ int zrnn_memory4_attend(int elem, const void* d_codes, const void* d_scales, int
 
 /* Y = act(W X + b) + R for n_cols columns: X (K x n_cols), Y and R (n_rows x n_cols) column-major as all activations; the K
  * weights of an output are contiguous and those of the next ldw further (W^T column-major).  d_bias (n_rows, fp32) and
- * d_residual may be NULL; d_residual may be d_Y itself (with ldr == ldy).  ZRNN_ELEM_F32 is accurate to fp32 (3xTF32 or FMA),
- * the 16-bit types multiply their operands as they are.  gelu is x/2 (1 + erf(x / sqrt 2)), silu x / (1 + exp -x). */
+ * d_residual may be NULL; d_residual may be d_Y itself (with ldr == ldy).  ZRNN_ELEM_F32 is accurate to fp32 (3xTF32; an
+ * infinity among its operands makes NaN), the 16-bit types multiply their operands as they are.  gelu is x/2 (1 + erf(x / sqrt 2)), silu x / (1 + exp -x). */
 typedef enum {
   ZRNN_ACT_NONE = 0, ZRNN_ACT_TANH = 1, ZRNN_ACT_SIGMOID = 2, ZRNN_ACT_RELU = 3, ZRNN_ACT_GELU = 4, ZRNN_ACT_SILU = 5
 } zrnn_activation;

@@ -45,6 +45,19 @@ def test_memory4_sizes_refuses(bad):
     refused(_lib.lib().zrnn_memory4_sizes(1, 1, 1, 1, None, ctypes.byref(s)), "null")
 
 
+def test_memory4_of_more_than_2_to_the_30_slots_is_refused():
+    """(A window's end, rounded up to whole tiles, has to be an int.)"""
+    L = _lib.lib()
+    c, s = ctypes.c_size_t(), ctypes.c_size_t()
+    assert L.zrnn_memory4_sizes(1, 1 << 30, 1, 32, ctypes.byref(c), ctypes.byref(s)) == _lib.OK
+    for S in ((1 << 30) + 1, 2**31 - 1):
+        refused(L.zrnn_memory4_sizes(1, S, 1, 32, ctypes.byref(c), ctypes.byref(s)), "slots")
+        refused(L.zrnn_memory4_attend_workspace(1, 1, S, 1, 32, ctypes.byref(c)), "slots")
+        refused(L.zrnn_memory4_pack(0, P, 32, 32, 1, 1, 1, 32, 0, S, P, P, None), "slots")
+        refused(L.zrnn_memory4_unpack(0, P, P, 1, S, 1, 32, 0, 1, P, None), "slots")
+        refused(L.zrnn_memory4_attend(0, P, P, 1, S, 1, 32, P, None, FAR[0], 32, 1, None, 1.0, FAR[1], 32, None, 0, None), "slots")
+
+
 @pytest.mark.parametrize("change, words", [
     (dict(elem=3), "element type"), (dict(elem=-1), "element type"), (dict(S=5, slot0=4), "outside"), (dict(slot0=-1), "outside"),
     (dict(S=-1), "outside"), (dict(S=2**31 - 1, slot0=2**31 - 1), "outside"), (dict(x=None), "null"), (dict(codes=None), "null"),

@@ -606,6 +606,7 @@ int link_store(int eng, const OpMem& w, int N, int H, int Kpad, const Act* a0, c
 int mem4_check(const char* what, int elem, int B, int S_cap, int heads, int d) {
   ZR_CHECK(elem >= ZRNN_ELEM_F32 && elem <= ZRNN_ELEM_F16, std::string(what) + ": unknown element type");
   ZR_CHECK(B >= 1 && S_cap >= 1 && heads >= 1 && d >= 1, std::string(what) + ": sizes must be positive");
+  ZR_CHECK(S_cap <= (1 << 30), std::string(what) + ": more than 2^30 slots");
   ZR_CHECK(heads <= 65535 && (long long)heads * zrnn::mem4_groups(d) <= (1 << 20), std::string(what) + ": heads * d is too large");
   ZR_CHECK((long long)B * S_cap <= (1ll << 40) / ((long long)heads * zrnn::mem4_groups(d)), std::string(what) + ": the memory is too large");
   return ZRNN_OK;
