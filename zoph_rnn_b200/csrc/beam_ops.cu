@@ -449,8 +449,8 @@ void select_plan(int elem, int n_sent, int beam, int V, int k, SelectPlan* pl) {
     pl->NT = 256;
     pl->segs_row = (int)segs(4);
     pl->n_seg = beam * pl->segs_row;
-    // (a part with fewer than k segments would have no bound in step 1)
-    const long long parts = std::max<long long>((pl->n_seg + kSelSegs - 1) / kSelSegs, 4 * sms / n_sent);
+    // (a part with fewer than k segments would have no bound in step 1, and k candidates of each)
+    const long long parts = std::max<long long>((pl->n_seg + kSelSegs - 1) / kSelSegs, std::min(4 * sms / n_sent, pl->n_seg / k));
     pl->per = (int)((pl->n_seg + parts - 1) / parts);
     pl->ctas = pl->parts = (pl->n_seg + pl->per - 1) / pl->per;
     return;
