@@ -17,17 +17,10 @@ constexpr float kMaxScale = 9352.0f;                       // the largest half t
 __device__ __forceinline__ __half mem4_scale(float a) {
   return a < INFINITY ? __float2half_rn(fminf(a * kSeventh, kMaxScale)) : __ushort_as_half(0x7e00);
 }
-// Eight codes: the integer nearest to x / s, ties to even, plus 8.  An addition of 1.5 * 2^23 rounds x times the reciprocal to a whole number, and
-// four of them are put together by multiplications with powers of 16.  The product may lie on the wrong side of the middle between two
-// numbers, by some 2^-20: next to the middle the remainder x - f s decides (exact: at most 24 bits), a tie being one where twice that is s.
-constexpr float kWhole = 12582912.f;
-__device__ __forceinline__ float mem4_near(float x, float s, float f) {
-  const float rem = 2.f * fmaf(-f, s, x);
-  const bool odd = ((int)f & 1) != 0;
-  if (rem > s || (rem == s && odd)) return f + 1.f;
-  if (rem < -s || (rem == -s && odd)) return f - 1.f;
-  return f;
-}
+// Eight codes: the integer nearest to x / s, ties to even, plus 8.  x times an approximate reciprocal, improved by the remainder, is the quotient
+// rounded to 32 bits: exact where x / s is half of an odd number v (16-bit states meet these often), and not v where it is not, for x
+// and v s differ by no less than x's last place, 2^-23 / m(v s) of it with m the mantissa, and half a place of v is 2^-24 / m(v).  An addition
+// of 1.5 * 2^23 then rounds it to a whole number, whose low bits go into the word as they are.
 // two 32-bit operations in one instruction
 __device__ __forceinline__ unsigned long long pair_of(float x, float y) {
   unsigned long long r;
@@ -35,45 +28,40 @@ __device__ __forceinline__ unsigned long long pair_of(float x, float y) {
   return r;
 }
 __device__ __forceinline__ void of_pair(unsigned long long p, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(p)); }
-__device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigned long long b) {
+__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
   unsigned long long r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
-__device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b) {
-  unsigned long long r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+__device__ __forceinline__ float max_abs_nan(float x, float y, float z) {  // the largest magnitude; NaN if one of them is
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
   return r;
 }
-__device__ __forceinline__ unsigned mem4_codes(const float (&x)[8], float s) {
-  float inv;  // (s is no less than 2^-24; an approximation will do)
+// most: the group's largest magnitude
+__device__ __forceinline__ unsigned mem4_codes(const float (&x)[8], float s, float most) {
+  float inv;  // (s is no less than 2^-24)
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
-  const unsigned long long inv2 = pair_of(inv, inv), whole = pair_of(kWhole, kWhole), less = pair_of(-kWhole, -kWhole);
-  float f[8], far = 0.f;
+  const unsigned long long inv2 = pair_of(inv, inv), minus_s = pair_of(-s, -s), zero = pair_of(0.f, 0.f), one = pair_of(1.f, 1.f), whole = pair_of(12582920.f, 12582920.f);
+  float t[8];
 #pragma unroll
   for (int u = 0; u < 8; u += 2) {
-    float t0, t1, d0, d1;
-    of_pair(mul2(pair_of(x[u], x[u + 1]), inv2), t0, t1);
-    t0 = fminf(fmaxf(t0, -7.25f), 7.25f);  // (beyond: 7)
-    t1 = fminf(fmaxf(t1, -7.25f), 7.25f);
-    const unsigned long long t = pair_of(t0, t1), r = add2(add2(t, whole), less);
-    of_pair(r, f[u], f[u + 1]);
-    of_pair(add2(t, pair_of(-f[u], -f[u + 1])), d0, d1);
-    far = fmaxf(far, fmaxf(fabsf(d0), fabsf(d1)));
+    const unsigned long long xs = pair_of(x[u], x[u + 1]), near = fma2(xs, inv2, zero);
+    of_pair(fma2(fma2(near, minus_s, xs), inv2, near), t[u], t[u + 1]);
   }
-  if (far > 0.4999f) {
+  if (most * inv > 7.25f) {  // s was rounded far down, or saturated
 #pragma unroll
-    for (int u = 0; u < 8; ++u) f[u] = fminf(fmaxf(mem4_near(x[u], s, f[u]), -7.f), 7.f);
+    for (int u = 0; u < 8; ++u) t[u] = fminf(fmaxf(t[u], -7.f), 7.f);
   }
-  constexpr float eights = 8.f + 128.f + 2048.f + 32768.f;
-  const float lo = fmaf(f[3], 4096.f, fmaf(f[2], 256.f, fmaf(f[1], 16.f, f[0]))) + (kWhole + eights);
-  const float hi = fmaf(f[7], 4096.f, fmaf(f[6], 256.f, fmaf(f[5], 16.f, f[4]))) + (kWhole + eights);
-  return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x5410);
-}
-__device__ __forceinline__ float max_nan(float x, float y) {  // NaN if one of them is
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
-  return r;
+  unsigned w[8];
+#pragma unroll
+  for (int u = 0; u < 8; u += 2) {
+    float r0, r1;
+    of_pair(fma2(pair_of(t[u], t[u + 1]), one, whole), r0, r1);
+    w[u] = __float_as_uint(r0);
+    w[u + 1] = __float_as_uint(r1);
+  }
+  return __byte_perm(w[0] + w[1] * 16 + w[2] * 256 + w[3] * 4096, w[4] + w[5] * 16 + w[6] * 256 + w[7] * 4096, 0x5410);
 }
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 __device__ __forceinline__ __half2 bits_h2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
@@ -94,18 +82,23 @@ __device__ __forceinline__ void dequant4(uint32_t x, __half2 s, uint32_t (&v)[4]
 }
 template <class T> struct Mem4Vec;  // 8 elements
 template <> struct Mem4Vec<float> {
-  static __device__ void load(const float* p, float (&x)[8]) {
-    const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+  float4 a, b;
+  __device__ void clear() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
+  __device__ void load(const float* p) {
+    a = __ldg(reinterpret_cast<const float4*>(p));
+    b = __ldg(reinterpret_cast<const float4*>(p) + 1);
   }
+  __device__ void get(float (&x)[8]) const { x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w; }
   static __device__ void store(float* p, const float (&x)[8]) {
     reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
     reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
   }
 };
 template <class T> struct Mem4Vec {
-  static __device__ void load(const T* p, float (&x)[8]) {
-    const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
+  uint4 a;
+  __device__ void clear() { a = make_uint4(0u, 0u, 0u, 0u); }
+  __device__ void load(const T* p) { a = __ldg(reinterpret_cast<const uint4*>(p)); }
+  __device__ void get(float (&x)[8]) const {
     const unsigned w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -132,9 +125,10 @@ template <class T> struct Mem4Vec {
 // A lane takes 8 elements, four lanes a group, a team of lanes one source column, whose slots it walks through: all indices are computed once
 // per thread (divided per vector, they were two thirds of the instructions).  ALIGNED: vectors lie on 16 bytes and a head is a
 // multiple of 8 elements; else a warp's eight groups, all of one vector, go through shared memory, 32 consecutive elements at a time.
+constexpr int kMem4PerSm = 6;       // CTAs resident on a multiprocessor
 constexpr int kMem4Stage = 8 * 36;  // floats of a warp's groups, four more per group: runs of 8 fall on different banks
 template <class T, bool ALIGNED>
-__global__ void __launch_bounds__(256) mem4_pack_kernel(const Mem4Pack a, int team) {
+__global__ void __launch_bounds__(256, kMem4PerSm) mem4_pack_kernel(const Mem4Pack a, int team) {
   __shared__ __align__(16) float s_stage[ALIGNED ? 1 : 8 * kMem4Stage];
   const int G = mem4_groups(a.d), lane = threadIdx.x % team, sub = threadIdx.x / team, q = blockIdx.z * team + lane, quads = a.heads * G * 4;
   const long long b = (long long)blockIdx.x * (256 / team) + sub;
@@ -149,13 +143,16 @@ __global__ void __launch_bounds__(256) mem4_pack_kernel(const Mem4Pack a, int te
   const long long x_step = gridDim.y * a.ld_slot, step = gridDim.y * row;
   float* stage = s_stage + (ALIGNED ? 0 : (threadIdx.x >> 5) * kMem4Stage);
   const int l32 = threadIdx.x & 31, g0 = (blockIdx.z * team + (lane & ~31)) >> 2;  // the warp's first group
+  Mem4Vec<T> next;  // the slot after this one
+  next.clear();
+  if (ALIGNED) row_x += (long long)h * a.d + i;
+  if (ALIGNED && i < a.d && blockIdx.y < a.S) next.load(row_x);
 #pragma unroll 2
   for (int s = blockIdx.y; s < a.S; s += gridDim.y, row_x += x_step, codes += step * 4, scales += step) {
     float v[8];
     if (ALIGNED) {
-#pragma unroll
-      for (int u = 0; u < 8; ++u) v[u] = 0.f;
-      if (i < a.d) Mem4Vec<T>::load(row_x + (long long)h * a.d + i, v);
+      next.get(v);
+      if (i < a.d && s + (int)gridDim.y < a.S) next.load(row_x + x_step);
     } else {
       float x[8];
 #pragma unroll
@@ -170,27 +167,30 @@ __global__ void __launch_bounds__(256) mem4_pack_kernel(const Mem4Pack a, int te
       const float4 lo = *reinterpret_cast<const float4*>(stage + (l32 >> 2) * 36 + (l32 & 3) * 8), hi = *reinterpret_cast<const float4*>(stage + (l32 >> 2) * 36 + (l32 & 3) * 8 + 4);
       v[0] = lo.x; v[1] = lo.y; v[2] = lo.z; v[3] = lo.w; v[4] = hi.x; v[5] = hi.y; v[6] = hi.z; v[7] = hi.w;
     }
-    float m = fabsf(v[0]);
-#pragma unroll
-    for (int u = 1; u < 8; ++u) m = max_nan(m, fabsf(v[u]));
-    m = max_nan(m, __shfl_xor_sync(four, m, 1));
-    m = max_nan(m, __shfl_xor_sync(four, m, 2));
+    float m = max_abs_nan(v[0], v[1], v[2]);
+    m = max_abs_nan(m, v[3], v[4]);
+    m = max_abs_nan(m, v[5], v[6]);
+    m = max_abs_nan(m, v[7], __shfl_xor_sync(four, max_abs_nan(m, v[7], 0.f), 1));
+    m = max_abs_nan(m, __shfl_xor_sync(four, m, 2), 0.f);
     const __half sh = mem4_scale(m);
     const float sc = __half2float(sh);
-    const unsigned w = sc > 0.f ? mem4_codes(v, sc) : 0x88888888u;
+    const unsigned w = sc > 0.f ? mem4_codes(v, sc, m) : 0x88888888u;
     if (ALIGNED || mine) {
       *codes = w;
       if ((q & 3) == 0) *scales = sh;
     }
   }
 }
+// In 32 bits two lanes share two words, each the same half of both, so that what a store writes are whole sectors (a word's 32 bytes by one lane:
+// 16 x 8192 vectors of 1024 in 153 us, so 99).
 template <class T, bool ALIGNED>
-__global__ void __launch_bounds__(256) mem4_unpack_kernel(const Mem4Unpack a, int team) {
+__global__ void __launch_bounds__(256, kMem4PerSm) mem4_unpack_kernel(const Mem4Unpack a, int team) {
+  constexpr bool HALVES = ALIGNED && sizeof(T) == 4;
   __shared__ __align__(16) float s_stage[ALIGNED ? 1 : 8 * kMem4Stage];
   const int G = mem4_groups(a.d), lane = threadIdx.x % team, sub = threadIdx.x / team, q = blockIdx.z * team + lane, quads = a.heads * G * 4;
   const long long b = (long long)blockIdx.x * (256 / team) + sub;
   const bool mine = q < quads;
-  const int g = q >> 2, h = g / G, i = (q - h * G * 4) * 8;
+  const int g = q >> 2, h = g / G, i = ((HALVES ? q & ~1 : q) - h * G * 4) * 8;
   if (sub >= 256 / team || b >= a.B || (ALIGNED && (!mine || i >= a.d))) return;
   const long long row = (long long)a.heads * G, from = (b * a.S_cap + a.slot0 + blockIdx.y) * row + g, width = (long long)a.heads * a.d;
   const unsigned* codes = reinterpret_cast<const unsigned*>(a.codes) + from * 4 + (q & 3);
@@ -199,10 +199,27 @@ __global__ void __launch_bounds__(256) mem4_unpack_kernel(const Mem4Unpack a, in
   const long long step = gridDim.y * row;
   float* stage = s_stage + (ALIGNED ? 0 : (threadIdx.x >> 5) * kMem4Stage);
   const int l32 = threadIdx.x & 31, g0 = (blockIdx.z * team + (lane & ~31)) >> 2;
-#pragma unroll 4
+  uint2 next[2];  // the words of this slot and the next one; .y: HALVES
+  __half next_scale[2];
+  auto request = [&](int k, int s, const unsigned* from, const __half* from_scale) {
+    next[k] = make_uint2(0u, 0u);
+    next_scale[k] = __ushort_as_half(0);
+    if (s >= a.S || !mine) return;
+    if (HALVES) next[k] = __ldg(reinterpret_cast<const uint2*>(from - (q & 1)));
+    else next[k].x = __ldg(from);
+    next_scale[k] = __ldg(from_scale);
+  };
+  request(0, blockIdx.y, codes, scales);
+  request(1, blockIdx.y + gridDim.y, codes + step * 4, scales + step);
+#pragma unroll 2
   for (int s = blockIdx.y; s < a.S; s += gridDim.y, codes += step * 4, scales += step, row_out += gridDim.y * width) {
-    uint32_t p[4] = {0u, 0u, 0u, 0u};  // (elements 0, 4), (1, 5), (2, 6), (3, 7)
-    if (ALIGNED || mine) dequant4(__ldg(codes), __half2half2(__ldg(scales)), p);
+    const uint2 w = next[0];
+    const __half2 sc = __half2half2(next_scale[0]);
+    next[0] = next[1];
+    next_scale[0] = next_scale[1];
+    request(1, s + 2 * gridDim.y, codes + step * 8, scales + step * 2);
+    uint32_t p[4];  // (elements 0, 4), (1, 5), (2, 6), (3, 7)
+    dequant4(HALVES ? __byte_perm(w.x, w.y, q & 1 ? 0x7632 : 0x5410) : w.x, sc, p);
     float v[8];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
@@ -210,7 +227,11 @@ __global__ void __launch_bounds__(256) mem4_unpack_kernel(const Mem4Unpack a, in
       v[u] = f.x;
       v[u + 4] = f.y;
     }
-    if (ALIGNED) {
+    if constexpr (HALVES) {
+      float4* at = reinterpret_cast<float4*>(row_out + (long long)h * a.d + i) + (q & 1);
+      at[0] = make_float4(v[0], v[1], v[2], v[3]);
+      if (i + 8 < a.d) at[2] = make_float4(v[4], v[5], v[6], v[7]);
+    } else if constexpr (ALIGNED) {
       Mem4Vec<T>::store(row_out + (long long)h * a.d + i, v);
     } else {
       __syncwarp();
@@ -870,19 +891,23 @@ __global__ void __launch_bounds__(256) mem4_combine_kernel(const __grid_constant
 
 namespace {
 
-// Teams of as many lanes as a vector has (256 at most, then several CTAs share it); CTAs along the slots: eight per multiprocessor in all
-dim3 mem4_grid(int B, int S, int heads, int d, bool aligned, int* team) {
+// Teams of as many lanes as a vector has (256 at most, then several CTAs share it).  CTAs along the slots: the six per multiprocessor that are resident
+// at once (with eight, 16 x 8192 vectors of 1024 in bf16 are packed in 78 us, not 64); of longer memories in unpacking, whose stores like
+// to lie together, up to 32 with 16 slots each (61 -> 59 us, fp32 115 -> 99).
+dim3 mem4_grid(int B, int S, int heads, int d, bool aligned, bool unpack, int* team) {
   const int quads = heads * mem4_groups(d) * 4;
   *team = std::min(aligned ? quads : (quads + 31) / 32 * 32, 256);  // (unaligned: whole warps)
   const long long x = (B + 256 / *team - 1) / (256 / *team), z = (quads + *team - 1) / *team;
-  const long long y = std::max<long long>(1, std::min<long long>(S, (16ll * device_sms() + x * z - 1) / (x * z)));
+  const auto along = [&](long long per_sm) { return (per_sm * device_sms() + x * z - 1) / (x * z); };
+  const long long want = unpack ? std::max(along(kMem4PerSm), std::min<long long>(S / 16, along(32))) : along(kMem4PerSm);
+  const long long y = std::max<long long>(1, std::min<long long>(S, want));
   return dim3((unsigned)x, (unsigned)std::min<long long>(y, 65535), (unsigned)z);
 }
 template <class T>
 cudaError_t pack_type(const Mem4Pack& a, cudaStream_t st) {
   int team;
   const bool aligned = ((uintptr_t)a.x & 15) == 0 && a.ld_slot * sizeof(T) % 16 == 0 && a.ld_col * sizeof(T) % 16 == 0 && a.d % 8 == 0;
-  const dim3 grid = mem4_grid(a.B, a.S, a.heads, a.d, aligned, &team);
+  const dim3 grid = mem4_grid(a.B, a.S, a.heads, a.d, aligned, false, &team);
   if (aligned) mem4_pack_kernel<T, true><<<grid, 256, 0, st>>>(a, team);
   else mem4_pack_kernel<T, false><<<grid, 256, 0, st>>>(a, team);
   return cudaGetLastError();
@@ -891,7 +916,7 @@ template <class T>
 cudaError_t unpack_type(const Mem4Unpack& a, cudaStream_t st) {
   int team;
   const bool aligned = ((uintptr_t)a.out & 15) == 0 && a.d % 8 == 0;
-  const dim3 grid = mem4_grid(a.B, a.S, a.heads, a.d, aligned, &team);
+  const dim3 grid = mem4_grid(a.B, a.S, a.heads, a.d, aligned, true, &team);
   if (aligned) mem4_unpack_kernel<T, true><<<grid, 256, 0, st>>>(a, team);
   else mem4_unpack_kernel<T, false><<<grid, 256, 0, st>>>(a, team);
   return cudaGetLastError();
