@@ -74,6 +74,35 @@ def test_codes_next_to_the_middle_between_two(api):
     np.testing.assert_array_equal(m.codes.cpu().numpy(), codes)
 
 
+@pytest.mark.parametrize("first", [0x2000, 0x0001, 0x6c00])
+def test_codes_next_to_the_middle_for_every_mantissa_of_a_scale(api, first):
+    """Scales of 2^-7 .. 2^-6, of the subnormal ones, of 4096 .. 8192: numbers on the middle between two codes and next to it."""
+    s = np.arange(first, first + 1024 - (first & 1), dtype=np.uint16).view(np.float16).astype(np.float32)
+    mid = s[:, None] * (np.arange(-7, 7, dtype=np.float32) + np.float32(0.5))  # (exact: 11 + 4 bits)
+    x = np.zeros((1, len(s), 64), np.float32)
+    for i, v in enumerate((mid, np.nextafter(mid, np.float32(-1e9)), np.nextafter(mid, np.float32(1e9)))):
+        x[0, :, i * 8 : i * 8 + 7] = v[:, :7]
+        x[0, :, 32 + i * 8 : 32 + i * 8 + 7] = v[:, 7:]
+    x[0, :, 31] = x[0, :, 63] = 7 * s  # the groups' largest
+    m = api.memory4(len(s), 1, 64).pack(torch.from_numpy(x).cuda())
+    codes, scales = ref.pack(x.astype(np.float64), 1, 64)
+    assert (scales.astype(np.float32).reshape(-1, 2) == s[:, None]).all()
+    np.testing.assert_array_equal(m.codes.cpu().numpy(), codes)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_ties_of_16_bit_states(api, dtype):
+    """Groups whose largest magnitude is a multiple of 7: a good part of the numbers lies on the middle between two codes."""
+    g = gen(5)
+    x = torch.randint(-28, 29, (40, 6, 320), generator=g, device="cuda").float() * 0.125
+    x[..., ::32] = 3.5  # (28 / 8: the scale is 1/2, odd multiples of 1/4 are ties)
+    x = (x * 2.0 ** torch.randint(-6, 7, (40, 6, 1), generator=g, device="cuda").float()).to(ref.TYPES[dtype])
+    m = api.memory4(6, 40, 320).pack(x)
+    codes, scales = ref.pack(f64(x), 1, 320)
+    np.testing.assert_array_equal(m.scales.cpu().numpy().view(np.uint16), scales.view(np.uint16))
+    np.testing.assert_array_equal(m.codes.cpu().numpy(), codes)
+
+
 def test_pack_of_numbers_at_the_ends_of_the_range(api):
     x = torch.zeros(1, 10, 64, device="cuda")
     x[0, 0, :32] = 1e-9          # below half precision: zeros
