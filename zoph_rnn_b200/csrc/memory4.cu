@@ -467,15 +467,12 @@ __device__ __forceinline__ void attend_part(const Mem4Attend& a, const AttPlan& 
   }
   keep_scales(1);
 
-  for (int it = 0; it < my; ++it) {
-    asm volatile("cp.async.wait_group 1;" ::: "memory");
-    team_sync();  // the tile is there for all, and all are done with the one before
-    request(it + 2);
-    const unsigned char* st = s_team + it % kAttStages * Sh::STAGE;
+  auto stage_at = [&](int it) { return s_team + it % kAttStages * Sh::STAGE; };
+  auto slots_left = [&](int it) { return hi - (lo + (tile0 + it * STRIDE) * kAttTile); };
+  auto scores = [&](int it, float (&z)[PARTS][4][4]) {
+    const unsigned char* st = stage_at(it);
     const unsigned char* s_sc = st + kAttTile * ROW;
-    const int n = hi - (lo + (tile0 + it * STRIDE) * kAttTile);
     // scores of this warp's elements; n-tile j has slot 8 j + c in its column c
-    float z[PARTS][4][4];
     {
       const unsigned char* cw = st + g * ROW + wt * (2 * NB * 16) + t * 4;
 #pragma unroll
@@ -502,48 +499,8 @@ __device__ __forceinline__ void attend_part(const Mem4Attend& a, const AttPlan& 
         }
       }
     }
-    uint4 w[2][PARTS];  // the weights as fragments of the second product
-    float al0, al1;     // what the rows' earlier sums are worth now
-    if constexpr (REG) {
-      // The scores lie as the weights have to: half u % 2 of register 2 (j % 2) (+ 1: rows 8 .. 15) of k-step j / 2 is slot 8 j + 2 t + u % 2
-      float m[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const float y = PARTS == 2 ? fmaf(z[PARTS - 1][j][u], 1.f / 2048.f, z[0][j][u]) : z[0][j][u];
-          z[0][j][u] = 8 * j + 2 * t + (u & 1) < n ? y * fac[u >> 1] : -INFINITY;
-          m[u >> 1] = fmaxf(m[u >> 1], z[0][j][u]);
-        }
-      float ref[2], al[2];
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        m[r] = fmaxf(m[r], __shfl_xor_sync(0xffffffffu, m[r], 1));
-        m[r] = fmaxf(fmaxf(m[r], __shfl_xor_sync(0xffffffffu, m[r], 2)), m_run[r]);
-        ref[r] = m[r] == -INFINITY ? 0.f : m[r];
-        al[r] = exp2_approx(m_run[r] - ref[r]);
-        m_run[r] = m[r];
-      }
-      al0 = al[0];
-      al1 = al[1];
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        uint32_t hi[4], lo[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {  // register k: n-tile 2 s + k / 2, rows of half k % 2
-          const int j = 2 * s + (k >> 1), r = k & 1;
-          const float p0 = exp2_approx(z[0][j][2 * r] - ref[r]), p1 = exp2_approx(z[0][j][2 * r + 1] - ref[r]);
-          const __half2 h = __floats2half2_rn(p0, p1);
-          hi[k] = h2_bits(h);
-          if (PARTS == 2) {
-            const float2 f = __half22float2(h);
-            lo[k] = h2_bits(__floats2half2_rn((p0 - f.x) * 2048.f, (p1 - f.y) * 2048.f));
-          }
-        }
-        w[s][0] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        if (PARTS == 2) w[s][PARTS - 1] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-      }
-    } else {
+  };
+  auto hand_in = [&](const float (&z)[PARTS][4][4]) {  // this warp's share of the scores
       float* at = s_part + (wt * 16 + g) * kAttPartLd + 2 * t;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -553,7 +510,8 @@ __device__ __forceinline__ void attend_part(const Mem4Attend& a, const AttPlan& 
         *reinterpret_cast<float2*>(at + 8 * j) = make_float2(y[0], y[1]);
         *reinterpret_cast<float2*>(at + 8 * j + 8 * kAttPartLd) = make_float2(y[2], y[3]);
       }
-    team_sync();
+  };
+  auto softmax = [&](int n) {
     // softmax: row r of this warp, slot `lane`; as the second product's k, slot 8 j + c is half j % 2 of register 2 (j / 2) (+ 1: rows 8 .. 15) of lane
     // c / 2 (of a row's four), k-step c % 2, so that a thread's four scales lie side by side
     {
@@ -587,14 +545,10 @@ __device__ __forceinline__ void attend_part(const Mem4Attend& a, const AttPlan& 
         }
       }
     }
-    team_sync();
-#pragma unroll
-      for (int s = 0; s < 2; ++s)
-#pragma unroll
-        for (int x = 0; x < PARTS; ++x) w[s][x] = *reinterpret_cast<const uint4*>(s_w + (s * PARTS + x) * 512 + lane * 16);
-      al0 = s_alpha[g];
-      al1 = s_alpha[g + 8];
-    }
+  };
+  auto output = [&](int it, const uint4 (&w)[2][PARTS], float al0, float al1) {
+    const unsigned char* st = stage_at(it);
+    const unsigned char* s_sc = st + kAttTile * ROW;
     // weights x values: n-tile j of a block has element 8 c + j of the block in its column c
     {
       // With 16-bit operands the products go straight onto the accumulators, which are rescaled where a maximum rose.  The tensor core cuts its
@@ -673,7 +627,94 @@ __device__ __forceinline__ void attend_part(const Mem4Attend& a, const AttPlan& 
         }
       }
     }
-    keep_scales(it + 2);
+  };
+  // w: the weights as fragments of the second product; al0, al1: what the rows' earlier sums are worth now
+  if constexpr (REG) {
+    for (int it = 0; it < my; ++it) {
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
+      team_sync();  // the tile is there for all, and all are done with the one before
+      request(it + 2);
+      const int n = slots_left(it);
+      float z[PARTS][4][4];
+      scores(it, z);
+      uint4 w[2][PARTS];
+      float al0, al1;
+      // The scores lie as the weights have to: half u % 2 of register 2 (j % 2) (+ 1: rows 8 .. 15) of k-step j / 2 is slot 8 j + 2 t + u % 2
+      float m[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const float y = PARTS == 2 ? fmaf(z[PARTS - 1][j][u], 1.f / 2048.f, z[0][j][u]) : z[0][j][u];
+          z[0][j][u] = 8 * j + 2 * t + (u & 1) < n ? y * fac[u >> 1] : -INFINITY;
+          m[u >> 1] = fmaxf(m[u >> 1], z[0][j][u]);
+        }
+      float ref[2], al[2];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        m[r] = fmaxf(m[r], __shfl_xor_sync(0xffffffffu, m[r], 1));
+        m[r] = fmaxf(fmaxf(m[r], __shfl_xor_sync(0xffffffffu, m[r], 2)), m_run[r]);
+        ref[r] = m[r] == -INFINITY ? 0.f : m[r];
+        al[r] = exp2_approx(m_run[r] - ref[r]);
+        m_run[r] = m[r];
+      }
+      al0 = al[0];
+      al1 = al[1];
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {  // register k: n-tile 2 s + k / 2, rows of half k % 2
+          const int j = 2 * s + (k >> 1), r = k & 1;
+          const float p0 = exp2_approx(z[0][j][2 * r] - ref[r]), p1 = exp2_approx(z[0][j][2 * r + 1] - ref[r]);
+          const __half2 h = __floats2half2_rn(p0, p1);
+          hi[k] = h2_bits(h);
+          if (PARTS == 2) {
+            const float2 f = __half22float2(h);
+            lo[k] = h2_bits(__floats2half2_rn((p0 - f.x) * 2048.f, (p1 - f.y) * 2048.f));
+          }
+        }
+        w[s][0] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        if (PARTS == 2) w[s][PARTS - 1] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      }
+      output(it, w, al0, al1);
+      keep_scales(it + 2);
+    }
+  } else if (my > 0) {
+    // A tile's scores before the output of the one ahead of it: between two barriers lies the work of both products, and the softmax after them is
+    // the other teams' time.
+    auto next_scores = [&](int it) {
+      float z[PARTS][4][4];
+      scores(it, z);
+      hand_in(z);
+    };
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    team_sync();  // tile 0 is there for all
+    next_scores(0);
+    team_sync();
+    request(2);
+    softmax(slots_left(0));
+    for (int it = 0; it < my; ++it) {
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
+      team_sync();  // tile it + 1 is there for all, and tile it's weights
+      if (it + 1 < my) next_scores(it + 1);
+      {
+        uint4 w[2][PARTS];
+        float al0, al1;
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int x = 0; x < PARTS; ++x) w[s][x] = *reinterpret_cast<const uint4*>(s_w + (s * PARTS + x) * 512 + lane * 16);
+      al0 = s_alpha[g];
+      al1 = s_alpha[g + 8];
+        output(it, w, al0, al1);
+      }
+      keep_scales(it + 2);
+      if (it + 1 == my) break;
+      team_sync();  // all are done with tile it, and their scores are there
+      request(it + 3);
+      softmax(slots_left(it + 1));
+    }
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
 
