@@ -815,12 +815,14 @@ __device__ __forceinline__ void attend_part(const Mem4Attend& a, const AttPlan& 
     }
   }
 }
-// `parts` CTAs are dealt out to the source columns, one to each and the others by their tiles (16 columns of 4000 .. 8192 slots, 9 CTAs each: the
-// multiprocessors were at work 70 % of the time): the first CTA of column b, for b = 0 .. B (B <= kMostColumns), and its tiles.  By one warp.
+// `parts` CTAs are dealt out to the source columns: at least one each, and so many that none has more tiles than the least number with which they
+// suffice.  (16 columns of 4000 .. 8192 slots: 9 CTAs each: the multiprocessors were at work 70 % of the time; one each and the others by
+// tiles, rounded down: 90 %, 54 us, so NEW.)  The first CTA of column b, for b = 0 .. B (B <= kMostColumns), and its tiles.  By one warp.
 constexpr int kMostColumns = 256;
 __device__ __forceinline__ void deal_out(const Mem4Attend& a, int parts, int* first, int* tiles) {
   const int lane = threadIdx.x & 31;
   int total = 0, before = 0;
+  const auto per_column = [](int tiles, int most) { return max(1, (tiles + most - 1) / most); };
   for (int b = lane; b < a.B; b += 32) {
     const long long off = a.offset ? a.offset[b] : 0;
     const int lo = (int)max(off, 0ll), hi = (int)min(max(off + a.len[b], 0ll), (long long)a.S_cap);
@@ -829,8 +831,16 @@ __device__ __forceinline__ void deal_out(const Mem4Attend& a, int parts, int* fi
     total += n;
   }
   total = __reduce_add_sync(0xffffffffu, total);
+  int low = max(1, (total + parts - 1) / parts), most = max(1, (total + parts - a.B - 1) / (parts - a.B));  // (with `most` they suffice: parts > B)
+  while (low < most) {
+    const int mid = (low + most) / 2;
+    int n = 0;
+    for (int b = lane; b < a.B; b += 32) n += per_column(tiles[b], mid);
+    if ((int)__reduce_add_sync(0xffffffffu, n) <= parts) most = mid;
+    else low = mid + 1;
+  }
   for (int b0 = 0; b0 < a.B; b0 += 32) {
-    const int b = b0 + lane, n = b < a.B ? 1 + (int)((long long)tiles[b] * (parts - a.B) / max(total, 1)) : 0;
+    const int b = b0 + lane, n = b < a.B ? per_column(tiles[b], most) : 0;
     int up = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
