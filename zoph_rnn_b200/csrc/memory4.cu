@@ -311,6 +311,9 @@ __device__ __forceinline__ float warp_max(float x) {
   asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
   return y;
 }
+// What a row's weights are relative to: a maximum that is followed only once it has risen by 2^8, so that sums are seldom rescaled (weights of
+// up to 256 are as good in half precision as those of up to 1)
+__device__ __forceinline__ float risen(float before, float now) { return now > before + 8.f ? now : before; }
 // x as a half and, times 2^11, what that leaves
 __device__ __forceinline__ void split_half(float x, __half& hi, __half& lo) {
   hi = __float2half_rn(x);
@@ -531,7 +534,7 @@ __device__ __forceinline__ void attend_part(const Mem4Attend& a, const AttPlan& 
 #pragma unroll
         for (int rr = 0; rr < RC; ++rr) {
           const int r = r0 + rr;
-          const float m_new = fmaxf(m_old[rr], warp_max(z[rr])), ref = m_new == -INFINITY ? 0.f : m_new;
+          const float m_new = risen(m_old[rr], warp_max(z[rr])), ref = m_new == -INFINITY ? 0.f : m_new;
           const float alpha = exp2_approx(m_old[rr] - ref), p = exp2_approx(z[rr] - ref);
           if (lane == 0) {
             s_alpha[r] = alpha;
@@ -653,7 +656,7 @@ __device__ __forceinline__ void attend_part(const Mem4Attend& a, const AttPlan& 
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         m[r] = fmaxf(m[r], __shfl_xor_sync(0xffffffffu, m[r], 1));
-        m[r] = fmaxf(fmaxf(m[r], __shfl_xor_sync(0xffffffffu, m[r], 2)), m_run[r]);
+        m[r] = risen(m_run[r], fmaxf(m[r], __shfl_xor_sync(0xffffffffu, m[r], 2)));
         ref[r] = m[r] == -INFINITY ? 0.f : m[r];
         al[r] = exp2_approx(m_run[r] - ref[r]);
         m_run[r] = m[r];
