@@ -36,7 +36,7 @@ constexpr int kEpiWarps = 16, kLoadWarp = 16, kMmaWarp = 17, kSplitWarp0 = 18, k
 constexpr int kSmem = 227 * 1024, kMaxStages = 8, kRound = 4;  // kRound: k-blocks per fresh accumulator (32 bits)
 static_assert(fills_sm(kSmem), "both CTAs of a pair hold all of the tensor memory");
 __host__ __device__ constexpr int lin_threads(int mode) { return mode == LIN_F32 ? 32 * (kSplitWarp0 + kSplitTeams * kSplitWarps) : 32 * kSplitWarp0; }
-__host__ __device__ constexpr int lin_max_nb(int mode, bool cut) { return mode == LIN_F32 || cut ? 128 : 256; }
+__host__ __device__ constexpr int lin_max_nb(int mode, bool cut) { return mode == LIN_F32 ? 96 : cut ? 128 : 256; }
 __host__ __device__ constexpr uint32_t lin_fmt(int mode) { return mode == LIN_BF16 ? 1u : mode == LIN_F16 ? 0u : 2u; }
 struct LinParams {
   CUtensorMap w, x;  // boxes of 128 rows and of nb / CG columns
@@ -70,6 +70,21 @@ __device__ __forceinline__ void lin_mma(uint32_t d, uint64_t da, uint64_t db, ui
   if constexpr (CG == 2) umma_pair<TF32>(d, da, db, idesc, accumulate);
   else umma<TF32>(d, da, db, idesc, accumulate);
 }
+// the same with the outputs' operand in tensor memory (a: its first column there), tf32
+template <int CG>
+__device__ __forceinline__ void lin_mma_ts(uint32_t d, uint32_t a, uint64_t db, uint32_t idesc) {
+  if constexpr (CG == 2)
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::tf32 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(db), "r"(idesc), "r"(1u) : "memory");
+  else
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::tf32 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(db), "r"(idesc), "r"(1u) : "memory");
+}
+// a lane's 16 words into 16 columns of tensor memory
+__device__ __forceinline__ void lin_tmem_st16(uint32_t at, const uint32_t (&v)[16]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(at), "r"(v[0]),
+               "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]),
+               "r"(v[13]), "r"(v[14]), "r"(v[15])
+               : "memory");
+}
 template <int CG>
 __device__ __forceinline__ void lin_commit(uint64_t* bar) {
   if constexpr (CG == 2) umma_commit_pair(bar);
@@ -93,9 +108,10 @@ __global__ void __launch_bounds__(lin_threads(MODE), 1) linear_tc_kernel(const _
   const int rank = CG == 2 ? (int)(blockIdx.x & 1) : 0, cut = CUT ? 1 << p.cut_log2 : 1, unit = blockIdx.x / CG >> (CUT ? p.cut_log2 : 0), n_units = gridDim.x / CG >> (CUT ? p.cut_log2 : 0);
   const int part = CUT ? (int)blockIdx.x & (cut - 1) : 0;
   const int kb0 = CUT ? (int)((long long)p.kb * part >> p.cut_log2) : 0, kb = CUT ? (int)((long long)p.kb * (part + 1) >> p.cut_log2) - kb0 : p.kb;  // this CTA's k-blocks
-  const int nb = p.nb, x_rows = nb / CG, w_bytes = 128 * 128, x_bytes = x_rows * 128, raw = w_bytes + x_bytes, stage = raw * (F32 ? 2 : 1);
-  // a stage: W, X; in 32 bits also X lo and W lo, in that order: X and its rest are one operand of twice the columns
-  const int w_off = w_bytes + 2 * x_bytes, acc = nb * (F32 ? 2 : 1);
+  const int nb = p.nb, x_rows = nb / CG, w_bytes = 128 * 128, x_bytes = x_rows * 128, raw = w_bytes + x_bytes, stage = raw + (F32 ? x_bytes : 0);
+  // a stage: W, X; in 32 bits also X lo: X and its rest are one operand of twice the columns.  W lo lies in tensor memory, 32 columns per stage
+  // behind the accumulators.
+  const int acc = nb * (F32 ? 2 : 1);
   LinCtrl& ct = *reinterpret_cast<LinCtrl*>(lin_smem + (size_t)p.stages * stage);
   const int n_tiles = p.r_tiles * p.n_ct, rounds = F32 ? (kb + kRound - 1) / kRound : 1;
   if (threadIdx.x == 0) {
@@ -152,6 +168,7 @@ __global__ void __launch_bounds__(lin_threads(MODE), 1) linear_tc_kernel(const _
     if (rank == 0 && sound) {
       const bool one = elect_one();
       const uint32_t idesc = CG == 2 ? make_idesc_pair(lin_fmt(MODE), (uint32_t)nb) : make_idesc(lin_fmt(MODE), (uint32_t)nb);
+      const uint32_t w_lo = tmem_base + 2u * acc;
       const uint32_t idesc2 = CG == 2 ? 0u : make_idesc(lin_fmt(MODE), 2u * nb);
       int st = 0, use = 0;
       uint32_t ph = 0;
@@ -168,7 +185,7 @@ __global__ void __launch_bounds__(lin_threads(MODE), 1) linear_tc_kernel(const _
                                : mbar_wait_warp(F32 ? &ct.split[st] : &ct.full[st], ph, &ct.abort, p.a.err, 2))) { ok = false; break; }
           tc_fence_after();
           const uint32_t w_addr = smem_u32(lin_smem + (size_t)st * stage), x_addr = w_addr + w_bytes;
-          const uint64_t dw = make_smem_desc(w_addr), dx = make_smem_desc(x_addr), dwl = make_smem_desc(w_addr + w_off), dxl = make_smem_desc(x_addr + x_bytes);
+          const uint64_t dw = make_smem_desc(w_addr), dx = make_smem_desc(x_addr), dxl = make_smem_desc(x_addr + x_bytes);
           if (one) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -179,7 +196,7 @@ __global__ void __launch_bounds__(lin_threads(MODE), 1) linear_tc_kernel(const _
                 lin_mma<CG, F32>(d, dw + 2 * i, dx + 2 * i, idesc, more);
                 if (F32) lin_mma<CG, F32>(d + nb, dw + 2 * i, dxl + 2 * i, idesc, more);
               }
-              if (F32) lin_mma<CG, F32>(d + nb, dwl + 2 * i, dx + 2 * i, idesc, 1u);
+              if constexpr (F32) lin_mma_ts<CG>(d + nb, w_lo + (uint32_t)(32 * st + 8 * i), dx + 2 * i, idesc);
             }
             lin_commit<CG>(&ct.empty[st]);
           }
@@ -340,7 +357,8 @@ __global__ void __launch_bounds__(lin_threads(MODE), 1) linear_tc_kernel(const _
     // ------------------------------------------------------------ the lo parts of a stage: what tf32 cuts off of the tile beside it
     // Teams of four warps take the k-blocks in turn: one's waits are filled by the others.
     const int team = (warp - kSplitWarp0) / kSplitWarps, me = (warp - kSplitWarp0) % kSplitWarps * 32 + lane;
-    const int wv = w_bytes / 16, xv = x_bytes / 16;
+    const int wv = w_bytes / 16, xv = x_bytes / 16, row = 32 * (warp & 3) + lane;  // (a warp reaches the lanes of tensor memory that its number gives)
+    const uint32_t w_lo = tmem_base + 2u * acc + ((uint32_t)(row & ~31) << 16);
     long long its = 0;
     for (int tile = unit; tile < n_tiles; tile += n_units) its += kb;
     int st = team % p.stages;
@@ -348,17 +366,25 @@ __global__ void __launch_bounds__(lin_threads(MODE), 1) linear_tc_kernel(const _
     for (long long it = team; it < its && sound; it += kSplitTeams) {
       if (!mbar_wait_warp(&ct.full[st], ph, &ct.abort, p.a.err, 6)) break;
       uint4* tiles = reinterpret_cast<uint4*>(lin_smem + (size_t)st * stage);
-#pragma unroll 4
-      for (int e = me; e < wv; e += kSplitWarps * 32) {
-        const uint4 x = tiles[e];
-        tiles[w_off / 16 + e] = make_uint4(tf32_rest(x.x), tf32_rest(x.y), tf32_rest(x.z), tf32_rest(x.w));
+      tc_fence_after();
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {  // a lane has a row; piece q of it lies at q ^ (row % 8)
+        uint32_t lo[16];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const uint4 x = tiles[row * 8 + ((4 * half + q) ^ (row & 7))];
+          lo[4 * q] = tf32_rest(x.x); lo[4 * q + 1] = tf32_rest(x.y); lo[4 * q + 2] = tf32_rest(x.z); lo[4 * q + 3] = tf32_rest(x.w);
+        }
+        lin_tmem_st16(w_lo + (uint32_t)(32 * st + 16 * half), lo);
       }
 #pragma unroll 2
       for (int e = wv + me; e < wv + xv; e += kSplitWarps * 32) {
         const uint4 x = tiles[e];
         tiles[xv + e] = make_uint4(tf32_rest(x.x), tf32_rest(x.y), tf32_rest(x.z), tf32_rest(x.w));
       }
+      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      tc_fence_before();
       __syncwarp();
       if (lane == 0) {
         if constexpr (CG == 2) mbar_arrive_remote(&ct.split[st], 0);
@@ -455,9 +481,10 @@ LinPlan lin_plan(const LinearArgs& a, int elem) {
 
 template <int MODE, int CG, int ACT, bool CUT>
 cudaError_t lin_launch(LinParams& p, cudaStream_t st) {
-  const int raw = (128 + p.nb / CG) * 128, stage = raw * (MODE == LIN_F32 ? 2 : 1);
+  const int raw = (128 + p.nb / CG) * 128, stage = raw + (MODE == LIN_F32 ? p.nb / CG * 128 : 0);
   const int out = p.bulk ? 128 * p.nb * 2 : 0;
   p.stages = std::min((kSmem - ((int)sizeof(LinCtrl) + 127) / 128 * 128 - out) / stage, (int)kMaxStages);
+  if (MODE == LIN_F32) p.stages = std::min(p.stages, (512 - 4 * p.nb) / 32);  // (what the accumulators leave of tensor memory)
   static bool configured[64] = {false};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
