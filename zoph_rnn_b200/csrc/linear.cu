@@ -1,22 +1,23 @@
 // Y = act(W X + bias) + R for more than a few columns, on tcgen05.
 //
 // A tile is 128 outputs (the M side: a lane of tensor memory per output, so that a warp stores 32 consecutive ones of a column) x nb columns, on one
-// CTA; where there are enough of them, 256 x nb on a pair of CTAs that share the MMAs and hold half of the columns' operand each
-// (tc_pair_device.cuh).  One warp brings the k-blocks of 128 bytes by TMA, one issues the MMAs, sixteen take the accumulators
+// CTA; of 16-bit operands, where there are enough of them, 256 x nb on a pair of CTAs that share the MMAs and hold half of the columns' operand
+// each (tc_pair_device.cuh).  One warp brings the k-blocks of 128 bytes by TMA, one issues the MMAs, sixteen take the accumulators
 // through bias, activation and residual while the next tile's MMAs run; persistent.
 //
 // 32-bit operands go as two tf32 parts each and three products (hi hi; hi lo and lo hi into an accumulator of their own).  The tensor cores
-// ignore the bits below tf32, so the tile that TMA brought is the hi part as it is; three teams of four warps write the lo parts of the stages
-// beside it, element by element, whatever the swizzle (one team alone: a product took 1.7 times as long).  hi and lo of the columns lie one
-// behind the other: on a single CTA W's hi part is read once for both.  A tensor-core accumulator cuts its sums off, so the products of
-// four k-blocks (16 additions) go into a fresh pair, two pairs in turn, and the sixteen warps add those up in ordinary 32-bit
-// arithmetic.  What bounds it is shared memory: per k-block of 256 x 128, a CTA's TMA writes, the splitting's reads and writes and the
-// MMAs' reads are 147 KB, 1152 cycles at 128 bytes each (1314 measured), for MMAs of 768.
+// ignore the bits below tf32, so the tile that TMA brought is the hi part as it is; three teams of four warps make the lo parts of the stages
+// (one team alone: a product took 1.7 times as long): the columns' beside the hi part in shared memory, so that W's hi part is read once for
+// both, the outputs' in tensor memory, which is an operand as well.  A tensor-core accumulator cuts its sums off, so the products of four
+// k-blocks (16 additions) go into a fresh pair, two pairs in turn, and the sixteen warps add those up in ordinary 32-bit arithmetic.
+// What bounds it is shared memory: per k-block of 128 x 96 the TMA writes, the splitting's reads and writes and the MMAs' reads are 120 KB,
+// 940 cycles at 128 bytes each, of 1020 measured (with both lo parts in shared memory 152 KB, with pairs of CTAs 1190 cycles), for MMAs of
+// 580.
 //
 // Long products of few tiles: 2, 4 or 8 CTAs of a cluster share a tile's K axis and exchange their sums through distributed shared memory.
 // 16-bit outputs and residuals of whole tiles go through shared memory and TMA.  us, this kernel / the library's product alone: bf16 16384 x
 // 4096 x 4096 358 / 345, 4096 x 4096 x 512 19 / 15, 512 x 8192 x 512 19 / 19, 1000 x 1000 x 64 6.3 / 4.0; fp32 16384 x 4096 x 4096
-// 2900 / 8390 (FMA), 1000 x 2000 x 768 25 / 83.
+// 2700 / 8400 (FMA), 1000 x 2000 x 768 23 / 83.
 //
 // A CTA asks for all of an SM's shared memory, so that a pair's allocation of tensor memory waits for nobody that could wait for it in turn.
 #include <algorithm>
@@ -71,12 +72,10 @@ __device__ __forceinline__ void lin_mma(uint32_t d, uint64_t da, uint64_t db, ui
   else umma<TF32>(d, da, db, idesc, accumulate);
 }
 // the same with the outputs' operand in tensor memory (a: its first column there), tf32
-template <int CG>
 __device__ __forceinline__ void lin_mma_ts(uint32_t d, uint32_t a, uint64_t db, uint32_t idesc) {
-  if constexpr (CG == 2)
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::tf32 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(db), "r"(idesc), "r"(1u) : "memory");
-  else
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::tf32 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(db), "r"(idesc), "r"(1u) : "memory");
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::tf32 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(db), "r"(idesc),
+               "r"(1u)
+               : "memory");
 }
 // a lane's 16 words into 16 columns of tensor memory
 __device__ __forceinline__ void lin_tmem_st16(uint32_t at, const uint32_t (&v)[16]) {
@@ -102,7 +101,7 @@ __global__ void __launch_bounds__(lin_threads(MODE), 1) linear_tc_kernel(const _
   using T = typename LinElem<MODE>::T;
   constexpr bool F32 = MODE == LIN_F32;
   constexpr int EPK = 128 / (int)sizeof(T), GROUPS = lin_max_nb(MODE, CUT) / 32;
-  static_assert(!CUT || CG == 1, "a pair's tiles are not cut");
+  static_assert(CG == 1 || (!CUT && !F32), "a pair's tiles are of 16-bit operands and not cut");
   extern __shared__ __align__(1024) uint8_t lin_smem[];
   const int warp = uniform_warp(), lane = threadIdx.x & 31;
   const int rank = CG == 2 ? (int)(blockIdx.x & 1) : 0, cut = CUT ? 1 << p.cut_log2 : 1, unit = blockIdx.x / CG >> (CUT ? p.cut_log2 : 0), n_units = gridDim.x / CG >> (CUT ? p.cut_log2 : 0);
@@ -116,8 +115,8 @@ __global__ void __launch_bounds__(lin_threads(MODE), 1) linear_tc_kernel(const _
   const int n_tiles = p.r_tiles * p.n_ct, rounds = F32 ? (kb + kRound - 1) / kRound : 1;
   if (threadIdx.x == 0) {
     for (int s = 0; s < p.stages; ++s) {
-      mbar_init(&ct.full[s], 1);                       // the stage's bytes: 32 bits, of this CTA; else the leader's, of both
-      mbar_init(&ct.split[s], CG * kSplitWarps);       // (the leader's) the lo parts are written
+      mbar_init(&ct.full[s], 1);                       // the stage's bytes; the leader's, of both CTAs
+      mbar_init(&ct.split[s], kSplitWarps);            // the lo parts are written
       mbar_init(&ct.empty[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
@@ -152,11 +151,10 @@ __global__ void __launch_bounds__(lin_threads(MODE), 1) linear_tc_kernel(const _
         if (it >= p.stages && !mbar_wait_warp(&ct.empty[st], ph ^ 1u, &ct.abort, p.a.err, 1)) { ok = false; break; }
         uint8_t* dst = lin_smem + (size_t)st * stage;
         if (one) {
-          // 32 bits: counted here, for the warps that split; else on the leader's barrier, which expects both CTAs' bytes
-          const uint32_t bar = CG == 2 && !F32 ? cluster_map(smem_u32(&ct.full[st]), 0) : smem_u32(&ct.full[st]);
-          if (F32 || rank == 0) mbar_expect_tx(&ct.full[st], (uint32_t)(F32 ? raw : CG * raw));
-          lin_tma<F32 ? 1 : CG>(dst, &p.w, bar, k * EPK, row);
-          lin_tma<F32 ? 1 : CG>(dst + w_bytes, &p.x, bar, k * EPK, col);
+          const uint32_t bar = CG == 2 ? cluster_map(smem_u32(&ct.full[st]), 0) : smem_u32(&ct.full[st]);
+          if (rank == 0) mbar_expect_tx(&ct.full[st], (uint32_t)(CG * raw));
+          lin_tma<CG>(dst, &p.w, bar, k * EPK, row);
+          lin_tma<CG>(dst + w_bytes, &p.x, bar, k * EPK, col);
         }
         __syncwarp();
         if (++st == p.stages) { st = 0; ph ^= 1u; }
@@ -169,7 +167,7 @@ __global__ void __launch_bounds__(lin_threads(MODE), 1) linear_tc_kernel(const _
       const bool one = elect_one();
       const uint32_t idesc = CG == 2 ? make_idesc_pair(lin_fmt(MODE), (uint32_t)nb) : make_idesc(lin_fmt(MODE), (uint32_t)nb);
       const uint32_t w_lo = tmem_base + 2u * acc;
-      const uint32_t idesc2 = CG == 2 ? 0u : make_idesc(lin_fmt(MODE), 2u * nb);
+      const uint32_t idesc2 = make_idesc(lin_fmt(MODE), 2u * nb);
       int st = 0, use = 0;
       uint32_t ph = 0;
       bool ok = true;
@@ -181,22 +179,20 @@ __global__ void __launch_bounds__(lin_threads(MODE), 1) linear_tc_kernel(const _
             if (!mbar_wait_warp(&ct.acc_empty[use & 1], (uint32_t)(((use >> 1) & 1) ^ 1), &ct.abort, p.a.err, 4)) { ok = false; break; }
             d = tmem_base + (uint32_t)((use & 1) * acc);
           }
-          if (!(F32 && CG == 2 ? __all_sync(0xffffffffu, mbar_wait_cluster(&ct.split[st], ph, &ct.abort, p.a.err, 2))
-                               : mbar_wait_warp(F32 ? &ct.split[st] : &ct.full[st], ph, &ct.abort, p.a.err, 2))) { ok = false; break; }
+          if (!mbar_wait_warp(F32 ? &ct.split[st] : &ct.full[st], ph, &ct.abort, p.a.err, 2)) { ok = false; break; }
           tc_fence_after();
           const uint32_t w_addr = smem_u32(lin_smem + (size_t)st * stage), x_addr = w_addr + w_bytes;
-          const uint64_t dw = make_smem_desc(w_addr), dx = make_smem_desc(x_addr), dxl = make_smem_desc(x_addr + x_bytes);
+          const uint64_t dw = make_smem_desc(w_addr), dx = make_smem_desc(x_addr);
           if (one) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const uint32_t more = !fresh || i > 0 ? 1u : 0u;
-              if (F32 && CG == 1) {  // hi times [hi lo] of the columns, twice as wide
-                lin_mma<CG, F32>(d, dw + 2 * i, dx + 2 * i, idesc2, more);
-              } else {               // (of a pair, each CTA has half of the columns' operand: it would be hi lo hi lo)
-                lin_mma<CG, F32>(d, dw + 2 * i, dx + 2 * i, idesc, more);
-                if (F32) lin_mma<CG, F32>(d + nb, dw + 2 * i, dxl + 2 * i, idesc, more);
+              if constexpr (F32) {  // hi times [hi lo] of the columns, twice as wide; lo times hi
+                lin_mma<CG, 1>(d, dw + 2 * i, dx + 2 * i, idesc2, more);
+                lin_mma_ts(d + nb, w_lo + (uint32_t)(32 * st + 8 * i), dx + 2 * i, idesc);
+              } else {
+                lin_mma<CG, 0>(d, dw + 2 * i, dx + 2 * i, idesc, more);
               }
-              if constexpr (F32) lin_mma_ts<CG>(d + nb, w_lo + (uint32_t)(32 * st + 8 * i), dx + 2 * i, idesc);
             }
             lin_commit<CG>(&ct.empty[st]);
           }
@@ -386,10 +382,7 @@ __global__ void __launch_bounds__(lin_threads(MODE), 1) linear_tc_kernel(const _
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) {
-        if constexpr (CG == 2) mbar_arrive_remote(&ct.split[st], 0);
-        else mbar_arrive(&ct.split[st]);
-      }
+      if (lane == 0) mbar_arrive(&ct.split[st]);
       st += kSplitTeams;
       while (st >= p.stages) { st -= p.stages; ph ^= 1u; }
     }
@@ -434,16 +427,16 @@ LinPlan lin_plan(const LinearArgs& a, int elem) {
   const long long rows1 = (a.n + 127) / 128, rows2 = (a.n + 255) / 256;
   // The time of a launch in ns, as measured with all multiprocessors at work: a start and an end (6 us, with a cut 8), and for the busiest unit's
   // tiles the k-blocks or the epilogue, whichever takes longer.  A k-block of 16-bit operands takes a pair the MMAs' time, a CTA that of
-  // its shared memory (450 ns with 224 columns), but no less than 200 ns (its way from the L2); of 32 bits the splitting's and what shared memory lets through: a CTA 400 / 480 / 550 / 760 ns with 32 / 64 / 96 /
-  // 128 columns, a pair 640 up to 96 and 780 with 128 (a stage less).
+  // its shared memory (450 ns with 224 columns), but no less than 200 ns (its way from the L2); of 32 bits what shared memory lets through: 346 / 426 /
+  // 539 ns with 32 / 64 / 96 columns (a pair, with twice the rows on two multiprocessors, 511 / 533 / 627, so there are none).
   double best = 0;
   const bool f32 = elem == ELEM_F32;
-  for (int cg = 1; cg <= 2; ++cg)
+  for (int cg = 1; cg <= (f32 ? 1 : 2); ++cg)
     for (int w = lin_max_nb(elem, false); w >= 32; w -= 32) {
       const int n_ct = (a.N - 1) / w + 1, nb = ((a.N - 1) / n_ct + 32) / 32 * 32;
       if ((long long)nb * (n_ct - 1) >= a.N) continue;
       const long long tiles = (cg == 2 ? rows2 : rows1) * n_ct;
-      const double block = !f32 ? (cg == 2 ? std::max(200.0, 1.1 * nb) : std::max(200.0, 140 + 1.4 * nb)) : cg == 2 ? (nb > 96 ? 780.0 : 640.0) : 330 + 2.3 * nb + (nb > 96 ? 130.0 : 0.0), end = 14.0 * nb;
+      const double block = f32 ? 250 + 3.0 * nb : cg == 2 ? std::max(200.0, 1.1 * nb) : std::max(200.0, 140 + 1.4 * nb), end = 14.0 * nb;
       for (int cut = 1; cut <= 8; cut *= 2) {
         if (cut > 1 && (cg == 2 || kb < 4 * cut || nb / 8 < cut || nb > lin_max_nb(elem, true))) break;
         // clusters of 4 and 8 CTAs that take whole multiprocessors do not fill the processing clusters: 33 and 15 of them on 148
@@ -481,7 +474,7 @@ LinPlan lin_plan(const LinearArgs& a, int elem) {
 
 template <int MODE, int CG, int ACT, bool CUT>
 cudaError_t lin_launch(LinParams& p, cudaStream_t st) {
-  const int raw = (128 + p.nb / CG) * 128, stage = raw + (MODE == LIN_F32 ? p.nb / CG * 128 : 0);
+  const int raw = (128 + p.nb / CG) * 128, stage = raw + (MODE == LIN_F32 ? p.nb * 128 : 0);
   const int out = p.bulk ? 128 * p.nb * 2 : 0;
   p.stages = std::min((kSmem - ((int)sizeof(LinCtrl) + 127) / 128 * 128 - out) / stage, (int)kMaxStages);
   if (MODE == LIN_F32) p.stages = std::min(p.stages, (512 - 4 * p.nb) / 32);  // (what the accumulators leave of tensor memory)
@@ -556,7 +549,9 @@ cudaError_t lin_type(const LinearArgs& all, const LinPlan& pl, cudaStream_t st) 
            (!all.R || make_plain_map(&p.r, all.R, 2, all.n, all.N, all.ldr, 128, pl.nb));
   if (!make_kmajor_map(&p.w, p.a.W, sizeof(T), all.K, all.n, p.a.ldw, 128) || !make_kmajor_map(&p.x, p.a.X, sizeof(T), all.K, all.N, p.a.ldx, pl.nb / pl.cg))
     return cudaErrorInvalidValue;
-  return pl.cg == 2 ? lin_act<MODE, 2, false>(p, st) : pl.cut > 1 ? lin_act<MODE, 1, true>(p, st) : lin_act<MODE, 1, false>(p, st);
+  if constexpr (MODE != LIN_F32)
+    if (pl.cg == 2) return lin_act<MODE, 2, false>(p, st);
+  return pl.cut > 1 ? lin_act<MODE, 1, true>(p, st) : lin_act<MODE, 1, false>(p, st);
 }
 
 }  // namespace
