@@ -425,7 +425,7 @@ LinPlan lin_plan(const LinearArgs& a, int elem) {
   std::memset(&pl, 0, sizeof(pl));
   const int eb = elem_bytes(elem), sms = device_sms(), kb = (a.K * eb + 127) / 128;
   const long long rows1 = (a.n + 127) / 128, rows2 = (a.n + 255) / 256;
-  // The time of a launch in ns, as measured with all multiprocessors at work: a start and an end (6 us, with a cut 8), and for the busiest unit's
+  // The time of a launch in ns, as measured with all multiprocessors at work: a start and an end (4 us, with a cut 6), and for the busiest unit's
   // tiles the k-blocks or the epilogue, whichever takes longer.  A k-block of 16-bit operands takes a pair the MMAs' time, a CTA that of
   // its shared memory (450 ns with 224 columns), but no less than 200 ns (its way from the L2); of 32 bits what shared memory lets through: 346 / 426 /
   // 539 ns with 32 / 64 / 96 columns (a pair, with twice the rows on two multiprocessors, 511 / 533 / 627, so there are none).
@@ -442,7 +442,7 @@ LinPlan lin_plan(const LinearArgs& a, int elem) {
         // clusters of 4 and 8 CTAs that take whole multiprocessors do not fill the processing clusters: 33 and 15 of them on 148
         const long long units = cut == 1 ? sms / cg : cut == 2 ? sms / 2 : cut == 4 ? sms * 33 / 148 : sms * 15 / 148, waves = (tiles + units - 1) / units;
         if (cut > 1 && waves > 1) break;
-        const double cost = waves * std::max(block * ((kb + cut - 1) / cut), end) + end / cut + (cut > 1 ? 8000 : 6000);
+        const double cost = waves * std::max(block * ((kb + cut - 1) / cut), end) + end / cut + (cut > 1 ? 6000 : 4000);
         if (pl.nb == 0 || cost < best) {
           best = cost;
           pl.cg = cg; pl.nb = nb; pl.n_ct = n_ct; pl.cut = cut;
@@ -452,15 +452,18 @@ LinPlan lin_plan(const LinearArgs& a, int elem) {
   const auto off16 = [&](const void* p, long long ld) { return ((uintptr_t)p & 15) != 0 || (ld * eb) % 16 != 0; };
   pl.align_w = off16(a.W, a.ldw);
   pl.align_x = off16(a.X, a.ldx);
-  if (pl.align_w) best += 3000 + (double)a.n * a.K * eb / 1500;
-  if (pl.align_x) best += 3000 + (double)a.N * a.K * eb / 1500;
-  // The kernel for few columns: 4 us, and per chunk of a warp (64 bytes of K) its latency or its share of a multiprocessor that has many CTAs (both in ns, with
-  // tiles of 8, 16 and 32 columns).  Up to 8 columns it is ahead, up to 32 with few weights or rows that would have to be moved first.
+  if (pl.align_w) best += 2000 + (double)a.n * a.K * eb / 3000;
+  if (pl.align_x) best += 2000 + (double)a.N * a.K * eb / 3000;
+  // The kernel for few columns: 2.7 us, and per chunk of a warp (64 bytes of K) its latency or its share of a multiprocessor that has many CTAs (both
+  // in ns, with tiles of 8, 16 and 32 columns), 1.6 times that, in 16 bits 2.3 times, on rows that would have to be moved first.  Up to 8
+  // columns it is ahead, up to 32 with few weights or such rows (us, few / tcgen05: fp32 4000 x 1001 x 20 11.7 / 15.8, 212 x 559 x 1668
+  // 27 / 14, 1000 x 1000 x 48 7.1 / 8.8; bf16 4000 x 1001 x 20 8.8 / 12.1, 1000 x 2001 x 40 15.5 / 12.0, 512 x 512 x 64 3.9 / 5.6).
   static const double lat[2][3] = {{300, 460, 550}, {270, 460, 840}}, thr[2][3] = {{232, 390, 520}, {154, 230, 380}};
   const int t = a.N <= 8 ? 0 : a.N <= 16 ? 1 : 2, cols = 8 << t;
   const int shared = few_cut(a.n, a.N, a.K, eb);
   const double ctas = (double)((a.n + 15) / 16) * ((a.N + cols - 1) / cols) * shared, chunks = (((long long)a.K * eb + 63) / 64 + 8 * shared - 1) / (8 * shared);
-  pl.few = 4000 + (shared > 1 ? 1500 : 0) + chunks * std::max(lat[!f32][t], thr[!f32][t] * ctas / sms) <= best;
+  const double anywhere = !(pl.align_w || pl.align_x || a.K * eb % 16) ? 1.0 : f32 ? 1.6 : 2.3;
+  pl.few = 2700 + (shared > 1 ? 1500 : 0) + anywhere * chunks * std::max(lat[!f32][t], thr[!f32][t] * ctas / sms) <= best;
   if (pl.few) {
     pl.align_w = pl.align_x = false;
     return pl;
