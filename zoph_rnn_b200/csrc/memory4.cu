@@ -264,11 +264,11 @@ __global__ void __launch_bounds__(256, kMem4PerSm) mem4_unpack_kernel(const Mem4
 // with a CTA each 200).  WHOLE: a CTA has a source column.  DEALT: where there are fewer of those than multiprocessors, several CTAs, more for
 // longer ones, and a second launch that combines them.
 //
-// What bounds it is neither memory (16 x 12 columns, 4000 .. 8192 slots of 1024 in bf16: 54 us, 1.0 TB/s) nor one pipe: per 64 slots x 1024 elements a
-// quarter of a multiprocessor has 264 tensor instructions of 8 cycles, 1024 half-precision and some 800 integer ones of 2 each (a word of
-// 8 codes takes 13 instructions to become 4 pairs of halves, twice: the scores need pairs of elements, the output pairs of slots), 2100
-// cycles at the least in each of three pipes, and takes 5300: four warps and their barriers do not fill each other's latencies, and 64
-// registers of output per thread leave no room for more of them.
+// What bounds it is the issue of instructions, not memory (16 x 12 columns, 4000 .. 8192 slots of 1024 in bf16: 52 us, 1.1 TB/s; 40 of them the
+// slots', the rest the start, the teams' and the parts' sums and the combination).  Per 64 slots x 1024 elements a quarter of a
+// multiprocessor has 264 tensor instructions of 8 cycles, 1024 half-precision and some 1300 integer ones of 2 each (a word of 8 codes takes 13
+// instructions to become 4 pairs of halves, twice: the scores need pairs of elements, the output pairs of slots; kept between the two, they
+// would take 64 registers more), in all some 4000, and takes 5500 cycles: four warps do not fill the rest.
 constexpr int kAttWarps = 16, kAttTile = 32, kAttStages = 3, kAttPartLd = 40;
 enum { ALONE, WHOLE, DEALT };  // a warp per column tile and head; a CTA; several CTAs
 template <int PARTS, int WT, int NB, bool SOLO>
@@ -820,7 +820,7 @@ __device__ __forceinline__ void attend_part(const Mem4Attend& a, const AttPlan& 
 }
 // `parts` CTAs are dealt out to the source columns: at least one each, and so many that none has more tiles than the least number with which they
 // suffice.  (16 columns of 4000 .. 8192 slots: 9 CTAs each: the multiprocessors were at work 70 % of the time; one each and the others by
-// tiles, rounded down: 90 %, 54 us, so NEW.)  The first CTA of column b, for b = 0 .. B (B <= kMostColumns), and its tiles.  By one warp.
+// tiles, rounded down: 90 %, 54 us, so 52.5.)  The first CTA of column b, for b = 0 .. B (B <= kMostColumns), and its tiles.  By one warp.
 constexpr int kMostColumns = 256;
 __device__ __forceinline__ void deal_out(const Mem4Attend& a, int parts, int* first, int* tiles) {
   const int lane = threadIdx.x & 31;
