@@ -173,6 +173,29 @@ def check_attend(out, v, q, lens, offsets, scale, dtype, mask=None):
     assert np.isfinite(err).all() and (err <= tol).all(), (err.max(), (err / np.maximum(tol, 1e-300)).max())
 
 
+@pytest.mark.parametrize("lens", [[0, 0, 0, 0, 0], [0, 4000, 0, 0, 1], [4000, 33, 3999, 65, 1000], [2000] * 5])
+def test_attend_over_few_columns_of_very_different_lengths(api, lens):
+    """Source columns that share the multiprocessors: none, one or several CTAs' worth of slots each."""
+    attend_case(api, "bf16", 5, 3, 4000, 1, 264, lens, [4000 - n for n in lens], seed=sum(lens))
+    attend_case(api, "f32", 5, 2, 4000, 1, 72, lens, [0] * 5, seed=sum(lens))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("d, S", [(64, 700), (128, 90), (512, 700)])
+def test_attend_to_scores_that_rise_or_fall_along_the_window(api, dtype, d, S):
+    """Running maxima that rise in many small steps, in a few large ones, or never after the first slots."""
+    g = gen(d)
+    for span in (12.0, 120.0, -40.0):
+        ramp = torch.linspace(0.05, 1.0, S, device="cuda") if span > 0 else torch.linspace(1.0, 0.05, S, device="cuda")
+        u = torch.where(torch.rand(d, generator=g, device="cuda") < 0.5, -1.0, 1.0)
+        hs = (ramp[:, None, None] * u).expand(S, 2, d).contiguous()
+        q = (u * torch.tensor([1.0, 0.5], device="cuda").repeat(2)[:, None]).to(ref.TYPES[dtype])
+        m = api.memory4(2, S, d).pack(hs)
+        lens = [S, S - 40]
+        out = m.attend(q, torch.tensor(lens, dtype=torch.int32, device="cuda"), scale=abs(span) / d)
+        check_attend(out, ref.unpack(m.codes.cpu().numpy(), m.scales.cpu().numpy(), d), f64(q), lens, [0, 0], abs(span) / d, dtype)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("B, cols, S, heads, d", [
     (1, 1, 1, 1, 1), (1, 12, 23, 1, 1000), (3, 5, 33, 1, 100), (2, 12, 64, 1, 512), (4, 1, 31, 1, 320), (2, 17, 65, 1, 1024), (2, 33, 40, 1, 96), (3, 2, 100, 8, 64),
