@@ -493,6 +493,32 @@ def test_beam_select_ties_go_to_the_lowest_candidate(api, dtype, V):
     select_case(api, -up, s, beam, 64)
 
 
+@pytest.mark.parametrize("n, beam, V, k", [(1, 12, 40000, 12), (3, 1, 300, 1), (64, 12, 4000, 12), (20, 2, 64, 5)])
+def test_beam_select_of_one_outstanding_candidate_per_segment(api, n, beam, V, k):
+    """A segment that went missing shows: the best candidates lie one to a segment, in other segments in every call, right after launches that
+    leave the multiprocessors' shared memory full of larger numbers."""
+    g = gen(V + 1)
+    scores = torch.zeros(n * beam, device="cuda")
+    junk = 1e6 + torch.rand(n * beam, V, generator=g, device="cuda")
+    low = -100 - torch.rand(n * beam, V, generator=g, device="cuda")
+    zs, wants = [], []
+    for i in range(30):
+        z = low.clone().view(n, beam * V)
+        at = torch.stack([torch.randperm((beam * V + 127) // 128, generator=g, device="cuda")[:k] for _ in range(n)])
+        at = (128 * at + torch.randint(0, 128, at.shape, generator=g, device="cuda")).clamp(max=beam * V - 1)
+        best = torch.rand(n, at.shape[1], generator=g, device="cuda") + torch.arange(at.shape[1], device="cuda")
+        z.scatter_(1, at, best)
+        zs.append(z.view(n * beam, V))
+        val, cand = z.sort(1, descending=True)
+        wants.append((val[:, :at.shape[1]], cand[:, :at.shape[1]]))
+    for z, (val, cand) in zip(zs, wants):
+        api.beam_select(junk, scores, beam, k)
+        got, word, parent = api.beam_select(z, scores, beam, k)
+        m = val.shape[1]
+        first = torch.arange(n, device="cuda")[:, None] * beam
+        assert torch.equal(got[:, :m], val) and torch.equal((parent[:, :m].long() - first) * V + word[:, :m], cand)
+
+
 def test_beam_select_on_rows_that_start_anywhere(api):
     g = gen(6)
     for dtype in ref.TYPES:

@@ -107,3 +107,23 @@ def test_a_cta_with_all_of_the_tensor_memory_and_a_partner_has_its_sm_for_itself
                      and re.search(r"__cluster_dims__|ClusterDimension", open(os.path.join(CSRC, n)).read())}
     assert with_partners == {"tc_link.cu", "tc_decoder.cu"}  # (the pair kernels allocate through tc_pair_device.cuh)
     assert "static_assert(fills_sm(dec_smem(TC_BF16))" in open(os.path.join(CSRC, "tc_decoder.cu")).read()
+
+
+def test_the_selection_zeroes_its_maxima_before_any_warp_stores_one():
+    """All threads zero the segments' maxima; a warp that is ahead must not store one of its own before another warp's zero of that word has
+    arrived, which would delete the segment: a barrier of the whole CTA lies between, whatever the size of the cluster.  (The cluster
+    barrier that is only arrived at there orders nothing yet.)"""
+    s = body("beam_ops.cu", "beam_select_kernel(const BeamSelect a", "beam_select_merge_kernel")
+    zero, first_use = s.index("s_max[i] = 0;"), s.index("s_max[i] = o;")
+    between = [ln.strip() for ln in s[zero:first_use].splitlines()]
+    assert "__syncthreads();" in between  # (a statement of its own: not one side of a condition)
+    use = s.index("look(c, v0, i);")
+    assert zero < s.index("__syncthreads();", zero) < use
+
+
+def test_the_selection_is_whole_warps_at_its_aligned_cluster_barriers():
+    """The .aligned forms are for warps whose lanes run together; what stands before them may have parted the lanes."""
+    s = body("beam_ops.cu", "beam_select_kernel(const BeamSelect a", "beam_select_merge_kernel")
+    lines = [ln.strip() for ln in s.splitlines() if ln.strip()]
+    at = [i for i, ln in enumerate(lines) if "barrier.cluster" in ln and ".aligned" in ln]
+    assert len(at) == 2 and all(lines[i - 1] == "__syncwarp();" for i in at)

@@ -152,8 +152,9 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 4 : 1) beam_select_kernel(cons
     s_n = s_left = s_chosen_n = 0;
     s_bound = kOrderedMinusInf + 1;
   }
+  __syncthreads();  // (the words are zero before any warp stores a maximum there)
+  __syncwarp();
   if (C > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  else __syncthreads();
   // segment q of a row holds the values [q * E - lead, (q + 1) * E - lead): its vectors lie on 16 bytes
   auto lead_of = [&](const T* row) { return (int)(((uintptr_t)row & 15) / sizeof(T)); };
   // A warp walks over consecutive segments, the next one's vectors requested before it looks at the present one's.
@@ -234,6 +235,7 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 4 : 1) beam_select_kernel(cons
 #pragma unroll
     for (int u = 0; u < kSelSegs / NT; ++u)
       if (v[u] >= floor) s_seg[atomicAdd(&s_left, 1)] = ((unsigned long long)v[u] << 32) | (unsigned)~(first + u * NT + lane * W + warp);
+    __syncwarp();
     if (C > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // (the others' arrays are in place)
     __syncthreads();
     const int left = s_left;
