@@ -248,6 +248,95 @@ def test_what_lies_outside_the_window_is_not_looked_at(api, dtype, heads, d, S):
     assert torch.equal(bad[1, :, 1:], out.view(B, cols, heads, d)[1, :, 1:])
 
 
+def attend_ways(api, B, cols, S, heads, d):
+    """How many bytes of scratch memory an attention asks for: some where several CTAs share a source column, else none."""
+    n = ctypes.c_size_t()
+    assert api.lib().zrnn_memory4_attend_workspace(B, cols, S, heads, d, ctypes.byref(n)) == 0
+    return n.value
+
+
+# several CTAs per source column (heads of one warp, of two teams, of four), a CTA per source column, a warp per column tile and head
+DEALT = [(2, 3, 4000, 2, 64), (3, 4, 4000, 1, 264), (2, 17, 3000, 1, 1000)]
+OTHERS = [(3, 4, 90, 1, 500), (2, 5, 100, 1, 128), (40, 5, 70, 8, 64)]
+
+
+def test_attend_is_shared_by_several_ctas_where_these_tests_mean_it(api):
+    for shape in DEALT:
+        assert attend_ways(api, *shape) > 0
+    for shape in OTHERS:
+        assert attend_ways(api, *shape) == 0
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("B, cols, S, heads, d", DEALT)
+def test_attend_lengths_and_masks_on_several_ctas(api, dtype, B, cols, S, heads, d):
+    """Windows that stick out at either end, empty ones, one slot, masked columns."""
+    for lens, offs in (([S + 50, 0], [-20, 7]), ([-5, S], [3, 0]), ([1, 33], [S - 1, 31]), ([2 * S, S - 100], [100, 2 * S])):
+        lens, offs = (lens + [S // 2])[:B], (offs + [S // 3])[:B]
+        mask = [1] * (B * cols)
+        mask[1] = mask[-1] = 0
+        *_, out = attend_case(api, dtype, B, cols, S, heads, d, lens, offs, mask=mask, seed=d)
+        assert out[1].eq(0).all() and out[-1].eq(0).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("B, cols, S, heads, d", DEALT + OTHERS)
+def test_attend_numbers_that_are_not_finite(api, dtype, B, cols, S, heads, d):
+    """softmax of scores among which one is a NaN is NaN: a query that is not finite, a memory all of NaN, and NaNs in a few slots anywhere of a
+    window reach the columns that attend to them, and no others; masked columns and columns without slots are zeros."""
+    lens, offs = [S] * B, [0] * B
+    mask = [1] * (B * cols)
+    m, q, ln, of, scale, out = attend_case(api, dtype, B, cols, S, heads, d, lens, offs, seed=d)
+    base = out.view(B, cols, heads, d)
+    for bad in (float("nan"), float("inf"), float("-inf")):
+        q2 = q.clone()
+        q2[1, d - 1] = bad  # column 1, head 0
+        got = m.attend(q2, ln, of, scale=scale).view(B, cols, heads, d)
+        assert got[0, 1, 0].isnan().all()
+        got = got.clone()
+        got[0, 1, 0] = base[0, 1, 0]
+        assert torch.equal(got, base)
+        mk = torch.ones(B * cols, dtype=torch.int32, device="cuda")
+        mk[1] = 0
+        assert m.attend(q2, ln, of, scale=scale, mask01=mk)[1].eq(0).all()
+        ln0 = ln.clone()
+        ln0[0] = 0
+        assert m.attend(q2, ln0, of, scale=scale)[:cols].eq(0).all()
+    # NaNs in the memory: all of a sentence, a whole tile of slots, one slot, wherever they lie
+    for at in (slice(0, S), slice(0, min(32, S)), slice(max(0, S - 40), S), slice(S // 2, S // 2 + 1), slice(S - 1, S)):
+        bad = api.memory4(B, S, d, heads=heads, codes=m.codes, scales=m.scales.clone())
+        bad.scales[1, at, 0, -1] = float("nan")
+        got = bad.attend(q, ln, of, scale=scale).view(B, cols, heads, d)
+        assert got[1, :, 0].isnan().all()
+        got = got.clone()
+        got[1, :, 0] = base[1, :, 0]
+        assert torch.equal(got, base)
+    # a NaN among slots whose weights are nothing beside the largest one's
+    g = gen(d)
+    u = torch.where(torch.rand(heads * d, generator=g, device="cuda") < 0.5, -1.0, 1.0)
+    hs = (-u).repeat(S, B, 1)
+    hs[S // 5] = u
+    far = api.memory4(B, S, d, heads=heads).pack(hs)
+    qu = u.to(q.dtype).repeat(B * cols, 1)
+    fine = far.attend(qu, ln, of, scale=400.0 / d)
+    assert fine.isfinite().all()
+    far.scales[0, S - 2, 0, 0] = float("nan")
+    got = far.attend(qu, ln, of, scale=400.0 / d).view(B, cols, heads, d)
+    assert got[0, :, 0].isnan().all() and torch.equal(got[1:], fine.view(B, cols, heads, d)[1:])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("B, cols, S, heads, d", DEALT)
+def test_what_lies_outside_the_window_is_not_looked_at_by_several_ctas(api, dtype, B, cols, S, heads, d):
+    lens, offs = [S - 40, 70, 33][:B], [13, S - 70, 40][:B]
+    m, q, ln, of, scale, out = attend_case(api, dtype, B, cols, S, heads, d, lens, offs)
+    for b in range(B):
+        for at in (slice(0, offs[b]), slice(offs[b] + lens[b], S)):
+            m.codes[b, at] = 255
+            m.scales[b, at] = float("nan")
+    assert torch.equal(m.attend(q, ln, of, scale=scale), out)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 def test_attend_with_large_and_small_queries(api, dtype):
     """Scores in the thousands (one slot takes all the weight), scores of nothing (equal weights), zero queries."""

@@ -917,7 +917,7 @@ __global__ void __launch_bounds__(256) mem4_combine_kernel(const __grid_constant
   for (int s = tid; s < n; s += 256) {
     const float f = exp2f(s_f[s] - (m == -INFINITY ? 0.f : m));
     s_f[s] = f;
-    if (f != 0.f) l += __ldcg(w + s * step + 1) * f;
+    l += __ldcg(w + s * step + 1) * f;  // (also where f is 0: a part whose scores are all NaN has no maximum, but its sum is NaN)
   }
 #pragma unroll
   for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
@@ -926,7 +926,7 @@ __global__ void __launch_bounds__(256) mem4_combine_kernel(const __grid_constant
   l = 0.f;
 #pragma unroll
   for (int k = 0; k < 8; ++k) l += s_red[k];
-  // (l is 0 only where no part had a slot: a NaN among the weights is one here, too)
+  // (l is 0 only where no part had a slot: such a part's sums are zeros)
   const bool on = l != 0.f && (!a.mask || a.mask[c] != 0);
   T* out = static_cast<T*>(a.out) + c * a.ld_out + (long long)h * a.d;
   const int i = (int)(blockIdx.x - c * pieces) * 256 + tid;
@@ -935,7 +935,7 @@ __global__ void __launch_bounds__(256) mem4_combine_kernel(const __grid_constant
 #pragma unroll 8
     for (int s = 0; s < n; ++s) {
       const float x = __ldcg(w + s * step + 2 + i), f = s_f[s];
-      y = f != 0.f ? fmaf(x, f, y) : y;
+      y = fmaf(x, f, y);
     }
     out[i] = from_f32<T>(on ? y / l : 0.f);
   }
