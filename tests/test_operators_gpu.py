@@ -325,6 +325,24 @@ def test_attend_numbers_that_are_not_finite(api, dtype, B, cols, S, heads, d):
     assert got[0, :, 0].isnan().all() and torch.equal(got[1:], fine.view(B, cols, heads, d)[1:])
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("B, cols, S, heads, d", DEALT + OTHERS)
+def test_attend_to_scores_that_are_all_minus_infinity(api, dtype, B, cols, S, heads, d):
+    """The softmax of such a column is NaN; zeros are for columns without slots."""
+    g = gen(d)
+    m = api.memory4(B, S, d, heads=heads).pack(torch.full((S, B, heads * d), 0.5, device="cuda"))
+    q = torch.tanh(torch.randn(B * cols, heads * d, generator=g, device="cuda")).to(ref.TYPES[dtype])
+    ln = torch.full((B,), S, dtype=torch.int32, device="cuda")
+    base = m.attend(q, ln)
+    q2 = q.clone()
+    q2[0, 0] = float("-inf")
+    got = m.attend(q2, ln)
+    assert got[0, :d].isnan().all() and torch.equal(got[1:], base[1:]) and torch.equal(got[0, d:], base[0, d:])
+    mask = torch.ones(B * cols, dtype=torch.int32, device="cuda")
+    mask[0] = 0
+    assert m.attend(q2, ln, mask01=mask)[0].eq(0).all()
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("B, cols, S, heads, d", DEALT)
 def test_what_lies_outside_the_window_is_not_looked_at_by_several_ctas(api, dtype, B, cols, S, heads, d):

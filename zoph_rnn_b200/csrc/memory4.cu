@@ -727,8 +727,9 @@ __device__ __forceinline__ void attend_part(const Mem4Attend& a, const AttPlan& 
       const int r = g + 8 * half;
       if (r >= n_cols) break;
       const long long c = (long long)b * a.cols + c0 + r;
-      const float sum = l[2 * half], inv = sum != 0.f && (!a.mask || a.mask[c] != 0) ? 1.f / sum : 0.f;
-      const bool on = inv != 0.f;  // (a NaN is not 0)
+      // (a column with slots, whatever its sum: one whose scores are all -inf has weights of 0 and gets 0 / 0)
+      const bool on = hi > lo && (!a.mask || a.mask[c] != 0);
+      const float inv = 1.f / l[2 * half];
       T* o = static_cast<T*>(a.out) + c * a.ld_out + (long long)h * a.d;
       const bool vec = ((uintptr_t)o & 15) == 0;
 #pragma unroll
@@ -790,7 +791,7 @@ __device__ __forceinline__ void attend_part(const Mem4Attend& a, const AttPlan& 
     if (k < busy) sum += s_ml[256 + k * 16 + warp] * f[k];
   }
   const long long c = (long long)b * a.cols + c0 + warp;
-  const bool part = w != nullptr, on = sum != 0.f && (!a.mask || a.mask[c] != 0);
+  const bool part = w != nullptr, on = hi > lo && (!a.mask || a.mask[c] != 0);
   const int dp = G * 32;
   w += part ? warp * (dp + 2) : 0;
   T* out = static_cast<T*>(a.out) + c * a.ld_out + (long long)h * a.d;
@@ -926,8 +927,7 @@ __global__ void __launch_bounds__(256) mem4_combine_kernel(const __grid_constant
   l = 0.f;
 #pragma unroll
   for (int k = 0; k < 8; ++k) l += s_red[k];
-  // (l is 0 only where no part had a slot: such a part's sums are zeros)
-  const bool on = l != 0.f && (!a.mask || a.mask[c] != 0);
+  const bool on = s_tiles[b] > 0 && (!a.mask || a.mask[c] != 0);
   T* out = static_cast<T*>(a.out) + c * a.ld_out + (long long)h * a.d;
   const int i = (int)(blockIdx.x - c * pieces) * 256 + tid;
   if (i < a.d) {
