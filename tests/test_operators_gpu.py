@@ -363,6 +363,30 @@ def test_attend_with_large_and_small_queries(api, dtype):
     attend_case(api, dtype, 2, 5, 600, 4, 64, [600, 1], [0, 599], seed=5, qmul=20.0, scale=-0.7)
 
 
+@pytest.mark.parametrize("dtype, qmag, scale", [("f32", 3.0e38, 1.0), ("f32", 3.0e38, -1.0), ("f32", 1.0e38, 2.5), ("f32", 1.0, 3.0e38), ("f32", 2.0 ** -100, 2.0 ** 127), ("bf16", 3.0e38, 1.0), ("bf16", 1.0, -3.0e38), ("f16", 60000.0, 5.0e33), ("f16", 1.0, 3.0e38)])
+@pytest.mark.parametrize("B, cols, S, heads, d", DEALT + OTHERS)
+def test_attend_with_scores_at_the_end_of_the_range(api, dtype, qmag, scale, B, cols, S, heads, d):
+    """Scores of up to some 2^126, from large queries or a large scale: the slots of the largest score share all the weight, by equal parts.  (One element of a
+    query is not zero, so a score is one product, rounded; the memory's values differ by 2^-11 of themselves or not at all, so that the slots that share
+    are those of the largest value.)"""
+    g = gen(S + d)
+    x = 0.25 * torch.rand(S, B, heads, -(-d // 32), 1, generator=g, device="cuda").expand(S, B, heads, -(-d // 32), 32).reshape(S, B, heads, -1)[..., :d]
+    u = torch.where(torch.rand(S, B, heads, d, generator=g, device="cuda") < 0.5, -1.0, 1.0)
+    m = api.memory4(B, S, d, heads=heads).pack((x * u).reshape(S, B, heads * d))
+    q = torch.zeros(B * cols, heads, d, device="cuda")
+    at = torch.randint(0, d, (B * cols, heads), generator=g, device="cuda")
+    q.scatter_(2, at[..., None], torch.where(torch.rand(B * cols, heads, 1, generator=g, device="cuda") < 0.5, -qmag, qmag))
+    q = q.to(ref.TYPES[dtype]).view(B * cols, heads * d)
+    ln = torch.full((B,), S, dtype=torch.int32, device="cuda")
+    out = m.attend(q, ln, scale=scale).double().view(B, cols, heads, d)
+    v = m.unpack().double()
+    z = torch.einsum("bchd,bshd->bchs", q.double().view(B, cols, heads, d), v) * scale
+    best = (z == z.amax(-1, keepdim=True)).double()
+    want = torch.einsum("bchs,bshd->bchd", best, v) / best.sum(-1, keepdim=True)
+    tol = (sum_tol(S) + 4 * EPS) * 0.25 + ref.HALF_STEP[dtype] * want.abs()
+    assert bool(((out - want).abs() <= tol).all())
+
+
 def test_attend_on_strided_queries_and_outputs(api):
     g = gen(11)
     B, cols, S, d = 3, 4, 45, 100

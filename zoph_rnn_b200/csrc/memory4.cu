@@ -417,7 +417,7 @@ __device__ __forceinline__ void attend_part(const Mem4Attend& a, const AttPlan& 
     for (int k = 0; k < GP; ++k) m = max(m, __float_as_uint(x[k]) & 0x7fffffffu);
     m = __reduce_max_sync(0xffffffffu, m);
     int e = 0;
-    if (m != 0) frexpf(__uint_as_float(m), &e);
+    if (m - 1u < 0x7f7fffffu) frexpf(__uint_as_float(m), &e);  // (neither zero nor an infinity or NaN)
     const float down1 = ldexpf(1.f, -(e / 2)), down2 = ldexpf(1.f, -(e - e / 2));
     const int el = lane & 7, tt = lane >> 3;
     // (the fragments of odd k-steps have neighbouring rows exchanged: the two k-steps that a warp writes at once fall on different banks)
@@ -429,7 +429,10 @@ __device__ __forceinline__ void attend_part(const Mem4Attend& a, const AttPlan& 
       *reinterpret_cast<__half*>(at + k * 2 * PARTS * 512) = x0;
       if (PARTS == 2) *reinterpret_cast<__half*>(at + k * 2 * PARTS * 512 + 512) = x1;
     }
-    const float fac = ldexpf(a.scale * 1.44269504f, e);  // (exponentials are powers of two)
+    // (exponentials are powers of two.)  Beyond the range of 32 bits the largest number does as well: scores that are finite all the same come from sums
+    // of less than 1, and two such sums that differ, by 2^-59 at least, are then 2^68 apart.
+    float fac = ldexpf(a.scale, e) * 1.44269504f;
+    if (fabsf(a.scale) < INFINITY) fac = fminf(fmaxf(fac, -3.4028234663852886e38f), 3.4028234663852886e38f);
     if constexpr (SOLO) {
       if (lane == 0) s_fac[r] = fac;
     } else {  // every team has a copy
