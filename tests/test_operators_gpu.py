@@ -387,6 +387,25 @@ def test_attend_with_scores_at_the_end_of_the_range(api, dtype, qmag, scale, B, 
     assert bool(((out - want).abs() <= tol).all())
 
 
+@pytest.mark.parametrize("dtype, small", [("f32", 2.0 ** -28), ("bf16", 2.0 ** -30), ("f16", 2.0 ** -26)])
+@pytest.mark.parametrize("B, cols, S, heads, d", DEALT + OTHERS)
+def test_attend_with_queries_of_very_different_elements(api, dtype, small, B, cols, S, heads, d):
+    """Elements far below their row's largest decide, where the memory is large: each counts with its type's precision."""
+    g = gen(d)
+    top = 32768.0 if dtype == "f16" else 1.0
+    q = torch.randn(B * cols, heads, d, generator=g, device="cuda") * (small * top)
+    q[..., :32] = top  # times memory values of up to 2e-6
+    amp = torch.full((d,), 2.0 ** 12, device="cuda")
+    amp[:32] = 2.0 ** -19
+    v = torch.tanh(torch.randn(S, B, heads, d, generator=g, device="cuda")) * amp
+    m = api.memory4(B, S, d, heads=heads).pack(v.view(S, B, heads * d))
+    q = q.to(ref.TYPES[dtype]).view(B * cols, heads * d)
+    ln = torch.full((B,), S, dtype=torch.int32, device="cuda")
+    scale = 4.0 / (small * top * 2.0 ** 12 * d ** 0.5)
+    out = m.attend(q, ln, scale=scale)
+    check_attend(out, ref.unpack(m.codes.cpu().numpy(), m.scales.cpu().numpy(), d), f64(q), [S] * B, [0] * B, scale, dtype)
+
+
 def test_attend_on_strided_queries_and_outputs(api):
     g = gen(11)
     B, cols, S, d = 3, 4, 45, 100

@@ -409,8 +409,9 @@ __device__ __forceinline__ void attend_part(const Mem4Attend& a, const AttPlan& 
         reinterpret_cast<unsigned short*>(s_team + k * Sh::STAGE + kAttTile * ROW)[cq * kAttTile + (p & 7) * 4 + (p >> 3)] = 0;
       }
 
-  // Q scaled by a power of two to at most 1; element e of a thread's word of 8 is half e / 4 of register 2 (e % 2) (+ 1: rows 8 .. 15) of k-step
-  // (e % 4) / 2, so that a word of codes gives its fragments by masks alone
+  // Q scaled by a power of two to the upper end of half precision, so that elements down to 2^-32 of the row's largest keep all their bits in bf16, and
+  // 22 bits down to 2^-28 of it in 32 bits (whose rounding to a half must not reach 2^16); element e of a thread's word of 8 is half e / 4 of register
+  // 2 (e % 2) (+ 1: rows 8 .. 15) of k-step (e % 4) / 2, so that a word of codes gives its fragments by masks alone
   auto lay_out_row = [&](int r, const float (&x)[GP]) {
     unsigned m = 0;
 #pragma unroll
@@ -418,6 +419,7 @@ __device__ __forceinline__ void attend_part(const Mem4Attend& a, const AttPlan& 
     m = __reduce_max_sync(0xffffffffu, m);
     int e = 0;
     if (m - 1u < 0x7f7fffffu) frexpf(__uint_as_float(m), &e);  // (neither zero nor an infinity or NaN)
+    e -= PARTS == 2 ? 15 : 16;
     const float down1 = ldexpf(1.f, -(e / 2)), down2 = ldexpf(1.f, -(e - e / 2));
     const int el = lane & 7, tt = lane >> 3;
     // (the fragments of odd k-steps have neighbouring rows exchanged: the two k-steps that a warp writes at once fall on different banks)
