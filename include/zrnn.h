@@ -408,8 +408,9 @@ int zrnn_memory4_unpack(int elem, const void* d_codes, const void* d_scales, int
  *   out = sum_s softmax_s(scale * q . v_s) v_s   over the slots offset <= s < offset + len of that source column
  * (slots outside the memory do not count; d_offset NULL: 0).  Whatever other slots hold is not looked at.  A column without
  * slots, or with d_mask01[c] == 0 (NULL: all 1), gets zeros.  d <= 1024.  d_out must not overlap d_q.  Scores have to stay below
- * 2^127.  An element of a query counts with its type's precision (22 bits in 32 bits) down to 2^-28 of the largest of its column and
- * head, and with steps of 2^-40 of that (2^-50 in 32 bits) below. */
+ * 2^127.  The weights go into their sums, and into those of the values, rounded to 22 bits (bf16: 11), and to steps of 2^-31 of the largest
+ * one beside them (32 bits: 2^-42).  An element of a query counts with its type's precision (22 bits in 32 bits) down to 2^-28 of
+ * the largest of its column and head, and with steps of 2^-40 of that (32 bits: 2^-50) below. */
 int zrnn_memory4_attend_workspace(int B, int cols_per_sentence, int S_cap, int heads, int d, size_t* bytes);
 int zrnn_memory4_attend(int elem, const void* d_codes, const void* d_scales, int B, int S_cap, int heads, int d, const int* d_len,
                         const int* d_offset, const void* d_q, long long ld_q, int cols_per_sentence, const int* d_mask01, float scale,

@@ -406,6 +406,53 @@ def test_attend_with_queries_of_very_different_elements(api, dtype, small, B, co
     check_attend(out, ref.unpack(m.codes.cpu().numpy(), m.scales.cpu().numpy(), d), f64(q), [S] * B, [0] * B, scale, dtype)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("cols, d, teams", [(3, 264, 0), (1200, 1000, 2), (1200, 264, 4), (1200, 100, 16)])
+@pytest.mark.parametrize("peak", [0, 100001])
+def test_attend_to_one_large_weight_and_a_long_flat_tail(api, dtype, cols, d, teams, peak):
+    """One slot, and 2^19 others whose weights of 2^-25.5 of its are, together, 2^-6.5 of the whole.  1200 columns: the window is one CTA's, whose teams of
+    warps have an equal share of the slots each; 3: it is shared by many.
+
+    Tolerance.  out = v0 (1 - tail) / (1 + tail), since the others' values are the negative one's.  A score's error of t changes a tail weight by a factor 1 + t, out by
+    2 tail t.  The team that has the large weight adds its share of the tail to it: in 16 bits by tensor-core additions of 16 slots, cut off (2 eps of the sums
+    each), in 32 bits by additions of 32 slots, rounded (eps); numerator and denominator alike.  16-bit types have weights in steps of 2^-31 of the
+    largest: half a step is 2^-6.5 of a tail weight.  A window that many share has none of that: their sums are added in a few hundred roundings."""
+    S = 1 << 19
+    assert (attend_ways(api, 1, cols, S, 1, d) == 0) == (teams > 0)
+    g = gen(d)
+    u = torch.where(torch.rand(d, generator=g, device="cuda") < 0.5, -0.5, 0.5)
+    m = api.memory4(1, S, d)
+    m.pack((-u).expand(S, 1, d))
+    m.pack(u.expand(1, 1, d), slot0=peak)
+    v = m.unpack(slot0=peak, S=1).double().view(d)
+    q = (u * 2).to(ref.TYPES[dtype]).repeat(cols, 1)
+    scale = 12.75 * np.log(2.0) / float((q[0].double() * v).sum())  # scores of +-12.75 log 2
+    out = m.attend(q, torch.full((1,), S, dtype=torch.int32, device="cuda"), scale=scale).double()
+    tail = (S - 1) * 2.0 ** -25.5
+    want = v * ((1 - tail) / (1 + tail))
+    share = S / teams if teams else 0
+    cut = 2 * (share / 16 * 2 * EPS if dtype != "f32" else share / 32 * EPS) + 512 * EPS
+    step = 2 * tail * (1 / teams if teams else 2.0 ** -6) * (2.0 ** -6.5 if dtype != "f32" else 2.0 ** -17.5)
+    tol = float(v.abs().max()) * (2 * tail * 2 * sum_tol(d) * 13 + cut + step) + ref.HALF_STEP[dtype] * want.abs()
+    err = (out - want).abs()
+    assert bool((err <= tol).all()), (float(err.max()), float((err / tol).max()))
+
+
+@pytest.mark.parametrize("B, cols, S, heads, d", DEALT + OTHERS)
+def test_attend_in_fp16_is_rounded_once(api, B, cols, S, heads, d):
+    """Beside the result's rounding to fp16 there are only those of 32 bits: few slots of comparable weights, where a weight's rounding to a half would show."""
+    g = gen(7 * d)
+    m = api.memory4(B, S, d, heads=heads).pack(torch.tanh(torch.randn(S, B, heads * d, generator=g, device="cuda")))
+    q = (0.1 * torch.randn(B * cols, heads * d, generator=g, device="cuda")).half()
+    v = ref.unpack(m.codes.cpu().numpy(), m.scales.cpu().numpy(), d)
+    for n in (2, 3, 7):
+        lens, offs = [n] * B, [(b * 17) % (S - n) for b in range(B)]
+        out = m.attend(q, torch.tensor(lens, dtype=torch.int32, device="cuda"), torch.tensor(offs, dtype=torch.int32, device="cuda"), scale=d ** -0.5)
+        want, mag = ref.attend(v, f64(q), lens, offs, d ** -0.5)
+        tol = np.abs(v).max() * (2 * sum_tol(d) * mag + 4 * sum_tol(n))[..., None] + ref.HALF_STEP["f16"] * np.abs(want) + 2.0 ** -25  # (half a step of its subnormals)
+        assert (np.abs(f64(out).reshape(want.shape) - want) <= tol).all()
+
+
 def test_attend_on_strided_queries_and_outputs(api):
     g = gen(11)
     B, cols, S, d = 3, 4, 45, 100

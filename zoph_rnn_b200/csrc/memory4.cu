@@ -264,20 +264,26 @@ __global__ void __launch_bounds__(256, kMem4PerSm) mem4_unpack_kernel(const Mem4
 // with a CTA each 200).  WHOLE: a CTA has a source column.  DEALT: where there are fewer of those than multiprocessors, several CTAs, more for
 // longer ones, and a second launch that combines them.
 //
-// What bounds it is the issue of instructions, not memory (16 x 12 columns, 4000 .. 8192 slots of 1024 in bf16: 52 us, 1.1 TB/s; 40 of them the
+// What bounds it is the issue of instructions, not memory (16 x 12 columns, 4000 .. 8192 slots of 1024 in bf16: 53 us, 1.1 TB/s; 40 of them the
 // slots', the rest the start, the teams' and the parts' sums and the combination).  Per 64 slots x 1024 elements a quarter of a
 // multiprocessor has 264 tensor instructions of 8 cycles, 1024 half-precision and some 1300 integer ones of 2 each (a word of 8 codes takes 13
 // instructions to become 4 pairs of halves, twice: the scores need pairs of elements, the output pairs of slots; kept between the two, they
 // would take 64 registers more), in all some 4000, and takes 5500 cycles: four warps do not fill the rest.
 constexpr int kAttWarps = 16, kAttTile = 32, kAttStages = 3, kAttPartLd = 40;
 enum { ALONE, WHOLE, DEALT };  // a warp per column tile and head; a CTA; several CTAs
-template <int PARTS, int WT, int NB, bool SOLO>
+// In 32 bits the weights are a half and 2^11 times the rest as another, in fp16 a half and the rest as it is (the result's 2^-12 would show the half
+// alone; 32 x 5 columns, 8 heads of 64, up to 1500 slots: 18.2 us, without the rests 16.0), in bf16 a half, whose 2^-12 is an eighth of the
+// result's 2^-9.
+template <class T> struct AttParts { static constexpr int Q = 1, W = 1; };
+template <> struct AttParts<float> { static constexpr int Q = 2, W = 2; };
+template <> struct AttParts<__half> { static constexpr int Q = 1, W = 2; };
+template <int PARTS, int W_PARTS, int WT, int NB, bool SOLO>
 struct AttShape {
   static constexpr int WARPS = SOLO ? 8 : kAttWarps, TEAMS = WARPS / WT, GP = 2 * NB * WT;  // groups that the team's warps have room for
   static constexpr int ROW = (GP | 1) * 16;                       // bytes of a slot's codes in shared memory: an odd number of 16 spreads them over the banks
   static constexpr int Q = GP * 2 * PARTS * 512;                  // Q as fragments
   static constexpr int STAGE = kAttTile * ROW + GP * kAttTile * 2;
-  static constexpr int PART = WT == 1 ? 0 : WT * 16 * kAttPartLd * 4, W = WT == 1 ? 0 : 2 * PARTS * 512;  // partial scores, weights: a warp alone keeps them
+  static constexpr int PART = WT == 1 ? 0 : WT * 16 * kAttPartLd * 4, W = WT == 1 ? 0 : 2 * W_PARTS * 512;  // partial scores, weights: a warp alone keeps them
   static constexpr int TEAM = kAttStages * STAGE + PART + W + 192 + (SOLO ? Q : 0);
   static constexpr int OUT_LD = GP * 32 + 2;                      // floats; the teams' outputs take the place of all that
   static constexpr int RUN = (SOLO ? 0 : Q) + TEAMS * TEAM, OUT = SOLO ? 0 : TEAMS * 16 * OUT_LD * 4;
@@ -311,13 +317,14 @@ __device__ __forceinline__ float warp_max(float x) {
   asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
   return y;
 }
-// What a row's weights are relative to: a maximum that is followed only once it has risen by 2^8, so that sums are seldom rescaled (weights of
-// up to 256 are as good in half precision as those of up to 1)
+// What a row's weights are relative to: a maximum that is followed only once it has risen by 2^8, so that sums are seldom rescaled.  The weights are
+// 2^7 times what they are relative to that: of up to 2^15 they use all of half precision, whose steps of 2^-24 are 2^-31 of the reference.
 __device__ __forceinline__ float risen(float before, float now) { return now > before + 8.f ? now : before; }
-// x as a half and, times 2^11, what that leaves
-__device__ __forceinline__ void split_half(float x, __half& hi, __half& lo) {
+__device__ __forceinline__ float weight(float z, float ref) { return exp2_approx(z - ref + 7.f); }
+// x as a half and, times `up`, what that leaves
+__device__ __forceinline__ void split_half(float x, float up, __half& hi, __half& lo) {
   hi = __float2half_rn(x);
-  lo = __float2half_rn((x - __half2float(hi)) * 2048.f);
+  lo = __float2half_rn((x - __half2float(hi)) * up);
 }
 __device__ __forceinline__ uint32_t shared_at(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void copy16(void* dst, const void* src) {
@@ -327,8 +334,9 @@ __device__ __forceinline__ void copy16(void* dst, const void* src) {
 // Tiles t0 .. t1 - 1 of source column b (t1 < 0: all of them) for the columns from c0 on and head h.  w: where the sums go, if the column has others
 template <class T, int WT, int NB, bool SOLO>
 __device__ __forceinline__ void attend_part(const Mem4Attend& a, const AttPlan& pl, unsigned char* smem, int b, int c0, int h, int t0, int t1, float* w) {
-  constexpr int PARTS = std::is_same<T, float>::value ? 2 : 1, ROWS = 16 / WT;
-  using Sh = AttShape<PARTS, WT, NB, SOLO>;
+  constexpr int PARTS = AttParts<T>::Q, W_PARTS = AttParts<T>::W, ROWS = 16 / WT;
+  constexpr float W_UP = PARTS == 2 ? 2048.f : 1.f;
+  using Sh = AttShape<PARTS, W_PARTS, WT, NB, SOLO>;
   static_assert(!SOLO || WT == 1, "");
   constexpr int TEAMS = Sh::TEAMS, GP = Sh::GP, ROW = Sh::ROW;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, team = warp / WT, wt = warp % WT;
@@ -427,7 +435,7 @@ __device__ __forceinline__ void attend_part(const Mem4Attend& a, const AttPlan& 
 #pragma unroll
     for (int k = 0; k < GP; ++k) {
       __half x0, x1;
-      split_half(x[k] * down1 * down2, x0, x1);
+      split_half(x[k] * down1 * down2, 2048.f, x0, x1);
       *reinterpret_cast<__half*>(at + k * 2 * PARTS * 512) = x0;
       if (PARTS == 2) *reinterpret_cast<__half*>(at + k * 2 * PARTS * 512 + 512) = x1;
     }
@@ -523,7 +531,7 @@ __device__ __forceinline__ void attend_part(const Mem4Attend& a, const AttPlan& 
     // softmax: row r of this warp, slot `lane`; as the second product's k, slot 8 j + c is half j % 2 of register 2 (j / 2) (+ 1: rows 8 .. 15) of lane
     // c / 2 (of a row's four), k-step c % 2, so that a thread's four scales lie side by side
     {
-      unsigned char* at0 = s_w + (lane & 1) * PARTS * 512 + (lane & 7) / 2 * 16 + (lane >> 4) * 8 + (lane >> 3 & 1) * 2;
+      unsigned char* at0 = s_w + (lane & 1) * W_PARTS * 512 + (lane & 7) / 2 * 16 + (lane >> 4) * 8 + (lane >> 3 & 1) * 2;
       constexpr int RC = ROWS < 4 ? ROWS : 4;  // rows side by side: one's latency is another's work
       for (int r0 = wt * ROWS; r0 < (wt + 1) * ROWS && r0 < n_cols; r0 += RC) {
         float z[RC], m_old[RC];
@@ -540,53 +548,44 @@ __device__ __forceinline__ void attend_part(const Mem4Attend& a, const AttPlan& 
         for (int rr = 0; rr < RC; ++rr) {
           const int r = r0 + rr;
           const float m_new = risen(m_old[rr], warp_max(z[rr])), ref = m_new == -INFINITY ? 0.f : m_new;
-          const float alpha = exp2_approx(m_old[rr] - ref), p = exp2_approx(z[rr] - ref);
+          const float alpha = exp2_approx(m_old[rr] - ref), p = weight(z[rr], ref);
           if (lane == 0) {
             s_alpha[r] = alpha;
             s_m[r] = m_new;
           }
           __half p0h, p1h;
-          split_half(p, p0h, p1h);
+          split_half(p, W_UP, p0h, p1h);
           unsigned char* at = at0 + (r & 7) * 64 + (r >> 3) * 4;
           *reinterpret_cast<__half*>(at) = p0h;
-          if (PARTS == 2) *reinterpret_cast<__half*>(at + 512) = p1h;
+          if (W_PARTS == 2) *reinterpret_cast<__half*>(at + 512) = p1h;
         }
       }
     }
   };
-  auto output = [&](int it, const uint4 (&w)[2][PARTS], float al0, float al1) {
+  // onto the sums with the weights' rests those with their large parts
+  auto add_large_parts = [&](float (&y)[4], const uint4 (&w)[2][W_PARTS], uint32_t b0, uint32_t b1, uint32_t b2, uint32_t b3) {
+    if (W_PARTS == 1) return;
+    if (W_UP != 1.f)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) y[u] *= 1.f / W_UP;
+    mma_f16(y, w[0][0], b0, b1);
+    mma_f16(y, w[1][0], b2, b3);
+  };
+  auto output = [&](int it, const uint4 (&w)[2][W_PARTS], float al0, float al1) {
     const unsigned char* st = stage_at(it);
     const unsigned char* s_sc = st + kAttTile * ROW;
     // weights x values: n-tile j of a block has element 8 c + j of the block in its column c
     {
-      // With 16-bit operands the products go straight onto the accumulators, which are rescaled where a maximum rose.  The tensor core cuts its
-      // sums off: 2^-23 per tile, which 32 bits of result would show, so those add the tile's sums in the ordinary way.
-      if (PARTS == 1 && __any_sync(0xffffffffu, al0 != 1.f || al1 != 1.f)) {
-#pragma unroll
-        for (int x = 0; x < NB; ++x)
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-#pragma unroll
-            for (int u = 0; u < 4; ++u) acc[x][j][u] *= u < 2 ? al0 : al1;
-#pragma unroll
-        for (int u = 0; u < 4; ++u) l[u] *= u < 2 ? al0 : al1;
-      }
+      // A tile's sums are added to the earlier ones in the ordinary way.  Straight onto the accumulators the tensor core would cut off what is below 2^-24 of
+      // them, of every product: a window's many small weights beside a large one would be lost (1 us less of 53).
       {
         constexpr uint32_t ones = 0x3c003c00u;
-        if (PARTS == 1) {
-          mma_f16(l, w[0][0], ones, ones);
-          mma_f16(l, w[1][0], ones, ones);
-        } else {
-          float y[4];
-          mma_f16_first(y, w[0][PARTS - 1], ones, ones);
-          mma_f16(y, w[1][PARTS - 1], ones, ones);
+        float y[4];
+        mma_f16_first(y, w[0][W_PARTS - 1], ones, ones);
+        mma_f16(y, w[1][W_PARTS - 1], ones, ones);
+        add_large_parts(y, w, ones, ones, ones, ones);
 #pragma unroll
-          for (int u = 0; u < 4; ++u) y[u] *= 1.f / 2048.f;
-          mma_f16(y, w[0][0], ones, ones);
-          mma_f16(y, w[1][0], ones, ones);
-#pragma unroll
-          for (int u = 0; u < 4; ++u) l[u] = fmaf(l[u], u < 2 ? al0 : al1, y[u]);
-        }
+        for (int u = 0; u < 4; ++u) l[u] = fmaf(l[u], u < 2 ? al0 : al1, y[u]);
       }
 #pragma unroll
       for (int x = 0; x < NB; ++x) {
@@ -617,20 +616,12 @@ __device__ __forceinline__ void attend_part(const Mem4Attend& a, const AttPlan& 
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             float (&o)[4] = acc[x][half * 4 + j];
-            if (PARTS == 1) {
-              mma_f16(o, w[0][0], v[0][0][j], v[0][1][j]);
-              mma_f16(o, w[1][0], v[1][0][j], v[1][1][j]);
-            } else {
-              float y[4];
-              mma_f16_first(y, w[0][PARTS - 1], v[0][0][j], v[0][1][j]);
-              mma_f16(y, w[1][PARTS - 1], v[1][0][j], v[1][1][j]);
+            float y[4];
+            mma_f16_first(y, w[0][W_PARTS - 1], v[0][0][j], v[0][1][j]);
+            mma_f16(y, w[1][W_PARTS - 1], v[1][0][j], v[1][1][j]);
+            add_large_parts(y, w, v[0][0][j], v[0][1][j], v[1][0][j], v[1][1][j]);
 #pragma unroll
-              for (int u = 0; u < 4; ++u) y[u] *= 1.f / 2048.f;
-              mma_f16(y, w[0][0], v[0][0][j], v[0][1][j]);
-              mma_f16(y, w[1][0], v[1][0][j], v[1][1][j]);
-#pragma unroll
-              for (int u = 0; u < 4; ++u) o[u] = fmaf(o[u], u < 2 ? al0 : al1, y[u]);
-            }
+            for (int u = 0; u < 4; ++u) o[u] = fmaf(o[u], u < 2 ? al0 : al1, y[u]);
           }
         }
       }
@@ -645,7 +636,7 @@ __device__ __forceinline__ void attend_part(const Mem4Attend& a, const AttPlan& 
       const int n = slots_left(it);
       float z[PARTS][4][4];
       scores(it, z);
-      uint4 w[2][PARTS];
+      uint4 w[2][W_PARTS];
       float al0, al1;
       // The scores lie as the weights have to: half u % 2 of register 2 (j % 2) (+ 1: rows 8 .. 15) of k-step j / 2 is slot 8 j + 2 t + u % 2
       float m[2] = {-INFINITY, -INFINITY};
@@ -674,16 +665,16 @@ __device__ __forceinline__ void attend_part(const Mem4Attend& a, const AttPlan& 
 #pragma unroll
         for (int k = 0; k < 4; ++k) {  // register k: n-tile 2 s + k / 2, rows of half k % 2
           const int j = 2 * s + (k >> 1), r = k & 1;
-          const float p0 = exp2_approx(z[0][j][2 * r] - ref[r]), p1 = exp2_approx(z[0][j][2 * r + 1] - ref[r]);
+          const float p0 = weight(z[0][j][2 * r], ref[r]), p1 = weight(z[0][j][2 * r + 1], ref[r]);
           const __half2 h = __floats2half2_rn(p0, p1);
           hi[k] = h2_bits(h);
-          if (PARTS == 2) {
+          if (W_PARTS == 2) {
             const float2 f = __half22float2(h);
-            lo[k] = h2_bits(__floats2half2_rn((p0 - f.x) * 2048.f, (p1 - f.y) * 2048.f));
+            lo[k] = h2_bits(__floats2half2_rn((p0 - f.x) * W_UP, (p1 - f.y) * W_UP));
           }
         }
         w[s][0] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        if (PARTS == 2) w[s][PARTS - 1] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        if (W_PARTS == 2) w[s][W_PARTS - 1] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
       }
       output(it, w, al0, al1);
       keep_scales(it + 2);
@@ -707,12 +698,12 @@ __device__ __forceinline__ void attend_part(const Mem4Attend& a, const AttPlan& 
       team_sync();  // tile it + 1 is there for all, and tile it's weights
       if (it + 1 < my) next_scores(it + 1);
       {
-        uint4 w[2][PARTS];
+        uint4 w[2][W_PARTS];
         float al0, al1;
 #pragma unroll
       for (int s = 0; s < 2; ++s)
 #pragma unroll
-        for (int x = 0; x < PARTS; ++x) w[s][x] = *reinterpret_cast<const uint4*>(s_w + (s * PARTS + x) * 512 + lane * 16);
+        for (int x = 0; x < W_PARTS; ++x) w[s][x] = *reinterpret_cast<const uint4*>(s_w + (s * W_PARTS + x) * 512 + lane * 16);
       al0 = s_alpha[g];
       al1 = s_alpha[g + 8];
         output(it, w, al0, al1);
@@ -1016,7 +1007,7 @@ AttPlan att_plan(int B, int cols, int S_cap, int heads, int d) {
 template <class T, int WT, int NB, int HOW>
 cudaError_t attend_launch(const Mem4Attend& a, const AttPlan& pl, cudaStream_t st) {
   constexpr bool SOLO = HOW == ALONE;
-  using Sh = AttShape<std::is_same<T, float>::value ? 2 : 1, WT, NB, SOLO>;
+  using Sh = AttShape<AttParts<T>::Q, AttParts<T>::W, WT, NB, SOLO>;
   constexpr int smem = Sh::SMEM;
   static bool configured[64] = {false};
   int dev = 0;
