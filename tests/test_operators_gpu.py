@@ -993,6 +993,23 @@ def test_linear_long_products_with_a_residual(api, dtype, n, K, N):
     linear_case(api, dtype, n, K, N, "relu", residual=True, pad=(0, 0, 1, 3), seed=8)
 
 
+@pytest.mark.parametrize("N", [32, 64, 96, 200])
+def test_linear_in_32_bits_with_weights_from_far_memory(api, N):
+    """One tile per multiprocessor, weights beyond the L2's size that come out of order: every call gives the same, and what it should."""
+    g = gen(N)
+    n, K = 18944, 2048
+    W = [randn(g, n, K) * K ** -0.5 for _ in range(2)]
+    X = randn(g, N, K)
+    want = [X.double() @ w.double().t() for w in W]
+    mag = [X.double().abs() @ w.double().abs().t() for w in W]
+    first = [api.linear(w, X) for w in W]
+    for a, b, m in zip(first, want, mag):
+        assert bool(((a.double() - b).abs() <= sum_tol(K) * m).all())
+    for _ in range(20):
+        for w, a in zip(W, first):
+            assert torch.equal(api.linear(w, X), a)
+
+
 def test_many_sentences(api):
     """More sentences than a grid's dimension holds."""
     g = gen(40)

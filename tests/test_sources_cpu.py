@@ -127,3 +127,15 @@ def test_the_selection_is_whole_warps_at_its_aligned_cluster_barriers():
     lines = [ln.strip() for ln in s.splitlines() if ln.strip()]
     at = [i for i, ln in enumerate(lines) if "barrier.cluster" in ln and ".aligned" in ln]
     assert len(at) == 2 and all(lines[i - 1] == "__syncwarp();" for i in at)
+
+
+def test_a_splitting_team_waits_until_a_stages_last_round_is_used_up():
+    """The teams of the 32-bit product take the k-blocks in turn, so a stage of the ring has another user every round.  A wait for a copy by its parity is
+    answered at once while the copy before is still on its way (tests/test_ring_cpu.py)."""
+    s = body("linear.cu", "const int team = (warp - kSplitWarp0)", "if (CUT && warp >= kEpiWarps)")
+    order = re.findall(r"mbar_wait_warp\(&ct\.(\w+)\[st\], ([^,]*),", s)
+    assert order == [("empty", "ph ^ 1u"), ("full", "ph")], order
+    # what that wait relies on: a ring of no fewer stages than teams
+    launch = body("linear.cu", "cudaError_t lin_launch(", "cudaLaunchKernelEx")
+    assert "(512 - 4 * p.nb) / 32" in launch and re.search(r"return mode == LIN_F32 \? 96", body("linear.cu", "lin_max_nb(", "\n"))
+    assert (512 - 4 * 96) // 32 >= 3 and "kSplitTeams = 3" in body("linear.cu", "constexpr int kEpiWarps", ";")

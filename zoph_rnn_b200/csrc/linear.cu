@@ -351,7 +351,10 @@ __global__ void __launch_bounds__(lin_threads(MODE), 1) linear_tc_kernel(const _
     if (BULK && p.bulk && one) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   } else if (F32) {
     // ------------------------------------------------------------ the lo parts of a stage: what tf32 cuts off of the tile beside it
-    // Teams of four warps take the k-blocks in turn: one's waits are filled by the others.
+    // Teams of four warps take the k-blocks in turn: one's waits are filled by the others.  A stage's next user may be another team, and copies may arrive out
+    // of order: a team waits until the MMAs have used up the stage's last round before it asks for its own copy.  (While that copy ahead is still on its way,
+    // the barrier would answer the question for the next one's parity with yes.  The round before that is used up: the team has seen the copy
+    // of kSplitTeams k-blocks ago, and copies are requested in order, the stage's last one when the round before it was used up.)
     const int team = (warp - kSplitWarp0) / kSplitWarps, me = (warp - kSplitWarp0) % kSplitWarps * 32 + lane;
     const int wv = w_bytes / 16, xv = x_bytes / 16, row = 32 * (warp & 3) + lane;  // (a warp reaches the lanes of tensor memory that its number gives)
     const uint32_t w_lo = tmem_base + 2u * acc + ((uint32_t)(row & ~31) << 16);
@@ -360,6 +363,7 @@ __global__ void __launch_bounds__(lin_threads(MODE), 1) linear_tc_kernel(const _
     int st = team % p.stages;
     uint32_t ph = (uint32_t)(team / p.stages) & 1u;
     for (long long it = team; it < its && sound; it += kSplitTeams) {
+      if (!mbar_wait_warp(&ct.empty[st], ph ^ 1u, &ct.abort, p.a.err, 6)) break;
       if (!mbar_wait_warp(&ct.full[st], ph, &ct.abort, p.a.err, 6)) break;
       uint4* tiles = reinterpret_cast<uint4*>(lin_smem + (size_t)st * stage);
       tc_fence_after();
