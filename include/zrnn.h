@@ -418,8 +418,11 @@ int zrnn_memory4_attend(int elem, const void* d_codes, const void* d_scales, int
 
 /* Y = act(W X + b) + R for n_cols columns: X (K x n_cols), Y and R (n_rows x n_cols) column-major as all activations; the K
  * weights of an output are contiguous and those of the next ldw further (W^T column-major).  d_bias (n_rows, fp32) and
- * d_residual may be NULL; d_residual may be d_Y itself (with ldr == ldy).  ZRNN_ELEM_F32 is accurate to fp32 (3xTF32; an
- * infinity among its operands makes NaN), the 16-bit types multiply their operands as they are.  gelu is x/2 (1 + erf(x / sqrt 2)), silu x / (1 + exp -x). */
+ * d_residual may be NULL; d_residual may be d_Y itself (with ldr == ldy).  ZRNN_ELEM_F32 is 3xTF32:
+ * every product within 2^-20 of itself (1.2e-7 on the average, without a side), its sums cut off now and then by the tensor core (together some
+ * 3.5e-7 of the root of the sum of the products' squares; 6e-7 too small where all products are positive; a sum in plain fp32 is off by
+ * 4e-7 over 512 of them).  An infinity among its operands may make NaN.  The 16-bit types multiply their operands as they are and add in
+ * the tensor core.  gelu is x/2 (1 + erf(x / sqrt 2)), silu x / (1 + exp -x). */
 typedef enum {
   ZRNN_ACT_NONE = 0, ZRNN_ACT_TANH = 1, ZRNN_ACT_SIGMOID = 2, ZRNN_ACT_RELU = 3, ZRNN_ACT_GELU = 4, ZRNN_ACT_SILU = 5
 } zrnn_activation;

@@ -570,6 +570,53 @@ def test_linear_in_32_bits_of_wide_ranges(api):
         assert bool(((out - want).abs() <= sum_tol(K) * mag).all())
 
 
+@pytest.mark.parametrize("N", [6, 3000])  # the kernel for few columns, the one on tcgen05
+@pytest.mark.parametrize("K", [8, 32, 128, 512, 2000])
+def test_linear_in_32_bits_beside_a_plain_product(api, N, K):
+    """Errors of single operands' splitting, which a sum's tolerance hides: the root of the mean square and the mean, signed error, of results relative to the root of the
+    sum of the products' squares (random signs) or to the result (positive operands), and next to a product in ordinary 32-bit arithmetic, step by step.
+
+    Bounds.  An operand's hi + lo is off by 2^-22 at most, 0.8e-7 on the average and to either side; what a product leaves out, lo lo, is 0.8e-7 on the average
+    and has no side: 1.2e-7 together, 2^-22 with a factor of two in hand, and a mean of 2^-24.  A tensor-core instruction cuts a sum off, by 2^-23 of what there is
+    of it at most: of m of them in a row, (m + 1) / 2 times that.  The additions in 32 bits: 2^-23.  Operands just below 1 + 2^-10 all have the same hi and lo as
+    large as it gets: off by 2^-22, all to one side."""
+    g = gen(K + N)
+    n = 1000
+    m = min(16, -(-K // 8)) if N > 100 else min(8, 2 * -(-K // 128))
+    cut = (m + 1) / 2 * 2.0 ** -23
+    u = lambda *s: torch.rand(s, generator=g, device="cuda")  # noqa: E731
+    below = lambda *s: 1 + 2.0 ** -10 - 2.0 ** -23 * torch.randint(1, 9, s, generator=g, device="cuda").float()  # noqa: E731
+    for kind, make, one_side in (("signs", lambda *s: randn(g, *s), 2.0 ** -24), ("positive", lambda *s: 1 + u(*s), 2.0 ** -24), ("below", below, 2.0 ** -22 + 2.0 ** -24)):
+        W, X = make(n, K), make(N, K)
+        want = X.double() @ W.double().t()
+        scale = want.abs() if kind != "signs" else ((X.double() ** 2) @ (W.double() ** 2).t()).sqrt()
+        plain = torch.zeros(N, n, device="cuda")
+        for k in range(K):
+            plain += X[:, k:k + 1] * W[:, k]
+        err, ours = [(y.double() - want) * want.sign() / scale for y in (plain, api.linear(W, X))]
+        mean, rms = float(ours.mean()), float(ours.square().mean().sqrt())
+        of_plain = float(err.mean()), float(err.square().mean().sqrt())
+        assert abs(mean) <= one_side + cut, (kind, mean, rms, of_plain)
+        assert rms <= 2.0 ** -22 + cut + 2.0 ** -23 + (one_side if kind == "below" else 0), (kind, mean, rms, of_plain)
+        if kind == "signs" and K >= 512:  # (a plain sum's errors grow with its length)
+            assert rms <= 2 * of_plain[1], (rms, of_plain)
+
+
+@pytest.mark.parametrize("N", [6, 300])
+def test_linear_in_32_bits_of_the_largest_numbers(api, N):
+    """Operands next to the largest number do not round to an infinity on the way."""
+    g = gen(N)
+    top = torch.tensor([0x7f7fffff, 0x7f7ff000, 0x7f7fefff, 0x7f7fe000], dtype=torch.int32).view(torch.float32).cuda()
+    W = (2.0 ** -20 * torch.rand(200, 64, generator=g, device="cuda"))
+    X = torch.zeros(N, 64, device="cuda")
+    X[:, 5] = top[torch.arange(N, device="cuda") % 4]
+    X[1::2] *= -1
+    for a, b in ((W, X), (X, W)):
+        want = b.double() @ a.double().t()
+        out = api.linear(a, b)
+        assert bool(((out.double() - want).abs() <= sum_tol(64) * want.abs()).all())
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("N", [6, 200])
 def test_linear_numbers_that_are_not_finite(api, dtype, N):

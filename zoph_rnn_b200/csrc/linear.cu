@@ -6,18 +6,21 @@
 // through bias, activation and residual while the next tile's MMAs run; persistent.
 //
 // 32-bit operands go as two tf32 parts each and three products (hi hi; hi lo and lo hi into an accumulator of their own).  The tensor cores
-// ignore the bits below tf32, so the tile that TMA brought is the hi part as it is; three teams of four warps make the lo parts of the stages
-// (one team alone: a product took 1.7 times as long): the columns' beside the hi part in shared memory, so that W's hi part is read once for
-// both, the outputs' in tensor memory, which is an operand as well.  A tensor-core accumulator cuts its sums off, so the products of four
-// k-blocks (16 additions) go into a fresh pair, two pairs in turn, and the sixteen warps add those up in ordinary 32-bit arithmetic.
-// What bounds it is shared memory: per k-block of 128 x 96 the TMA writes, the splitting's reads and writes and the MMAs' reads are 120 KB,
-// 940 cycles at 128 bytes each, of 1020 measured (with both lo parts in shared memory 152 KB, with pairs of CTAs 1190 cycles), for MMAs of
+// ignore the bits below tf32, so the outputs' tile that TMA brought is their hi part as it is; three teams of four warps make the rest of the stages
+// (one team alone: a product took 1.7 times as long): the columns' hi, rounded, in the tile's place and lo beside it in shared memory, so that W's hi part is
+// read once for both, the outputs' lo in tensor memory, which is an operand as well.  Rounding hi of one of the factors is what keeps the left-out lo lo
+// without a side (linear_device.cuh); it costs 8 % (1000 x 2000 x 768: 23.6 us, with both cut off 21.9), lo lo as a fourth product 18 %.  A
+// tensor-core accumulator cuts its sums off, so the products of four k-blocks (16 additions) go into a fresh pair, two pairs in turn, and the
+// sixteen warps add those up in ordinary 32-bit arithmetic: sums of positive products come out 6e-7 of themselves too small (fresh pairs every two
+// k-blocks: 2.2e-7, for 4 to 13 % more time).
+// What bounds it is shared memory: per k-block of 128 x 96 the TMA writes, the splitting's reads and writes and the MMAs' reads are 132 KB,
+// 1060 cycles at 128 bytes each, of 1110 measured (with both lo parts in shared memory, or with pairs of CTAs, 170 to 250 more), for MMAs of
 // 580.
 //
 // Long products of few tiles: 2, 4 or 8 CTAs of a cluster share a tile's K axis and exchange their sums through distributed shared memory.
 // 16-bit outputs and residuals of whole tiles go through shared memory and TMA.  us, this kernel / the library's product alone: bf16 16384 x
 // 4096 x 4096 350 / 337, 4096 x 4096 x 512 20 / 15, 512 x 8192 x 512 18 / 17, 1000 x 1000 x 64 7.8 / 4.7; fp32 16384 x 4096 x 4096
-// 2700 / 8400 (FMA), 1000 x 2000 x 768 23 / 83.
+// 2850 / 8400 (FMA), 1000 x 2000 x 768 23.6 / 83.
 //
 // A CTA asks for all of an SM's shared memory, so that a pair's allocation of tensor memory waits for nobody that could wait for it in turn.
 #include <algorithm>
@@ -380,7 +383,10 @@ __global__ void __launch_bounds__(lin_threads(MODE), 1) linear_tc_kernel(const _
 #pragma unroll 2
       for (int e = wv + me; e < wv + xv; e += kSplitWarps * 32) {
         const uint4 x = tiles[e];
-        tiles[xv + e] = make_uint4(tf32_rest(x.x), tf32_rest(x.y), tf32_rest(x.z), tf32_rest(x.w));
+        uint4 hi, lo;
+        split_tf32(x.x, hi.x, lo.x); split_tf32(x.y, hi.y, lo.y); split_tf32(x.z, hi.z, lo.z); split_tf32(x.w, hi.w, lo.w);
+        tiles[e] = hi;
+        tiles[xv + e] = lo;
       }
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -431,8 +437,8 @@ LinPlan lin_plan(const LinearArgs& a, int elem) {
   const long long rows1 = (a.n + 127) / 128, rows2 = (a.n + 255) / 256;
   // The time of a launch in ns, as measured with all multiprocessors at work: a start and an end (4 us, with a cut 6), and for the busiest unit's
   // tiles the k-blocks or the epilogue, whichever takes longer.  A k-block of 16-bit operands takes a pair the MMAs' time, a CTA that of
-  // its shared memory (450 ns with 224 columns), but no less than 200 ns (its way from the L2); of 32 bits what shared memory lets through: 346 / 426 /
-  // 539 ns with 32 / 64 / 96 columns (a pair, with twice the rows on two multiprocessors, 511 / 533 / 627, so there are none).
+  // its shared memory (450 ns with 224 columns), but no less than 200 ns (its way from the L2); of 32 bits what shared memory lets through: 583 ns
+  // with 96 columns, 3.5 less per column (a pair, with twice the rows on two multiprocessors, took some 90 ns more than a CTA, so there are none).
   double best = 0;
   const bool f32 = elem == ELEM_F32;
   for (int cg = 1; cg <= (f32 ? 1 : 2); ++cg)
@@ -440,7 +446,7 @@ LinPlan lin_plan(const LinearArgs& a, int elem) {
       const int n_ct = (a.N - 1) / w + 1, nb = ((a.N - 1) / n_ct + 32) / 32 * 32;
       if ((long long)nb * (n_ct - 1) >= a.N) continue;
       const long long tiles = (cg == 2 ? rows2 : rows1) * n_ct;
-      const double block = f32 ? 250 + 3.0 * nb : cg == 2 ? std::max(200.0, 1.1 * nb) : std::max(200.0, 140 + 1.4 * nb), end = 14.0 * nb;
+      const double block = f32 ? 250 + 3.5 * nb : cg == 2 ? std::max(200.0, 1.1 * nb) : std::max(200.0, 140 + 1.4 * nb), end = 14.0 * nb;
       for (int cut = 1; cut <= 8; cut *= 2) {
         if (cut > 1 && (cg == 2 || kb < 4 * cut || nb / 8 < cut || nb > lin_max_nb(elem, true))) break;
         // clusters of 4 and 8 CTAs that take whole multiprocessors do not fill the processing clusters: 33 and 15 of them on 148

@@ -19,14 +19,25 @@ __device__ __forceinline__ float linear_act(float x, int act) {
   return x;
 }
 
-// x in 32 bits as two tf32 operands, of which the tensor cores take the upper 19 bits: hi is x as it is, cut off there; lo what that leaves,
-// 13 bits of which 11 count.  What lo loses makes an operand smaller by some 1e-7 of itself; rounding it instead would take three more
-// instructions per element, and the splitting of a stage takes as long as its products.  Of an infinity lo is NaN.
-__device__ __forceinline__ uint32_t tf32_rest(uint32_t x) { return __float_as_uint(__uint_as_float(x) - __uint_as_float(x & 0xffffe000u)); }
-__device__ __forceinline__ void split_tf32(uint32_t x, uint32_t& hi, uint32_t& lo) {
-  hi = x;
-  lo = tf32_rest(x);
+// x in 32 bits as two tf32 operands (11 bits of mantissa; the tensor cores ignore what lies below), whose product with another one's leaves out lo lo.
+// hi is x rounded to the nearest, so that lo has either sign and is 2^-11 of x at most: what is left out is small and has no side.  (An infinity's hi is the
+// largest number, its lo the infinity; a NaN's are both NaN.)
+__device__ __forceinline__ uint32_t tf32_near(float x) {
+  uint32_t r;
+  asm("cvt.rn.satfinite.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
+  return r;
 }
+// lo has up to 13 bits, of which the tensor cores cut off those below 11: a little more, half a step where the mantissa is 1.5, makes that a rounding,
+// off to either side as often.
+__device__ __forceinline__ uint32_t tf32_less_cut(float lo) { return __float_as_uint(fmaf(lo, 1.0f / 3072.0f, lo)); }
+__device__ __forceinline__ void split_tf32(uint32_t x, uint32_t& hi, uint32_t& lo) {
+  hi = tf32_near(__uint_as_float(x));
+  lo = tf32_less_cut(__uint_as_float(x) - __uint_as_float(hi));
+}
+// ... where x stays as it is and hi is what the tensor cores leave of it.  One factor of a product may be split so: its lo is up to 2^-10 of x, with x's
+// sign, but what is left out has the other factor's.  (With both hi parts cut off, and lo, sums of positive products came out 2.7e-7 too small, of
+// numbers just below 1 + 2^-10 1.3e-6; now 0.5e-7.)  Of an infinity: NaN.
+__device__ __forceinline__ uint32_t tf32_rest(uint32_t x) { return tf32_less_cut(__uint_as_float(x) - __uint_as_float(x & 0xffffe000u)); }
 
 // 16 bytes of a row from element k on, zeros from K on.  Rows that lie on 16 bytes with K a multiple of a vector: one load.
 template <class T, bool ALIGNED>

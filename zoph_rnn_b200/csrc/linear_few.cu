@@ -3,8 +3,8 @@
 // A CTA computes 16 outputs x up to 32 columns, its eight warps an eighth of the K axis each.  A lane reads 16 consecutive bytes of a weight row and of a
 // column: which K indices it holds does not matter as long as both operands agree, so the fragments of a product are what the
 // loads bring, without a pass through shared memory (m16n8k16 in 16 bits: 8 elements are two k-steps' halves; m16n8k8 in tf32: 4 elements
-// are two k-steps).  32-bit operands are split into tf32 parts, hi and rest, for three products; the sums of four chunks are added in
-// ordinary 32-bit arithmetic, since the tensor core cuts its sums off.  What bounds a call is the latency of a warp's loads, a dozen chunks one
+// are two k-steps).  32-bit operands are split into tf32 parts, both rounded, for three products; the sums of four chunks (two of
+// more than 8 columns) are added in ordinary 32-bit arithmetic, since the tensor core cuts its sums off.  What bounds a call is the latency of a warp's loads, a dozen chunks one
 // after the other; where there are few outputs and a long K axis, up to 8 CTAs of a cluster share it (245 x 7429 bf16, 3 columns, rows that
 // start anywhere: 27 us on 16 CTAs, so 9).
 #include <cooperative_groups.h>
