@@ -142,6 +142,34 @@ def test_beam_select_refuses_a_small_workspace():
             refused(L.zrnn_beam_select(0, FAR[0], 40000, None, FAR[1], None, 1, 12, 40000, 12, 1, FAR[2], FAR[3], FAR[4], w, k, None), "workspace", str(n))
 
 
+# A workspace that is null, too short by a byte or not aligned; each size asks for one, so that the checks are reached.
+@pytest.mark.parametrize("elem", [0, 1, 2])
+def test_linear_refuses_a_workspace_that_does_not_do(elem):
+    L = _lib.lib()
+    n = size_of(L.zrnn_linear_workspace, elem, 4096, 2048, 333, FAR[0], 333, FAR[1], 333)
+    assert n >= (4096 + 2048) * 333 * (4 if elem == 0 else 2)  # (both operands are moved)
+    for w, k in ((None, n), (P, n - 1), (P, 0), (at(16), n), (at(128), n)):
+        refused(L.zrnn_linear(elem, 0, 4096, 2048, 333, FAR[0], 333, FAR[1], 333, None, None, 0, FAR[2], 4096, w, k, None), "workspace", str(n))
+
+
+@pytest.mark.parametrize("elem, n_sent, beam, V", [(0, 1, 25, 190003), (0, 3, 25, 190003), (1, 2, 50, 200000), (2, 1, 3, 3000001)])
+def test_beam_select_refuses_a_workspace_that_does_not_do(elem, n_sent, beam, V):
+    L = _lib.lib()
+    n = size_of(L.zrnn_beam_select_workspace, elem, n_sent, beam, V, 12)
+    assert n >= n_sent * 2 * 12 * 8  # (lists of two CTAs at least)
+    for w, k in ((None, n), (P, n - 1), (P, 0), (at(8), n)):
+        refused(L.zrnn_beam_select(elem, FAR[0], V, None, FAR[1], None, n_sent, beam, V, 12, 1, FAR[2], FAR[3], FAR[4], w, k, None), "workspace", str(n))
+
+
+@pytest.mark.parametrize("B, cols, S, heads, d", [(1, 12, 1 << 20, 1, 512), (2, 3, 4000, 2, 64), (3, 4, 4000, 1, 264)])
+def test_memory4_attend_refuses_a_workspace_that_does_not_do(B, cols, S, heads, d):
+    L = _lib.lib()
+    n = size_of(L.zrnn_memory4_attend_workspace, B, cols, S, heads, d)
+    assert n >= 2 * B * 16 * d * 4  # (two parts of a source column at least)
+    for w, k in ((None, n), (P, n - 1), (P, 0), (at(4), n)):
+        refused(L.zrnn_memory4_attend(0, P, P, B, S, heads, d, P, None, FAR[0], heads * d, cols, None, 1.0, FAR[1], heads * d, w, k, None), "workspace", str(n))
+
+
 def reorder(src, dst, sizes, n_cols=12, n_src=12, group=12, parents=P):
     k = len(src)
     return _lib.lib().zrnn_beam_reorder(k, (ctypes.c_void_p * k)(*[getattr(s, "value", s) for s in src]), (ctypes.c_void_p * k)(*[getattr(s, "value", s) for s in dst]),
