@@ -436,7 +436,7 @@ int zrnn_linear(int elem, int act, int n_rows, int n_cols, int K, const void* d_
  * hypothesis j of the sentence; the candidate (j, v) is worth d_scores[r] + (d_logp[r][v] - d_lse[r]), each operation rounded
  * to fp32 (d_lse NULL: log-probabilities).  A hypothesis with d_done[r] != 0 (NULL: none) has one candidate, (j, eos), worth
  * d_scores[r].  A NaN or -inf is no candidate.  Outputs [n_sent][k], best first, equal ones by j and then v: value, word v, and
- * parent = r as zrnn_beam_reorder takes it; where a sentence has fewer than k candidates: -inf, -1, -1.  k <= 64. */
+ * parent = r as zrnn_beam_reorder takes it; where a sentence has fewer than k candidates: -inf, -1, -1.  k <= 64, beam <= 2^25. */
 int zrnn_beam_select_workspace(int elem, int n_sent, int beam, int V, int k, size_t* bytes);
 int zrnn_beam_select(int elem, const void* d_logp, long long ld, const float* d_lse, const float* d_scores, const int* d_done,
                      int n_sent, int beam, int V, int k, int eos, float* d_score_out, int* d_word_out, int* d_parent_out,

@@ -170,6 +170,16 @@ def test_memory4_attend_refuses_a_workspace_that_does_not_do(B, cols, S, heads, 
         refused(L.zrnn_memory4_attend(0, P, P, B, S, heads, d, P, None, FAR[0], heads * d, cols, None, 1.0, FAR[1], heads * d, w, k, None), "workspace", str(n))
 
 
+def test_beam_select_of_more_than_2_to_the_25_hypotheses_is_refused():
+    """(The merge keeps a byte per list, and a list has 1024 rows at most, in shared memory.)"""
+    L = _lib.lib()
+    c = ctypes.c_size_t()
+    assert L.zrnn_beam_select_workspace(0, 1, 1 << 25, 1, 1, ctypes.byref(c)) == _lib.OK and c.value == (1 << 15) * 8
+    refused(L.zrnn_beam_select_workspace(0, 1, (1 << 25) + 1, 1, 1, ctypes.byref(c)), "hypotheses")
+    refused(L.zrnn_beam_select(0, FAR[0], 1, None, FAR[1], None, 1, (1 << 25) + 1, 1, 1, 1, FAR[2], FAR[3], FAR[4], None, 0, None), "hypotheses")
+    assert L.zrnn_beam_select_workspace(0, 1 << 28, 1, 1, 1, ctypes.byref(c)) == _lib.OK and c.value == 0
+
+
 def reorder(src, dst, sizes, n_cols=12, n_src=12, group=12, parents=P):
     k = len(src)
     return _lib.lib().zrnn_beam_reorder(k, (ctypes.c_void_p * k)(*[getattr(s, "value", s) for s in src]), (ctypes.c_void_p * k)(*[getattr(s, "value", s) for s in dst]),

@@ -763,6 +763,17 @@ def test_beam_select_of_one_outstanding_candidate_per_segment(api, n, beam, V, k
         assert torch.equal(got[:, :m], val) and torch.equal((parent[:, :m].long() - first) * V + word[:, :m], cand)
 
 
+@pytest.mark.parametrize("beam, V, k", [(5_100_000, 2, 1), (5_050_000, 1, 1), (600_000, 2, 64)])
+def test_beam_select_of_millions_of_hypotheses(api, beam, V, k):
+    """A segment per row: thousands of lists to merge."""
+    g = gen(beam)
+    z, scores = randn(g, beam, V), -20 + 3 * randn(g, beam)
+    val, word, parent = api.beam_select(z, scores, beam, k)
+    cand = (scores[:, None] + z).view(-1)
+    want, at = torch.sort(cand, descending=True, stable=True)
+    assert torch.equal(val[0], want[:k]) and torch.equal(parent[0].long() * V + word[0], at[:k])
+
+
 def test_beam_select_on_rows_that_start_anywhere(api):
     g = gen(6)
     for dtype in ref.TYPES:

@@ -326,7 +326,9 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 4 : 1) beam_select_kernel(cons
 
 // The parts' lists, each sorted, of a sentence.  What fits into shared memory is brought there; the keys that reach a bound for the k-th best (at
 // least k heads do) are ranked.  Where there are too many of those (ties), or the lists are too long: k rounds for the largest head.
-constexpr int kMergeThreads = 256, kMergeKeys = 5000, kMergeRank = 512;
+// (A byte per list as well: both fit into the 48 KB that need no asking, 2^15 lists, of 2^25 rows of a segment each, without the keys.)
+constexpr int kMergeThreads = 256, kMergeKeys = 4800, kMergeRank = 512;
+static_assert(kMergeKeys * 9 + kMergeRank * 8 + 1024 <= 48 * 1024 && (1 << 15) + kMergeRank * 8 + 1024 <= 48 * 1024, "");
 __global__ void __launch_bounds__(kMergeThreads) beam_select_merge_kernel(const BeamSelect a, int parts) {
   extern __shared__ __align__(16) unsigned long long s_keys[];  // the keys, if they fit; then per list how many are gone
   __shared__ unsigned long long s_cand[kMergeRank];
@@ -441,9 +443,9 @@ void select_plan(int elem, int n_sent, int beam, int V, int k, SelectPlan* pl) {
   const int vec = 32 * 16 / elem_bytes(elem), sms = device_sms();
   auto segs = [&](int u) { return (long long)(V + 16 / elem_bytes(elem) - 2) / (vec * u) + 1; };
   int C = 1;
-  pl->NT = n_sent * kSelCluster * 2 > sms * 4 ? 256 : 1024;
+  pl->NT = (long long)n_sent * kSelCluster * 2 > sms * 4 ? 256 : 1024;
   const int slots = pl->NT == 256 ? 4 * sms : sms;
-  while (C < kSelCluster && n_sent * 2 * C <= slots) C *= 2;
+  while (C < kSelCluster && (long long)n_sent * 2 * C <= slots) C *= 2;
   while (C < kSelCluster && segs(4) * beam > (long long)C * kSelSegs) C *= 2;
   pl->parts = 1;
   pl->U = 4;

@@ -3239,6 +3239,7 @@ static int select_args(const char* what, int elem, int n_sent, int beam, int V, 
   ZR_CHECK(elem >= ZRNN_ELEM_F32 && elem <= ZRNN_ELEM_F16, std::string(what) + ": unknown element type");
   ZR_CHECK(n_sent >= 0 && beam >= 1 && V >= 1, std::string(what) + ": sizes must be positive");
   ZR_CHECK((long long)beam * V <= 0x7fff0000 && (long long)n_sent * beam <= 0x7fffffff, std::string(what) + ": too many candidates");
+  ZR_CHECK(beam <= (1 << 25), std::string(what) + ": more than 2^25 hypotheses of a sentence");
   ZR_CHECK(k >= 1 && k <= zrnn::kSelectMax && k <= (long long)beam * V, std::string(what) + ": k must be in [1,64] and at most beam * V");
   return ZRNN_OK;
 }
