@@ -139,3 +139,14 @@ def test_a_splitting_team_waits_until_a_stages_last_round_is_used_up():
     launch = body("linear.cu", "cudaError_t lin_launch(", "cudaLaunchKernelEx")
     assert "(512 - 4 * p.nb) / 32" in launch and re.search(r"return mode == LIN_F32 \? 96", body("linear.cu", "lin_max_nb(", "\n"))
     assert (512 - 4 * 96) // 32 >= 3 and "kSplitTeams = 3" in body("linear.cu", "constexpr int kEpiWarps", ";")
+
+
+def test_a_product_whose_wait_gave_up_waits_for_its_copies():
+    """Every role of the product that requests copies, the epilogue's residual among them, lets them land before its CTA may retire."""
+    s = body("linear.cu", "linear_tc_kernel(const __grid_constant__", "linear_align_kernel")
+    load, rest = s[s.index("warp == kLoadWarp"):].split("else if (warp == kMmaWarp)", 1)
+    mma, rest = rest.split("else if (warp < kEpiWarps)", 1)
+    epilogue = rest[:rest.index("} else if (F32) {")]
+    assert "if (sound && !ok) settle_copies();" in load and "if (!ok) settle_copies();" in mma
+    assert "bring_residual(" in epilogue
+    assert re.search(r"if \(BULK && p\.bulk && a\.R && one && sound && !ready\) settle_copies\(\);", epilogue[epilogue.index("bulk.wait_group 0"):])

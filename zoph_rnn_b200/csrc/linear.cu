@@ -352,6 +352,7 @@ __global__ void __launch_bounds__(lin_threads(MODE), 1) linear_tc_kernel(const _
       __syncwarp();
     }
     if (BULK && p.bulk && one) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    if (BULK && p.bulk && a.R && one && sound && !ready) settle_copies();  // (a residual may still be on its way)
   } else if (F32) {
     // ------------------------------------------------------------ the lo parts of a stage: what tf32 cuts off of the tile beside it
     // Teams of four warps take the k-blocks in turn: one's waits are filled by the others.  A stage's next user may be another team, and copies may arrive out
