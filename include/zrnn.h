@@ -407,7 +407,8 @@ int zrnn_memory4_unpack(int elem, const void* d_codes, const void* d_scales, int
  * belongs to source column c / cols_per_sentence, and per head
  *   out = sum_s softmax_s(scale * q . v_s) v_s   over the slots offset <= s < offset + len of that source column
  * (slots outside the memory do not count; d_offset NULL: 0).  Whatever other slots hold is not looked at.  A column without
- * slots, or with d_mask01[c] == 0 (NULL: all 1), gets zeros.  d <= 1024.  d_out must not overlap d_q.  Scores have to stay below
+ * slots, or with d_mask01[c] == 0 (NULL: all 1), gets zeros.  d <= 1024.  d_out must not overlap d_q
+ * (columns of one wider matrix, side by side, do not).  Scores have to stay below
  * 2^127.  The weights go into their sums, and into those of the values, rounded to 22 bits (bf16: 11), and to steps of 2^-31 of the largest
  * one beside them (32 bits: 2^-42).  An element of a query counts with its type's precision (22 bits in 32 bits) down to 2^-28 of
  * the largest of its column and head, and with steps of 2^-40 of that (32 bits: 2^-50) below. */
@@ -418,7 +419,8 @@ int zrnn_memory4_attend(int elem, const void* d_codes, const void* d_scales, int
 
 /* Y = act(W X + b) + R for n_cols columns: X (K x n_cols), Y and R (n_rows x n_cols) column-major as all activations; the K
  * weights of an output are contiguous and those of the next ldw further (W^T column-major).  d_bias (n_rows, fp32) and
- * d_residual may be NULL; d_residual may be d_Y itself (with ldr == ldy).  ZRNN_ELEM_F32 is 3xTF32:
+ * d_residual may be NULL; d_residual may be d_Y itself (with ldr == ldy); d_Y must not overlap anything else (columns of one wider
+ * matrix, side by side, do not).  ZRNN_ELEM_F32 is 3xTF32:
  * every product within 2^-20 of itself (1.2e-7 on the average, without a side), its sums cut off now and then by the tensor core (together some
  * 3.5e-7 of the root of the sum of the products' squares; 6e-7 too small where all products are positive; a sum in plain fp32 is off by
  * 4e-7 over 512 of them).  An infinity among its operands may make NaN.  The 16-bit types multiply their operands as they are and add in

@@ -180,6 +180,26 @@ def test_beam_select_of_more_than_2_to_the_25_hypotheses_is_refused():
     assert L.zrnn_beam_select_workspace(0, 1 << 28, 1, 1, 1, ctypes.byref(c)) == _lib.OK and c.value == 0
 
 
+def byte(p, k):
+    return ctypes.c_void_p(p.value + k)
+
+
+# (on a machine without a device the calls that are let through end there)
+@pytest.mark.parametrize("shift, ld, fits", [(128, 64, True), (127 * 4, 160, True), (32 * 4, 160, True), (31 * 4, 160, False), (129 * 4, 160, False), (0, 160, False), (160 * 4 * 2, 160, False), (160 * 4 * 2 + 32 * 4, 160, True), (-128 * 4, 160, True)])
+def test_columns_of_one_wider_matrix_do_not_overlap(shift, ld, fits):
+    """Queries and outputs, or operands and outputs, side by side in one matrix; columns that share an element are refused."""
+    L = _lib.lib()
+    for call in (lambda q, o: L.zrnn_memory4_attend(0, P, P, 3, 8, 1, 32, P, None, q, ld, 2, None, 1.0, o, ld, None, 0, None),
+                 lambda x, y: L.zrnn_linear(0, 0, 32, 6, 32, FAR[3], 32, x, ld, None, None, 0, y, ld, None, 0, None),
+                 lambda r, y: L.zrnn_linear(0, 0, 32, 6, 32, FAR[3], 32, FAR[4], 32, None, r, ld, y, ld, None, 0, None) if shift else _lib.E_ARG):
+        status = call(FAR[0], byte(FAR[0], shift))
+        assert (status != _lib.E_ARG) == fits, (status, L.zrnn_last_error())
+    # a single column within another matrix's; other strides are not looked into
+    one = L.zrnn_linear(0, 0, 32, 1, 32, FAR[3], 32, FAR[0], 32, None, byte(FAR[0], 0), 64, byte(FAR[0], 32 * 4), 999, None, 0, None)
+    assert one != _lib.E_ARG
+    refused(L.zrnn_linear(0, 0, 32, 6, 32, FAR[3], 32, FAR[0], 96, None, None, 0, byte(FAR[0], 128), 160, None, 0, None), "overlaps")
+
+
 def reorder(src, dst, sizes, n_cols=12, n_src=12, group=12, parents=P):
     k = len(src)
     return _lib.lib().zrnn_beam_reorder(k, (ctypes.c_void_p * k)(*[getattr(s, "value", s) for s in src]), (ctypes.c_void_p * k)(*[getattr(s, "value", s) for s in dst]),

@@ -1086,6 +1086,32 @@ def test_many_sentences(api):
     check_attend(out[at], v, f64(q)[at], lens.cpu().numpy()[at], [0] * 6, 1.0, "f32")
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_operands_and_outputs_side_by_side_in_one_matrix(api, dtype):
+    """[context; state] without a copy: the attention writes one half of the combiner's input, whose other half are its queries."""
+    g = gen(77)
+    for n_src, cols, H, n in ((3, 4, 100, 60), (2, 150, 256, 256), (5, 3, 72, 300)):
+        N = n_src * cols
+        m = api.memory4(n_src, 40, H).pack(torch.tanh(randn(g, 40, n_src, H, dtype=dtype)))
+        lens = torch.randint(1, 41, (n_src,), generator=g, device="cuda", dtype=torch.int32)
+        both = randn(g, N, 2 * H + n, dtype=dtype)
+        keep = both.clone()
+        m.attend(both[:, H:2 * H], lens, out=both[:, :H])
+        assert torch.equal(both[:, :H], m.attend(keep[:, H:2 * H].contiguous(), lens)) and torch.equal(both[:, H:], keep[:, H:])
+        W = randn(g, n, 2 * H, dtype=dtype) * 0.1
+        # (another stride may mean another kernel: the sums of both stray from the exact one, and may be rounded to either side)
+        off = 2 * sum_tol(2 * H) * (both[:, :2 * H].double().abs() @ W.double().abs().t()) + 32 * EPS
+        want = api.linear(W, both[:, :2 * H].contiguous(), act="tanh")
+        api.linear(W, both[:, :2 * H], act="tanh", out=both[:, 2 * H:])
+        assert bool(((both[:, 2 * H:].double() - want.double()).abs() <= off + 2 * ref.HALF_STEP[dtype]).all())
+        assert torch.equal(both[:, H:2 * H], keep[:, H:2 * H])
+        pair = randn(g, N, 2 * n, dtype=dtype)
+        R = pair[:, n:].clone()
+        api.linear(W, both[:, :2 * H], residual=pair[:, n:], out=pair[:, :n])
+        again = api.linear(W, both[:, :2 * H], residual=R)
+        assert torch.equal(pair[:, n:], R) and bool(((pair[:, :n].double() - again.double()).abs() <= off + 2 * ref.HALF_STEP[dtype] * (again.double().abs() + off)).all())
+
+
 def test_rows_that_overlap_are_refused(api):
     one = torch.zeros(1, 64, device="cuda")
     W = torch.zeros(8, 64, device="cuda")

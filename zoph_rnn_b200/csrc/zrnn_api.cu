@@ -3114,6 +3114,19 @@ struct Span {
 };
 // elements from the first one of a strided matrix to its last
 long long extent(long long cols, long long ld, long long width) { return cols > 0 ? (cols - 1) * ld + width : 0; }
+// columns of `width` elements, ld apart.  Those of two matrices with one ld may lie between one another, as parts of one wider matrix do.
+struct Columns : Span {
+  long long n, ld, width;  // bytes
+  Columns(const void* p, long long cols, long long ld_, long long width_, int eb)
+      : Span(p, extent(cols, ld_, width_), eb), n(cols), ld(ld_ * eb), width(width_ * eb) {}
+  bool meets(const Columns& o) const {
+    if (!Span::meets(o)) return false;
+    const long long step = n == 1 ? o.ld : ld;
+    if (o.n != 1 && o.ld != step) return true;
+    const long long d = ((long long)(o.lo - lo) % step + step) % step;  // where the other's columns start, from the start of one of these
+    return d < width || d + o.width > step;
+  }
+};
 bool elem_aligned(const void* p, int elem) { return ((uintptr_t)p & (zrnn::elem_bytes(elem) - 1)) == 0; }
 
 }  // namespace
@@ -3175,7 +3188,7 @@ int zrnn_memory4_attend(int elem, const void* d_codes, const void* d_scales, int
   ZR_CHECK(elem_aligned(d_q, elem) && elem_aligned(d_out, elem) && ((uintptr_t)d_codes & 15) == 0 && ((uintptr_t)d_scales & 1) == 0,
            "memory4_attend: misaligned pointer (codes: 16 bytes)");
   const int eb = zrnn::elem_bytes(elem);
-  ZR_CHECK(!Span(d_q, extent(N, ld_q, width), eb).meets(Span(d_out, extent(N, ld_out, width), eb)), "memory4_attend: the output overlaps the queries");
+  ZR_CHECK(!Columns(d_q, N, ld_q, width, eb).meets(Columns(d_out, N, ld_out, width, eb)), "memory4_attend: the output overlaps the queries");
   const size_t need = zrnn::mem4_attend_work(B, cols_per_sentence, S_cap, heads, d) * sizeof(float);
   ZR_CHECK(need == 0 || (d_workspace && workspace_bytes >= need && ((uintptr_t)d_workspace & 15) == 0),
            "memory4_attend: the workspace must hold " + std::to_string(need) + " bytes (16-byte aligned)");
@@ -3215,11 +3228,11 @@ int zrnn_linear(int elem, int act, int n_rows, int n_cols, int K, const void* d_
   ZR_CHECK(ldy >= n_rows && ldy <= (1ll << 30) && (!d_residual || (ldr >= n_rows && ldr <= (1ll << 30))), "linear: bad leading dimension");
   ZR_CHECK(elem_aligned(d_Y, elem) && elem_aligned(d_residual, elem) && ((uintptr_t)d_bias & 3) == 0, "linear: misaligned pointer");
   const int eb = zrnn::elem_bytes(elem);
-  const Span y(d_Y, extent(n_cols, ldy, n_rows), eb);
-  ZR_CHECK(!y.meets(Span(d_W, extent(n_rows, ldw, K), eb)) && !y.meets(Span(d_X, extent(n_cols, ldx, K), eb)) &&
-               !(d_bias && y.meets(Span(d_bias, n_rows, 4))),
+  const Columns y(d_Y, n_cols, ldy, n_rows, eb);
+  ZR_CHECK(!y.meets(Columns(d_W, n_rows, ldw, K, eb)) && !y.meets(Columns(d_X, n_cols, ldx, K, eb)) &&
+               !(d_bias && static_cast<const Span&>(y).meets(Span(d_bias, n_rows, 4))),
            "linear: the output overlaps an input");
-  ZR_CHECK(!d_residual || (d_residual == d_Y && ldr == ldy) || !y.meets(Span(d_residual, extent(n_cols, ldr, n_rows), eb)),
+  ZR_CHECK(!d_residual || (d_residual == d_Y && ldr == ldy) || !y.meets(Columns(d_residual, n_cols, ldr, n_rows, eb)),
            "linear: the output overlaps the residual without being it");
   zrnn::LinearArgs a;
   std::memset(&a, 0, sizeof(a));
