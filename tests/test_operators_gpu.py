@@ -943,6 +943,51 @@ def test_the_calls_allocate_nothing(api):
     assert torch.cuda.mem_get_info()[0] >= before
 
 
+def test_the_c_abi_allocates_nothing(api):
+    """Every call with the caller's buffers and workspaces, at sizes that need one: neither torch's allocator nor the device's free memory moves, from the
+    second call of a size on and for larger ones after it (the first loads the kernels)."""
+    L = api.lib()
+
+    def step(scale, run):
+        S, n, K, N, V = 4000 * scale, 512 * scale, 333, 512 * scale, 190003 * scale
+        f32 = dict(dtype=torch.float32, device="cuda")
+        t = dict(x=torch.zeros(S, 2, 64, **f32), q=torch.zeros(6, 64, **f32), ctx=torch.empty(6, 64, **f32), back=torch.empty(2, S, 64, **f32), W=torch.zeros(n * 8, K, **f32), X=torch.zeros(N * 4, K, **f32),
+                 Y=torch.empty(N * 4, n * 8, **f32), z=torch.zeros(25, V, **f32), s=torch.zeros(25, **f32), val=torch.empty(12, **f32), moved=torch.empty(12, 100, **f32), state=torch.zeros(25, 100, **f32),
+                 codes=torch.empty(2, S, 1, 32, dtype=torch.uint8, device="cuda"), scales=torch.empty(2, S, 1, 2, dtype=torch.float16, device="cuda"), lens=torch.full((2,), S, dtype=torch.int32, device="cuda"),
+                 word=torch.empty(12, dtype=torch.int32, device="cuda"), parent=torch.empty(12, dtype=torch.int32, device="cuda"))
+        p = {k: v.data_ptr() for k, v in t.items()}
+        sizes = [ctypes.c_size_t() for _ in range(3)]
+        assert L.zrnn_memory4_attend_workspace(2, 3, S, 1, 64, ctypes.byref(sizes[0])) == 0
+        assert L.zrnn_linear_workspace(0, n * 8, N * 4, K, p["W"], K, p["X"], K, ctypes.byref(sizes[1])) == 0
+        assert L.zrnn_beam_select_workspace(0, 1, 25, V, 12, ctypes.byref(sizes[2])) == 0
+        assert all(z.value > 0 for z in sizes)
+        work = [torch.empty(z.value, dtype=torch.uint8, device="cuda") for z in sizes]
+        st = torch.cuda.current_stream().cuda_stream
+
+        def calls():
+            one = lambda a: (ctypes.c_void_p * 1)(a)  # noqa: E731
+            assert [L.zrnn_memory4_pack(0, p["x"], 128, 64, S, 2, 1, 64, 0, S, p["codes"], p["scales"], st),
+                    L.zrnn_memory4_unpack(0, p["codes"], p["scales"], 2, S, 1, 64, 0, S, p["back"], st),
+                    L.zrnn_memory4_attend(0, p["codes"], p["scales"], 2, S, 1, 64, p["lens"], None, p["q"], 64, 3, None, 1.0, p["ctx"], 64, work[0].data_ptr(), sizes[0].value, st),
+                    L.zrnn_linear(0, 1, n * 8, N * 4, K, p["W"], K, p["X"], K, None, None, 0, p["Y"], n * 8, work[1].data_ptr(), sizes[1].value, st),
+                    L.zrnn_beam_select(0, p["z"], V, None, p["s"], None, 1, 25, V, 12, 1, p["val"], p["word"], p["parent"], work[2].data_ptr(), sizes[2].value, st),
+                    L.zrnn_beam_reorder(1, one(p["state"]), one(p["moved"]), (ctypes.c_size_t * 1)(400), p["parent"], 12, 25, 1, st)] == [0] * 6
+        if run:
+            calls()
+            torch.cuda.synchronize()
+        return t, work, calls
+
+    keep = step(1, True)
+    larger = step(2, False)
+    torch.cuda.synchronize()
+    before = torch.cuda.mem_get_info()[0], torch.cuda.memory_stats()["allocation.all.allocated"]
+    for calls in (keep[2], larger[2]) * 3:
+        calls()
+    torch.cuda.synchronize()
+    assert (torch.cuda.mem_get_info()[0], torch.cuda.memory_stats()["allocation.all.allocated"]) == before
+    assert L.zrnn_tc_error() == 0
+
+
 @pytest.mark.parametrize("dtype", [3, 0, 1, 4])  # exact fp32, fp16 split, bf16, 3xTF32
 @pytest.mark.parametrize("H, S, B, cols", [(64, 20, 3, 1), (320, 50, 5, 12), (1000, 33, 2, 4)])
 def test_attention_layer_over_a_source_in_4_bits(api, dtype, H, S, B, cols):
