@@ -19,7 +19,7 @@
 //
 // Long products of few tiles: 2, 4 or 8 CTAs of a cluster share a tile's K axis and exchange their sums through distributed shared memory.
 // 16-bit outputs and residuals of whole tiles go through shared memory and TMA.  us, this kernel / the library's product alone: bf16 16384 x
-// 4096 x 4096 350 / 337, 4096 x 4096 x 512 20 / 15, 512 x 8192 x 512 18 / 17, 1000 x 1000 x 64 7.8 / 4.7; fp32 16384 x 4096 x 4096
+// 4096 x 4096 350 / 337, 4096 x 4096 x 512 18.5 / 15.2, 512 x 8192 x 512 18 / 17, 1000 x 1000 x 64 6.5 / 3.9; fp32 16384 x 4096 x 4096
 // 2850 / 8400 (FMA), 1000 x 2000 x 768 23.6 / 83.
 //
 // A CTA asks for all of an SM's shared memory, so that a pair's allocation of tensor memory waits for nobody that could wait for it in turn.

@@ -66,7 +66,7 @@ __device__ __forceinline__ unsigned mem4_codes(const float (&x)[8], float s, flo
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 __device__ __forceinline__ __half2 bits_h2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
 // Nibbles 0 .. 3 of each half of x, as pairs (low half, high half) of q * s: 1024 + u and 1024 + 16 u are halves made by or-ing u into a
-// mantissa, and what follows is exact but for the last product, whose rounding is the definition's.
+// mantissa (a well-known way to make numbers of small whole ones), and what follows is exact but for the last product, whose rounding is the definition's.
 __device__ __forceinline__ void dequant4(uint32_t x, __half2 s, uint32_t (&v)[4]) {
   const __half2 m1032 = __half2half2(__ushort_as_half(0xe408)), sixteenth = __half2half2(__ushort_as_half(0x2c00)), m72 = __half2half2(__ushort_as_half(0xd480));
   const uint32_t y = x >> 8;
