@@ -29,7 +29,7 @@ __device__ __forceinline__ uint32_t tf32_near(float x) {
 }
 // lo has up to 13 bits, of which the tensor cores cut off those below 11: a little more, half a step where the mantissa is 1.5, makes that a rounding,
 // off to either side as often.
-__device__ __forceinline__ uint32_t tf32_less_cut(float lo) { return __float_as_uint(fmaf(lo, 1.0f / 3072.0f, lo)); }
+__device__ __forceinline__ uint32_t tf32_less_cut(float lo) { return __float_as_uint(fmaf(lo, 1.0f / 2048.0f / 1.5f, lo)); }
 __device__ __forceinline__ void split_tf32(uint32_t x, uint32_t& hi, uint32_t& lo) {
   hi = tf32_near(__uint_as_float(x));
   lo = tf32_less_cut(__uint_as_float(x) - __uint_as_float(hi));
